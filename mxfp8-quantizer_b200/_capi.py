@@ -44,6 +44,12 @@ EXPORTS = (
     "mxfp8_last_error",
 )
 
+# include/mxfp4.h
+FP4_EXPORTS = (
+    "mxfp4_quantize",
+    "mxfp4_dequantize",
+)
+
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 
@@ -77,6 +83,10 @@ def configure(L: ctypes.CDLL) -> ctypes.CDLL:
     L.mxfp8_strerror.restype = ctypes.c_char_p
     L.mxfp8_last_error.argtypes = []
     L.mxfp8_last_error.restype = ctypes.c_char_p
+    L.mxfp4_quantize.argtypes = [vp, i32, i64, i64, i64, vp, i64, vp, i64, vp]
+    L.mxfp4_quantize.restype = i32
+    L.mxfp4_dequantize.argtypes = [vp, i64, i64, i64, vp, i64, vp, i32, i64, vp]
+    L.mxfp4_dequantize.restype = i32
     if hasattr(L, "mxfp8_checked_window_slack"):
         L.mxfp8_checked_window_slack.argtypes = [i64]
         L.mxfp8_checked_window_slack.restype = i32
@@ -163,6 +173,20 @@ def dequantize(q_ptr: int, rows: int, cols: int, ld_q: int, s_ptr: int, s_bytes:
     rc = lib().mxfp8_dequantize(q_ptr or None, rows, cols, ld_q, s_ptr or None, s_bytes, out_ptr or None,
                                 out_dtype, ld_out, stream or None)
     check(rc, "dequantizer launch")
+
+
+def fp4_quantize(x_ptr: int, dtype: int, m: int, k: int, ld_x: int, q_ptr: int, ld_q: int, s_ptr: int, s_bytes: int,
+                 stream: int) -> None:
+    rc = lib().mxfp4_quantize(x_ptr or None, dtype, m, k, ld_x, q_ptr or None, ld_q, s_ptr or None, s_bytes,
+                              stream or None)
+    check(rc, "MXFP4 quantizer launch")
+
+
+def fp4_dequantize(q_ptr: int, rows: int, cols: int, ld_q: int, s_ptr: int, s_bytes: int, out_ptr: int,
+                   out_dtype: int, ld_out: int, stream: int) -> None:
+    rc = lib().mxfp4_dequantize(q_ptr or None, rows, cols, ld_q, s_ptr or None, s_bytes, out_ptr or None, out_dtype,
+                                ld_out, stream or None)
+    check(rc, "MXFP4 dequantizer launch")
 
 
 def device_status(clear: bool = False) -> int:

@@ -99,18 +99,6 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 std::atomic<int64_t> g_window_slack{0};
 #endif
 
-// The bytes [base, base + bytes) a kernel may write.  The checked build
-// narrows it by mxfp8_checked_window_slack bytes, to show that its store
-// guards fire; the product build ignores the window.
-StoreWindow make_window(void* base, int64_t bytes) {
-    uint8_t* lo = static_cast<uint8_t*>(base);
-#ifdef MXFP8_CHECKED
-    bytes -= g_window_slack.load(std::memory_order_relaxed);
-    if (bytes < 0) bytes = 0;
-#endif
-    return StoreWindow{lo, lo + bytes};
-}
-
 // Argument checks and problem description shared by both quantize entries,
 // so the two keep one contract.  Returns 0 or a negative status; *launch is
 // false when there is nothing to write (q_rows or q_cols == 0).
@@ -149,6 +137,23 @@ int make_quantize_args(const void* x, int dtype, int64_t m, int64_t k, int64_t l
 }
 
 }  // namespace
+
+StoreWindow make_window(void* base, int64_t bytes) {
+    uint8_t* lo = static_cast<uint8_t*>(base);
+#ifdef MXFP8_CHECKED
+    bytes -= g_window_slack.load(std::memory_order_relaxed);
+    if (bytes < 0) bytes = 0;
+#endif
+    return StoreWindow{lo, lo + bytes};
+}
+
+int ready_device(int* sm_count, unsigned int** status) {
+    DeviceState* dev = nullptr;
+    if (int rc = current_device(&dev)) return rc;
+    *sm_count = dev->sm_count;
+    *status = dev->status;
+    return MXFP8_OK;
+}
 
 // A key of the CUDA context current on this host thread, unique for the
 // process's lifetime (cuCtxGetId: never reused, unlike the handle), or 0 if

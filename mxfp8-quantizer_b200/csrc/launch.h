@@ -34,6 +34,31 @@ int launch_dequantize(const uint8_t* q, int64_t rows, int64_t cols, int64_t ld_q
 
 int launch_bounded_wait_selftest(unsigned int* status, uint32_t limit_us, cudaStream_t stream);
 
+// Problem description of an MXFP4 quantization after argument validation.
+struct Fp4QuantizeArgs {
+    const void* x;
+    int dtype;
+    int64_t m, k, ld_x;
+    uint8_t* q;
+    int64_t q_cols, ld_q;  // columns rounded up to 32, row stride in bytes
+    uint8_t* s;
+    unsigned int* status;
+    StoreWindow qw, sw;
+};
+
+int launch_mxfp4_quantize(const Fp4QuantizeArgs& a, cudaStream_t stream);
+int launch_mxfp4_dequantize(const uint8_t* q, int64_t rows, int64_t cols, int64_t ld_q, const uint8_t* s, void* out,
+                            int out_dtype, int64_t ld_out, StoreWindow ow, unsigned int* status, cudaStream_t stream);
+
+// SM count and device error word of the current device (made ready by the
+// first call on it); 0 or a negative mxfp8_status.
+int ready_device(int* sm_count, unsigned int** status);
+
+// The bytes [base, base + bytes) a kernel may write.  The checked build
+// narrows it by mxfp8_checked_window_slack bytes, to show that its store
+// guards fire; the product build ignores the window.
+StoreWindow make_window(void* base, int64_t bytes);
+
 // Records the CUDA error text for mxfp8_last_error() on this host thread.
 void set_last_error(const char* what, int code);
 

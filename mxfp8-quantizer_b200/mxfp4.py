@@ -1,0 +1,85 @@
+"""4-bit microscaling beside the MXFP8 quantizer: quantize, dequantize and the
+product of two MXFP4 matrices (C ABI in include/mxfp4.h).
+
+An MXFP4 matrix is a pair ``(q, s)``: ``q`` (rows, cols / 2) uint8 holds two
+E2M1 codes a byte (the even column in the low four bits), ``s`` one UE8M0 byte
+per 1x32 block along the columns, in the chunk layout of
+``packed_scale_storage_bytes(rows, cols)`` that ``quantize`` writes too.  The
+reference quantizes to E4M3 only, so nothing here has a counterpart there.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _capi
+from ._launch import in_dtype, on_stream, out_dtype_code
+
+FP4_E2M1_MAX = 6.0
+_PAYLOAD_DTYPES = (torch.uint8, torch.int8, torch.float4_e2m1fn_x2)
+
+
+def _check_payload(name: str, q: torch.Tensor) -> tuple[int, int]:
+    """(rows, cols) of an MXFP4 payload."""
+    if q.dim() != 2 or q.dtype not in _PAYLOAD_DTYPES or (q.stride(1) != 1 and q.shape[1] > 1):
+        raise ValueError(f"{name} must be a row-major matrix of bytes, got {tuple(q.shape)} {q.dtype}")
+    if q.shape[1] % 16:
+        raise ValueError(f"{name} must have a multiple of 32 columns (16 bytes), got {2 * q.shape[1]}")
+    return q.shape[0], 2 * q.shape[1]
+
+
+def _check_scales(name: str, s: torch.Tensor) -> None:
+    """The library checks the size."""
+    if s.element_size() != 1 or not s.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous buffer of bytes")
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Row stride, also of a matrix whose single row carries none."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def quantize_mxfp4(x: torch.Tensor, q: torch.Tensor | None = None, s: torch.Tensor | None = None, stream=None):
+    """Quantize a CUDA (m, k) bf16/fp16 tensor to MXFP4; returns (q, s).
+
+    The scale of a block is the smallest power of two that keeps its largest
+    magnitude within 6, the codes are rounded to nearest (ties to even); a
+    block that holds an inf or a NaN decodes to NaN.  Columns are padded with
+    zeros to a multiple of 32.  ``x`` may have any row stride and offset; one
+    whose last dimension is not contiguous is copied first.  Preallocated
+    ``q`` (m, ceil(k/32)*16) and ``s`` are written in place."""
+    if x.dim() != 2:
+        raise ValueError(f"X must be 2-D, got shape {tuple(x.shape)}")
+    code = in_dtype("X", x.dtype)
+    m, k = x.shape
+    q_cols = -(-k // 32) * 32
+    given = [t for t in (q, s) if t is not None]
+    context, handle = on_stream(stream, x, *given)
+    with context:
+        if (x.stride(1) != 1 and k > 1) or (m > 1 and x.stride(0) < k):
+            x = x.contiguous()
+        if q is None:
+            q = torch.empty((m, q_cols // 2), dtype=torch.uint8, device=x.device)
+        elif _check_payload("q", q) != (m, q_cols):
+            raise ValueError(f"q must be ({m}, {q_cols // 2}) bytes, got {tuple(q.shape)}")
+        need = -(-m // 128) * 128 * (-(-q_cols // 128) * 4)
+        if s is None:
+            s = torch.empty((need,), dtype=torch.uint8, device=x.device)
+        else:
+            _check_scales("s", s)
+        _capi.fp4_quantize(x.data_ptr(), code, m, k, _row_stride(x), q.data_ptr(), _row_stride(q), s.data_ptr(),
+                           s.numel(), handle)
+    return q, s
+
+
+def dequantize_mxfp4(q: torch.Tensor, s: torch.Tensor, out_dtype: torch.dtype = torch.float32, stream=None):
+    """MXFP4 payload + packed UE8M0 scales -> out_dtype (bf16, fp16 or fp32)."""
+    rows, cols = _check_payload("q", q)
+    _check_scales("s", s)
+    code = out_dtype_code(out_dtype)
+    context, handle = on_stream(stream, q, s)
+    with context:
+        out = torch.empty((rows, cols), dtype=out_dtype, device=q.device)
+        _capi.fp4_dequantize(q.data_ptr(), rows, cols, _row_stride(q), s.data_ptr(), s.numel(), out.data_ptr(), code,
+                             cols, handle)
+    return out
