@@ -41,6 +41,21 @@ MXFP8_API int mxfp4_quantize(const void* x, int dtype, int64_t m, int64_t k, int
 MXFP8_API int mxfp4_dequantize(const void* q, int64_t rows, int64_t cols, int64_t ld_q, const void* s,
                                int64_t s_bytes, void* out, int out_dtype, int64_t ld_out, mxfp8_stream_t stream);
 
+/* out (m, n) of out_dtype (MXFP8_BF16, MXFP8_FP16 or MXFP8_F32), row stride
+ * ld_out elements = A B^T for the MXFP4 matrices A (m, k) and B (n, k),
+ * k % 32 == 0: products of E2M1 values scaled by both blocks' powers of two,
+ * summed in f32 on the tensor cores, rounded once.  A block whose scale byte is
+ * 255 makes its row of A (its row of B) give NaN in every output that it meets.
+ * Padding scale bytes must not be 255 (mxfp4_quantize writes 0).  out is
+ * aligned to its element; it must not overlap the operands.  k == 0 gives
+ * zeros.  Any m from single tokens to long prefills; the sum's order depends on
+ * the sizes and the device alone, so equal calls give equal bits.  A pipeline
+ * wait that runs out (about 1 s) sets bit 32 of the device status word
+ * (mxfp8_device_status). */
+MXFP8_API int mxfp4_gemm(const void* a_q, int64_t m, int64_t ld_a, const void* a_s, int64_t a_s_bytes,
+                         const void* b_q, int64_t n, int64_t ld_b, const void* b_s, int64_t b_s_bytes, int64_t k,
+                         void* out, int out_dtype, int64_t ld_out, mxfp8_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -48,6 +48,7 @@ EXPORTS = (
 FP4_EXPORTS = (
     "mxfp4_quantize",
     "mxfp4_dequantize",
+    "mxfp4_gemm",
 )
 
 _lock = threading.Lock()
@@ -87,6 +88,8 @@ def configure(L: ctypes.CDLL) -> ctypes.CDLL:
     L.mxfp4_quantize.restype = i32
     L.mxfp4_dequantize.argtypes = [vp, i64, i64, i64, vp, i64, vp, i32, i64, vp]
     L.mxfp4_dequantize.restype = i32
+    L.mxfp4_gemm.argtypes = [vp, i64, i64, vp, i64, vp, i64, i64, vp, i64, i64, vp, i32, i64, vp]
+    L.mxfp4_gemm.restype = i32
     if hasattr(L, "mxfp8_checked_window_slack"):
         L.mxfp8_checked_window_slack.argtypes = [i64]
         L.mxfp8_checked_window_slack.restype = i32
@@ -187,6 +190,13 @@ def fp4_dequantize(q_ptr: int, rows: int, cols: int, ld_q: int, s_ptr: int, s_by
     rc = lib().mxfp4_dequantize(q_ptr or None, rows, cols, ld_q, s_ptr or None, s_bytes, out_ptr or None, out_dtype,
                                 ld_out, stream or None)
     check(rc, "MXFP4 dequantizer launch")
+
+
+def fp4_gemm(a_ptr: int, m: int, ld_a: int, a_s_ptr: int, a_s_bytes: int, b_ptr: int, n: int, ld_b: int, b_s_ptr: int,
+             b_s_bytes: int, k: int, out_ptr: int, out_dtype: int, ld_out: int, stream: int) -> None:
+    rc = lib().mxfp4_gemm(a_ptr or None, m, ld_a, a_s_ptr or None, a_s_bytes, b_ptr or None, n, ld_b, b_s_ptr or None,
+                          b_s_bytes, k, out_ptr or None, out_dtype, ld_out, stream or None)
+    check(rc, "MXFP4 product launch")
 
 
 def device_status(clear: bool = False) -> int:

@@ -23,8 +23,8 @@ CSRC = PKG / "csrc"
 LIB = PKG / "libmxfp8.so"
 CHECKED_LIB = PKG / "libmxfp8_checked.so"
 SOURCES = ["capi.cu", "quantize_tma.cu", "quantize_generic.cu", "dequantize.cu", "selftest.cu",
-           "capi_mxfp4.cu", "mxfp4_convert.cu"]
-HEADERS = ["ptx.cuh", "recipe.cuh", "launch.h", "guard.cuh", "tile.cuh", "row_path.cuh", "stores.cuh", "mxfp4.cuh"]
+           "capi_mxfp4.cu", "mxfp4_convert.cu", "mxfp4_gemm.cu"]
+HEADERS = ["ptx.cuh", "recipe.cuh", "launch.h", "guard.cuh", "tile.cuh", "row_path.cuh", "stores.cuh", "mxfp4.cuh", "tcgen05.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

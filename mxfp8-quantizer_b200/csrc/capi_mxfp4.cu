@@ -1,5 +1,6 @@
 // capi_mxfp4.cu -- the extern "C" boundary declared in include/mxfp4.h:
-// argument validation, then the launches of mxfp4_convert.cu.
+// argument validation, then the launches of mxfp4_convert.cu and
+// mxfp4_gemm.cu.
 #include <cuda_runtime.h>
 
 #include "../../include/mxfp4.h"
@@ -72,4 +73,37 @@ extern "C" MXFP8_API int mxfp4_dequantize(const void* q, int64_t rows, int64_t c
     const StoreWindow ow = make_window(out, ((rows - 1) * ld_out + cols) * out_bytes(out_dtype));
     return launch_mxfp4_dequantize(static_cast<const uint8_t*>(q), rows, cols, ld_q, static_cast<const uint8_t*>(s),
                                    out, out_dtype, ld_out, ow, status, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" MXFP8_API int mxfp4_gemm(const void* a_q, int64_t m, int64_t ld_a, const void* a_s, int64_t a_s_bytes,
+                                    const void* b_q, int64_t n, int64_t ld_b, const void* b_s, int64_t b_s_bytes,
+                                    int64_t k, void* out, int out_dtype, int64_t ld_out, mxfp8_stream_t stream) {
+    if (!is_out_dtype(out_dtype)) return MXFP8_ERR_DTYPE;
+    if (m < 0 || n < 0 || k < 0 || k % 32 != 0 || m > kInt32Max || n > kInt32Max || k > kInt32Max - 255 ||
+        ld_a < k / 2 || ld_b < k / 2 || ld_a > kMaxStride || ld_b > kMaxStride || ld_out < n || ld_out > kMaxStride)
+        return MXFP8_ERR_SHAPE;
+    if (m == 0 || n == 0) return MXFP8_OK;
+    if (!out) return MXFP8_ERR_NULL_POINTER;
+    const int es = out_bytes(out_dtype);
+    if (!aligned(out, es)) return MXFP8_ERR_ALIGNMENT;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (k == 0) {
+        const cudaError_t e = cudaMemset2DAsync(out, (size_t)(ld_out * es), 0, (size_t)(n * es), (size_t)m, st);
+        if (e == cudaSuccess) return MXFP8_OK;
+        set_last_error("cudaMemset2DAsync", (int)e);
+        return MXFP8_ERR_CUDA;
+    }
+    if (int rc = check_fp4(a_q, m, k, ld_a, a_s, a_s_bytes)) return rc;
+    if (int rc = check_fp4(b_q, n, k, ld_b, b_s, b_s_bytes)) return rc;
+    Fp4GemmArgs g;
+    int sms = 0;
+    if (int rc = ready_device(&sms, &g.status)) return rc;
+    g.a = Fp4Operand{static_cast<const uint8_t*>(a_q), static_cast<const uint8_t*>(a_s), m, ld_a};
+    g.b = Fp4Operand{static_cast<const uint8_t*>(b_q), static_cast<const uint8_t*>(b_s), n, ld_b};
+    g.k = k;
+    g.out = out;
+    g.out_dtype = out_dtype;
+    g.ld_out = ld_out;
+    g.ow = make_window(out, ((m - 1) * ld_out + n) * es);
+    return launch_mxfp4_gemm(g, sms, st);
 }

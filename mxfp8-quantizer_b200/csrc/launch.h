@@ -1,6 +1,8 @@
 // launch.h -- internal host-side launch interface between the C ABI
 // (capi.cu) and the kernel translation units.
 #pragma once
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -49,6 +51,29 @@ struct Fp4QuantizeArgs {
 int launch_mxfp4_quantize(const Fp4QuantizeArgs& a, cudaStream_t stream);
 int launch_mxfp4_dequantize(const uint8_t* q, int64_t rows, int64_t cols, int64_t ld_q, const uint8_t* s, void* out,
                             int out_dtype, int64_t ld_out, StoreWindow ow, unsigned int* status, cudaStream_t stream);
+
+// One operand of the MXFP4 product: payload (rows, k / 2 bytes, row stride ld
+// bytes) and packed scales.
+struct Fp4Operand {
+    const uint8_t* q;
+    const uint8_t* s;
+    int64_t rows, ld;
+};
+
+struct Fp4GemmArgs {
+    Fp4Operand a, b;
+    int64_t k;
+    void* out;
+    int out_dtype;
+    int64_t ld_out;  // elements
+    StoreWindow ow;
+    unsigned int* status;
+};
+
+int launch_mxfp4_gemm(const Fp4GemmArgs& g, int sm_count, cudaStream_t stream);
+
+// The driver's cuTensorMapEncodeTiled, looked up once; null if it is missing.
+PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn();
 
 // SM count and device error word of the current device (made ready by the
 // first call on it); 0 or a negative mxfp8_status.

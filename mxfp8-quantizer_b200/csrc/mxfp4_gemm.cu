@@ -1,0 +1,494 @@
+// mxfp4_gemm.cu -- C (m, n) = A (m, k) B (n, k)^T for MXFP4 A and B, on the
+// block-scaled tensor cores (tcgen05.mma kind::mxf4): 64 products of E2M1
+// values a step, each block of 32 scaled by 2^(sa + sb - 254), summed in f32.
+//
+// One matrix supplies the 128 rows of a tile (P), the other its BN columns
+// (Q).  A CTA has one warp that streams 256-column stages of both (TMA tiles
+// with the 128-byte swizzle, scale chunks as untiled copies: a 128-row block's
+// chunks are contiguous along K), one that copies the scales to tensor memory
+// and issues the MMAs, and four or eight that read the accumulators back.
+//
+// SWAP = false: P is A.  A lane of tensor memory is a row of C, its columns
+//   are contiguous in memory: 32-byte stores.
+// SWAP = true: P is B.  A lane is a column of C, so a warp's stores are
+//   contiguous for any alignment, and few rows of A make a narrow tile: the
+//   form for single tokens, where streaming B is the whole cost.  If there are
+//   fewer tiles than SMs, a cluster of CTAs shares a tile: each takes a part of
+//   K, and their sums meet in shared memory over the cluster in rank order, so
+//   the result does not depend on timing.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <atomic>
+#include <cstring>
+
+#include "../../include/mxfp4.h"
+#include "launch.h"
+#include "ptx.cuh"
+#include "tcgen05.cuh"
+
+namespace mxfp8 {
+
+namespace {
+
+constexpr int kTileP = 128;        // rows of P in a tile: the MMA's M
+constexpr int kStageK = 256;       // elements of K in a stage: 128 bytes a row
+constexpr int kStepK = 64;         // elements of K in one MMA
+constexpr int kChunk = 512;        // bytes of one 128-row x 4-block scale chunk
+constexpr uint64_t kWaitNs = 1000000000ull;
+constexpr unsigned kErrGemmWait = 32u;   // bit of the device status word
+
+template <int BN, bool SWAP>
+struct Config {
+    static constexpr int row_blocks_q = (BN + 127) / 128;
+    static constexpr int p_bytes = kTileP * 128;
+    static constexpr int q_bytes = BN * 128;
+    static constexpr int sp_off = p_bytes + q_bytes;
+    static constexpr int sq_off = sp_off + 2 * kChunk;
+    static constexpr int stage_bytes = sq_off + row_blocks_q * 2 * kChunk;
+    static constexpr int stages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+    static constexpr int acc = BN <= 128 ? 2 : 1;              // accumulators in tensor memory
+    static constexpr int epi_warps = BN <= 128 ? 4 : 8;
+    static constexpr int threads = 32 * (epi_warps + 2);
+    // tensor memory: accumulators, then two sets of scales (A's and B's of one stage)
+    static constexpr int sf_cols = 2 * 4 + 2 * 4 * row_blocks_q;
+    static constexpr int cols_used = acc * BN + 2 * sf_cols;
+    static constexpr int tmem_cols = cols_used <= 64 ? 64 : cols_used <= 128 ? 128 : cols_used <= 256 ? 256 : 512;
+    static constexpr int bar_off = stages * stage_bytes;
+    static constexpr int n_bars = 2 * stages + 2 * acc;
+    static constexpr int ctl_off = bar_off + 8 * n_bars;
+    static constexpr int smem = ctl_off + 16 + 1024;            // and room to align the base to 1024
+    static_assert(cols_used <= 512 && stage_bytes % 1024 == 0);
+    static_assert(!SWAP || BN <= 128, "the join of a split K holds one BN x 128 f32 tile in the stages");
+};
+
+struct GemmParams {
+    const uint8_t* sp;          // scales of P and Q
+    const uint8_t* sq;
+    int col_chunks;             // scale chunks along K, the same for both
+    int row_blocks_q;           // 128-row blocks in Q's scale storage
+    int rows_p, rows_q;
+    int k;
+    int n_stages;               // ceil(k / 256)
+    int tiles_p, n_tiles;
+    int split;                  // CTAs of a cluster that share a tile
+    void* out;
+    int64_t ld_out;
+    StoreWindow ow;
+    unsigned int* status;
+};
+
+// Wait for a barrier's phase, at most kWaitNs, or until another role gave up.
+__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, volatile int* abort, unsigned int* status) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = global_timer_ns();
+    for (uint32_t i = 1;; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 255u) == 0) {
+            if (*abort) return false;
+            if (global_timer_ns() - t0 > kWaitNs) {
+                if (status) atomicOr(status, kErrGemmWait);
+                *abort = 1;
+                return false;
+            }
+        }
+    }
+}
+
+// Tile t: groups of 16 tiles of P by all tiles of Q, so that the tiles in
+// flight share operands in L2.
+__device__ __forceinline__ void tile_of(const GemmParams& p, int t, int& tp, int& tq) {
+    const int tiles_q = p.n_tiles / p.tiles_p;
+    const int group = t / (16 * tiles_q);
+    const int in = t - group * 16 * tiles_q;
+    const int wide = min(16, p.tiles_p - group * 16);
+    tq = in / wide;
+    tp = group * 16 + in - tq * wide;
+}
+
+template <int OUT>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (OUT == MXFP8_BF16) {
+        const __nv_bfloat162 t = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&t);
+    } else {
+        const __half2 t = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&t);
+    }
+}
+
+template <int OUT>
+__device__ __forceinline__ void store1(void* out, int64_t at, float v, const StoreWindow& w, unsigned int* status) {
+    if constexpr (OUT == MXFP8_F32) {
+        gstore_plain(static_cast<float*>(out) + at, v, w, status);
+    } else {
+        gstore_plain(static_cast<unsigned short*>(out) + at, (unsigned short)(pack2<OUT>(v, 0.0f) & 0xFFFFu), w, status);
+    }
+}
+
+// 32 bytes to a 32-byte aligned address: one whole sector a thread.
+__device__ __forceinline__ void store32(void* p, const uint32_t* v, const StoreWindow& w, unsigned int* status) {
+#ifdef MXFP8_CHECKED
+    const uint8_t* a = static_cast<const uint8_t*>(p);
+    if (a < w.lo || a + 32 > w.hi || (reinterpret_cast<uintptr_t>(p) & 31) != 0) {
+        if (status) atomicOr(status, kErrBoundsStore);
+        return;
+    }
+#else
+    (void)w;
+    (void)status;
+#endif
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+
+// NC f32 of one row of C, columns col .. col + NC - 1 (those below n), to out.
+template <int OUT, int NC>
+__device__ __forceinline__ void store_row(const GemmParams& p, int64_t row, int col, int n, const uint32_t* acc,
+                                          bool vec) {
+    constexpr int kEs = OUT == MXFP8_F32 ? 4 : 2;
+    constexpr int kPer = 32 / kEs;  // elements of one 32-byte store
+    const int64_t at = row * p.ld_out + col;
+    if (vec && col + NC <= n) {
+#pragma unroll
+        for (int i = 0; i < NC; i += kPer) {
+            if constexpr (OUT == MXFP8_F32) {
+                store32(static_cast<float*>(p.out) + at + i, acc + i, p.ow, p.status);
+            } else {
+                uint32_t h[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    h[j] = pack2<OUT>(__uint_as_float(acc[i + 2 * j]), __uint_as_float(acc[i + 2 * j + 1]));
+                store32(static_cast<unsigned short*>(p.out) + at + i, h, p.ow, p.status);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+            if (col + i < n) store1<OUT>(p.out, at + i, __uint_as_float(acc[i]), p.ow, p.status);
+    }
+}
+
+template <int BN, bool SWAP, int OUT>
+__global__ void __launch_bounds__(Config<BN, SWAP>::threads, 1)
+    mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
+                      const GemmParams p) {
+    using C = Config<BN, SWAP>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    const uint32_t base = smem_u32(smem);
+    const uint32_t full0 = base + C::bar_off, empty0 = full0 + 8 * C::stages;
+    const uint32_t acc_full0 = empty0 + 8 * C::stages, acc_empty0 = acc_full0 + 8 * C::acc;
+    volatile int* ctl = reinterpret_cast<volatile int*>(smem + C::ctl_off);  // abort, consumed stages, TMEM address
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int kLoadWarp = C::epi_warps, kMmaWarp = C::epi_warps + 1;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::stages; ++i) {
+            mbar_init(full0 + 8 * i, 1);
+            mbar_init(empty0 + 8 * i, 1);
+        }
+        for (int i = 0; i < C::acc; ++i) {
+            mbar_init(acc_full0 + 8 * i, 1);
+            mbar_init(acc_empty0 + 8 * i, C::epi_warps);
+        }
+        ctl[0] = 0;
+        ctl[1] = 0;
+        fence_mbar_init();
+    }
+    if (warp == kMmaWarp) tmem_alloc(base + C::ctl_off + 8, C::tmem_cols);
+    if (warp == kLoadWarp && lane == 0) {
+        prefetch_tensormap(&map_p);
+        prefetch_tensormap(&map_q);
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    const uint32_t tmem = (uint32_t)ctl[2];
+    const uint32_t tmem_sf = tmem + C::acc * BN;
+    grid_launch_dependents();
+    grid_wait_prerequisites();
+
+    const int rank = p.split > 1 ? (int)(blockIdx.x % p.split) : 0;
+    const int first_tile = blockIdx.x / p.split, tile_step = gridDim.x / p.split;
+    const int ks0 = (int)((int64_t)rank * p.n_stages / p.split);
+    const int ks1 = (int)((int64_t)(rank + 1) * p.n_stages / p.split);
+    int issued = 0;  // stages loaded by the load thread
+
+    if (warp == kLoadWarp) {
+        if (lane == 0) {
+            bool ok = true;
+            for (int t = first_tile; ok && t < p.n_tiles; t += tile_step) {
+                int tp, tq;
+                tile_of(p, t, tp, tq);
+                for (int ks = ks0; ks < ks1; ++ks, ++issued) {
+                    const int s = issued % C::stages;
+                    if (issued >= C::stages &&
+                        !wait_phase(empty0 + 8 * s, ((issued / C::stages) - 1) & 1, ctl, p.status)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t dst = base + s * C::stage_bytes, bar = full0 + 8 * s;
+                    const int chunks = min(2, p.col_chunks - 2 * ks);
+                    const int rbq = tq * BN / 128;
+                    const int nrbq = min(C::row_blocks_q, p.row_blocks_q - rbq);
+                    mbar_arrive_expect_tx(bar, C::p_bytes + C::q_bytes + (1 + nrbq) * chunks * kChunk);
+                    tma_load_2d(dst, &map_p, ks * (kStageK / 2), tp * kTileP, bar);
+                    tma_load_2d(dst + C::p_bytes, &map_q, ks * (kStageK / 2), tq * BN, bar);
+                    bulk_load(dst + C::sp_off, p.sp + ((int64_t)tp * p.col_chunks + 2 * ks) * kChunk, chunks * kChunk,
+                              bar);
+                    for (int r = 0; r < nrbq; ++r)
+                        bulk_load(dst + C::sq_off + r * 2 * kChunk,
+                                  p.sq + ((int64_t)(rbq + r) * p.col_chunks + 2 * ks) * kChunk, chunks * kChunk, bar);
+                }
+            }
+        }
+    } else if (warp == kMmaWarp) {
+        if (lane == 0) {
+            int it = 0, a = 0;
+            bool ok = true;
+            for (int t = first_tile; ok && t < p.n_tiles; t += tile_step, ++a) {
+                const int slot = a % C::acc;
+                if (a >= C::acc && !wait_phase(acc_empty0 + 8 * slot, ((a / C::acc) - 1) & 1, ctl, p.status)) break;
+                tcgen05_fence_after();
+                const uint32_t d = tmem + slot * BN;
+                for (int ks = ks0; ks < ks1; ++ks, ++it) {
+                    const int s = it % C::stages;
+                    if (!wait_phase(full0 + 8 * s, (it / C::stages) & 1, ctl, p.status)) {
+                        ok = false;
+                        break;
+                    }
+                    tcgen05_fence_after();
+                    const uint32_t src = base + s * C::stage_bytes;
+                    const uint32_t sfp = tmem_sf + (it & 1) * C::sf_cols, sfq = sfp + 8;
+                    const int chunks = min(2, p.col_chunks - 2 * ks);
+                    for (int c = 0; c < chunks; ++c) {
+                        tmem_copy_scales(sfp + 4 * c, desc_scale_chunk(src + C::sp_off + c * kChunk));
+#pragma unroll
+                        for (int r = 0; r < C::row_blocks_q; ++r)
+                            tmem_copy_scales(sfq + 4 * (c * C::row_blocks_q + r),
+                                             desc_scale_chunk(src + C::sq_off + (2 * r + c) * kChunk));
+                    }
+                    const int steps = min(kStageK / kStepK, (p.k - ks * kStageK + kStepK - 1) / kStepK);
+                    for (int j = 0; j < steps; ++j) {
+                        const int c = j >> 1, sf = 2 * (j & 1);
+                        mma_mxf4(d, desc_sw128(src + 32 * j), desc_sw128(src + C::p_bytes + 32 * j),
+                                 mxf4_idesc(kTileP, BN, sf), sfp + 4 * c, sfq + 4 * c * C::row_blocks_q,
+                                 ks > ks0 || j > 0);
+                    }
+                    tcgen05_commit(empty0 + 8 * s);
+                }
+                if (ok) tcgen05_commit(acc_full0 + 8 * slot);
+            }
+            ctl[1] = it;
+            // an abort leaves MMAs in flight: let them end before the tensor memory goes
+            if (ctl[0]) {
+                tcgen05_commit(acc_full0);
+                mbar_wait_bounded(acc_full0, 0, kWaitNs);
+            }
+        }
+    } else {
+        const int q4 = warp & 3;
+        const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
+        int a = 0;
+        for (int t = first_tile; t < p.n_tiles; t += tile_step, ++a) {
+            const int slot = a % C::acc;
+            const bool ok = __all_sync(0xFFFFFFFFu, wait_phase(acc_full0 + 8 * slot, (a / C::acc) & 1, ctl, p.status));
+            if (!ok) break;
+            tcgen05_fence_after();
+            int tp, tq;
+            tile_of(p, t, tp, tq);
+            const uint32_t d = tmem + slot * BN + lane_off;
+            if constexpr (!SWAP) {
+                // eight warps: two for each quarter of the lanes, 128 columns each
+                const int col0 = (warp >> 2) * 128;
+                uint32_t v[4][32];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tmem_load_32(d + col0 + 32 * i, v[i]);
+                tmem_wait_loads();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tmem_loaded(v[i]);
+                // the accumulator is in registers: the next tile's MMAs may overwrite it
+                tcgen05_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(acc_empty0 + 8 * slot);
+                const int64_t row = (int64_t)tp * kTileP + q4 * 32 + lane;
+                constexpr int kEs = OUT == MXFP8_F32 ? 4 : 2;
+                const bool vec = ((reinterpret_cast<uintptr_t>(p.out) | (uint64_t)(p.ld_out * kEs)) & 31) == 0;
+                if (row < p.rows_p) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        store_row<OUT, 32>(p, row, tq * BN + col0 + 32 * i, p.rows_q, v[i], vec);
+                }
+            } else {
+                const int64_t n = (int64_t)tp * kTileP + q4 * 32 + lane;
+                const int left = min(BN, p.rows_q - tq * BN);
+                float* red = reinterpret_cast<float*>(smem);
+                for (int c0 = 0; c0 < left; c0 += 16) {
+                    uint32_t v[16];
+                    tmem_load_16(d + c0, v);
+                    tmem_wait_loads();
+                    tmem_loaded(v);
+                    if (p.split > 1) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) red[(c0 + j) * 128 + q4 * 32 + lane] = __uint_as_float(v[j]);
+                    } else if (n < p.rows_p) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (c0 + j < left)
+                                store1<OUT>(p.out, ((int64_t)tq * BN + c0 + j) * p.ld_out + n, __uint_as_float(v[j]),
+                                            p.ow, p.status);
+                    }
+                }
+                tcgen05_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(acc_empty0 + 8 * slot);
+            }
+        }
+    }
+    __syncwarp();
+    if constexpr (SWAP) {
+        if (p.split > 1) {  // one tile a cluster: add the parts up, each CTA its share of the columns
+            cluster_sync();
+            if (warp < C::epi_warps && !ctl[0]) {
+                int tp, tq;
+                tile_of(p, first_tile, tp, tq);
+                const int64_t n = (int64_t)tp * kTileP + threadIdx.x;
+                const int left = min(BN, p.rows_q - tq * BN);
+                for (int c = rank; c < left; c += p.split) {
+                    const uint32_t at = base + (uint32_t)(c * 128 + threadIdx.x) * 4u;
+                    float sum = 0.0f;
+                    for (int r = 0; r < p.split; ++r) sum += cluster_load_f32(cluster_map(at, r));
+                    if (n < p.rows_p)
+                        store1<OUT>(p.out, ((int64_t)tq * BN + c) * p.ld_out + n, sum, p.ow, p.status);
+                }
+            }
+            cluster_sync();  // nobody leaves while its part is still read
+        }
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    if (warp == kLoadWarp && lane == 0) {
+        // loads that nobody waited for (only after an abort) still target this CTA
+        for (int i = ctl[1]; i < issued; ++i)
+            if (!mbar_wait_bounded(full0 + 8 * (i % C::stages), (i / C::stages) & 1, kWaitNs)) break;
+    }
+    if (warp == kMmaWarp) tmem_dealloc(tmem, C::tmem_cols);
+}
+
+// Tensor map of a payload: bytes (rows, cols / 2), boxes of 128 bytes by
+// `box_rows`, 128-byte swizzle, zeros outside.
+int encode_payload(CUtensorMap* map, const void* q, int64_t rows, int64_t bytes, int64_t ld, int box_rows) {
+    auto encode = get_encode_fn();
+    if (!encode) {
+        set_last_error("cuTensorMapEncodeTiled entry point unavailable", 0);
+        return MXFP8_ERR_TENSOR_MAP;
+    }
+    cuuint64_t dims[2] = {(cuuint64_t)bytes, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)ld};
+    cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+    cuuint32_t step[2] = {1, 1};
+    CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(q), dims, strides, box, step,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_last_error("cuTensorMapEncodeTiled failed", (int)r);
+        return MXFP8_ERR_TENSOR_MAP;
+    }
+    return MXFP8_OK;
+}
+
+template <int BN, bool SWAP, int OUT>
+int launch_typed(const Fp4GemmArgs& g, int sm_count, cudaStream_t stream) {
+    using C = Config<BN, SWAP>;
+    auto kernel = mxfp4_gemm_kernel<BN, SWAP, OUT>;
+    // once per device: later launches, captured ones among them, make no such call
+    static std::atomic<uint64_t> attr_set{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (e == cudaSuccess && !(attr_set.load(std::memory_order_acquire) & bit)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem);
+        if (e == cudaSuccess) attr_set.fetch_or(bit, std::memory_order_acq_rel);
+    }
+    if (e != cudaSuccess) {
+        set_last_error("cudaFuncSetAttribute", (int)e);
+        return MXFP8_ERR_CUDA;
+    }
+    const Fp4Operand& P = SWAP ? g.b : g.a;
+    const Fp4Operand& Q = SWAP ? g.a : g.b;
+    CUtensorMap map_p, map_q;
+    if (int rc = encode_payload(&map_p, P.q, P.rows, g.k / 2, P.ld, kTileP)) return rc;
+    if (int rc = encode_payload(&map_q, Q.q, Q.rows, g.k / 2, Q.ld, BN)) return rc;
+    GemmParams p;
+    p.sp = P.s;
+    p.sq = Q.s;
+    p.col_chunks = (int)((g.k + 127) / 128);
+    p.row_blocks_q = (int)((Q.rows + 127) / 128);
+    p.rows_p = (int)P.rows;
+    p.rows_q = (int)Q.rows;
+    p.k = (int)g.k;
+    p.n_stages = (int)((g.k + kStageK - 1) / kStageK);
+    p.tiles_p = (int)((P.rows + kTileP - 1) / kTileP);
+    const int64_t tiles = (int64_t)p.tiles_p * ((Q.rows + BN - 1) / BN);
+    if (tiles > (1 << 24)) return MXFP8_ERR_SHAPE;
+    p.n_tiles = (int)tiles;
+    p.split = 1;
+    if (SWAP)  // double the CTAs of a tile while they fit the SMs and each keeps two stages
+        while (p.split < 8 && tiles * p.split * 2 <= sm_count && p.n_stages >= 4 * p.split) p.split *= 2;
+    p.out = g.out;
+    p.ld_out = g.ld_out;
+    p.ow = g.ow;
+    p.status = g.status;
+
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(p.split > 1 ? tiles * p.split : tiles < sm_count ? tiles : sm_count));
+    cfg.blockDim = dim3(C::threads);
+    cfg.dynamicSmemBytes = C::smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)p.split;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = p.split > 1 ? 2 : 1;
+    e = cudaLaunchKernelEx(&cfg, kernel, map_p, map_q, p);
+    if (e == cudaSuccess) e = cudaGetLastError();
+    if (e != cudaSuccess) {
+        set_last_error("mxfp4_gemm_kernel launch", (int)e);
+        return MXFP8_ERR_CUDA;
+    }
+    return MXFP8_OK;
+}
+
+template <int BN, bool SWAP>
+int launch_out(const Fp4GemmArgs& g, int sm_count, cudaStream_t stream) {
+    switch (g.out_dtype) {
+        case MXFP8_F32: return launch_typed<BN, SWAP, MXFP8_F32>(g, sm_count, stream);
+        case MXFP8_BF16: return launch_typed<BN, SWAP, MXFP8_BF16>(g, sm_count, stream);
+        default: return launch_typed<BN, SWAP, MXFP8_FP16>(g, sm_count, stream);
+    }
+}
+
+}  // namespace
+
+int launch_mxfp4_gemm(const Fp4GemmArgs& g, int sm_count, cudaStream_t stream) {
+    if (g.a.rows <= 16) return launch_out<16, true>(g, sm_count, stream);
+    if (g.a.rows <= 32) return launch_out<32, true>(g, sm_count, stream);
+    if (g.a.rows <= 64) return launch_out<64, true>(g, sm_count, stream);
+    const int es = g.out_dtype == MXFP8_F32 ? 4 : 2;
+    const bool vec = ((reinterpret_cast<uintptr_t>(g.out) | (uint64_t)(g.ld_out * es)) & 31) == 0;
+    const int64_t wide_tiles = ((g.a.rows + 127) / 128) * ((g.b.rows + 255) / 256);
+    if (vec && wide_tiles >= sm_count) return launch_out<256, false>(g, sm_count, stream);
+    return launch_out<128, true>(g, sm_count, stream);
+}
+
+}  // namespace mxfp8

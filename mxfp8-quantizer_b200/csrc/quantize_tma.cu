@@ -306,7 +306,7 @@ constexpr int64_t kMaxTilesPerLaunch = 148 * 128;  // ~0.94 GB of traffic per la
 // path, no change at 8192 tiles or below.
 constexpr int64_t kMaxTilesPerLaunchRows = 148 * 64;
 
-static PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn() {
+PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn() {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
     static std::once_flag once;
     std::call_once(once, [] {

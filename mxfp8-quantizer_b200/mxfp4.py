@@ -83,3 +83,33 @@ def dequantize_mxfp4(q: torch.Tensor, s: torch.Tensor, out_dtype: torch.dtype = 
         _capi.fp4_dequantize(q.data_ptr(), rows, cols, _row_stride(q), s.data_ptr(), s.numel(), out.data_ptr(), code,
                              cols, handle)
     return out
+
+
+def mxfp4_gemm(a_q: torch.Tensor, b_q: torch.Tensor, a_s: torch.Tensor, b_s: torch.Tensor,
+               out_dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """C (m, n) = A B^T of two MXFP4 matrices A (m, k) and B (n, k), summed in
+    fp32 and rounded once to out_dtype (fp32, bf16 or fp16): the 4-bit form of
+    ``blockscaled_gemm``, on this library's own kernel.
+
+    ``a_q``/``a_s`` and ``b_q``/``b_s`` are what ``quantize_mxfp4`` returns
+    (scale bytes of the padding must not be 255; it writes 0).  A given
+    ``out`` (m, n), row-major with any row stride, is written in place and
+    sets the output type; it must not overlap the operands."""
+    m, k = _check_payload("a_q", a_q)
+    n, k_b = _check_payload("b_q", b_q)
+    if k != k_b:
+        raise ValueError(f"a_q and b_q must have the same number of columns, got {k} and {k_b}")
+    _check_scales("a_s", a_s)
+    _check_scales("b_s", b_s)
+    if out is not None:
+        if out.dim() != 2 or tuple(out.shape) != (m, n) or (out.stride(1) != 1 and n > 1):
+            raise ValueError(f"out must be a row-major ({m}, {n}) matrix, got {tuple(out.shape)}")
+        out_dtype = out.dtype
+    code = out_dtype_code(out_dtype)
+    context, handle = on_stream(stream, a_q, b_q, a_s, b_s, *(() if out is None else (out,)))
+    with context:
+        if out is None:
+            out = torch.empty((m, n), dtype=out_dtype, device=a_q.device)
+        _capi.fp4_gemm(a_q.data_ptr(), m, _row_stride(a_q), a_s.data_ptr(), a_s.numel(), b_q.data_ptr(), n,
+                       _row_stride(b_q), b_s.data_ptr(), b_s.numel(), k, out.data_ptr(), code, _row_stride(out), handle)
+    return out

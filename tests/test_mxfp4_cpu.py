@@ -99,3 +99,40 @@ def test_the_64_bit_form_rounds_to_nearest_even():
     codes, scale = fp4_ref.quantize(bits, "bf16")
     assert codes[0, :9].tolist() == [7, 0, 2, 2, 4, 4, 6, 6, 8]
     assert scale.tolist() == [[127], [128]] and codes[1, :2].tolist() == [5, 0]
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(code=9), "dtype"),
+    (dict(k=48), "sizes"),
+    (dict(ld_a=48), "sizes"),
+    (dict(ld_out=7), "sizes"),
+    (dict(out=0), "NULL"),
+    (dict(out=0x7002), "alignment"),
+    (dict(a=0), "NULL"),
+    (dict(b_s=0), "NULL"),
+    (dict(a=0x1008), "alignment"),
+    (dict(ld_b=72), "alignment"),
+    (dict(b_s=0x4004), "alignment"),
+    (dict(a_s_bytes=511), "scale buffer"),
+    (dict(b_s_bytes=511), "scale buffer"),
+])
+def test_gemm_refuses(change, match):
+    a = dict(a=0x1000, m=4, ld_a=64, a_s=0x2000, a_s_bytes=512, b=0x3000, n=8, ld_b=64, b_s=0x4000, b_s_bytes=512,
+             k=128, out=0x7000, code=2, ld_out=8)
+    a.update(change)
+    with pytest.raises(ValueError, match=match):
+        capi.fp4_gemm(*a.values(), 0)
+
+
+def test_gemm_wrapper_refuses():
+    q, s = torch.zeros((4, 32), dtype=torch.uint8), torch.zeros(512, dtype=torch.uint8)
+    with pytest.raises(ValueError, match="CUDA"):
+        pkg.mxfp4_gemm(q, q, s, s)
+    with pytest.raises(ValueError, match="same number of columns"):
+        pkg.mxfp4_gemm(q, q[:, :16], s, s)
+    with pytest.raises(ValueError, match="out must"):
+        pkg.mxfp4_gemm(q, q, s, s, out=torch.zeros((4, 5)))
+    with pytest.raises(ValueError, match="out_dtype"):
+        pkg.mxfp4_gemm(q, q, s, s, torch.float64)
+    with pytest.raises(ValueError, match="contiguous"):
+        pkg.mxfp4_gemm(q, q, s[::2], s)

@@ -181,3 +181,188 @@ def test_checked_build_writes_the_same_bytes():
             assert word.value == expect, (m, k, slack)
         assert checked.mxfp8_checked_window_slack(0) == 0
         assert torch.equal(q2, q) and torch.equal(s2, s) and torch.equal(out, pkg.dequantize_mxfp4(q, s))
+
+
+# --------------------------------------------------------------------------
+# the product
+# --------------------------------------------------------------------------
+
+HALF_STEP = {"bf16": 2.0 ** -8, "fp16": 2.0 ** -11, "f32": 2.0 ** -24}
+
+
+def check_gemm(m, n, k, out, seed=0, spread=3):
+    """Against 64 bits.  The products are exact; each of the at most k f32
+    additions of an output is off by at most one unit in the last place
+    (2^-23) of a partial sum, which is at most sum |a||b|; then one rounding."""
+    rng = np.random.default_rng(seed + m * 7 + n * 3 + k)
+    a_q, a_s, a = fp4_ref.random_matrix(rng, m, k, spread)
+    b_q, b_s, b = fp4_ref.random_matrix(rng, n, k, spread)
+    a_q, a_s, b_q, b_s = (torch.from_numpy(t).cuda() for t in (a_q, a_s, b_q, b_s))
+    got = pkg.mxfp4_gemm(a_q, b_q, a_s, b_s, TORCH[out])
+    assert capi.device_status(clear=True) == 0
+    a, b = torch.from_numpy(a).cuda(), torch.from_numpy(b).cuda()
+    want = a @ b.t()
+    room = k * 2.0 ** -23 * (a.abs() @ b.abs().t()) + HALF_STEP[out] * want.abs() * (1 + 2.0 ** -8)
+    off = (got.double() - want).abs() - room
+    assert not (off > 0).any(), (m, n, k, out, off.max().item(), (off > 0).sum().item())
+    return got
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 1, 32), (1, 128, 64), (1, 128, 256), (1, 4096, 4096), (16, 300, 96),
+                                   (17, 129, 160), (32, 256, 1024), (33, 100, 352), (64, 512, 2048), (65, 17, 64),
+                                   (77, 1000, 2080), (128, 128, 128), (129, 255, 288), (200, 1024, 4096),
+                                   (300, 77, 1056)])
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+def test_gemm(m, n, k, out):
+    check_gemm(m, n, k, out)
+
+
+@pytest.mark.parametrize("m,n,k,out", [(4096, 1280, 512, "fp16"), (4096, 1280, 96, "f32"), (2048, 2304, 288, "bf16"),
+                                       (4000, 1296, 544, "bf16"), (4095, 1301, 256, "fp16"), (2500, 2500, 1024, "f32"),
+                                       (10000, 520, 320, "bf16")])
+def test_gemm_many_tiles(m, n, k, out):
+    check_gemm(m, n, k, out)
+
+
+@pytest.mark.parametrize("m", [1, 16, 40, 130, 4096])
+def test_gemm_small_integers_are_exact(m):
+    """All scales 1 and k <= 1024: every partial sum is a multiple of 1/4 below 2^16, so f32 holds it."""
+    rng = np.random.default_rng(m)
+    scale = np.full((m, 32), 127, np.uint8)
+    codes = rng.integers(0, 16, (m, 1024)).astype(np.uint8)
+    b_codes = rng.integers(0, 16, (1280, 1024)).astype(np.uint8)
+    b_scale = np.full((1280, 32), 127, np.uint8)
+    t = [torch.from_numpy(x).cuda() for x in (fp4_ref.pack_codes(codes), fp4_ref.pack_codes(b_codes),
+                                              fp4_ref.pack_scales(scale), fp4_ref.pack_scales(b_scale))]
+    want = torch.from_numpy(fp4_ref.values(codes, scale)).cuda() @ torch.from_numpy(fp4_ref.values(b_codes, b_scale)).cuda().t()
+    assert torch.equal(pkg.mxfp4_gemm(*t).double(), want)
+
+
+@pytest.mark.parametrize("m,n,ld,offset", [(5, 100, 101, 3), (70, 130, 137, 1), (2000, 2560, 2561, 5)])
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+def test_gemm_into_any_row_stride(m, n, ld, offset, out):
+    buf = torch.full((m * ld + offset + 8,), -7.0, dtype=TORCH[out], device="cuda")
+    view = buf[offset:offset + m * ld].view(m, ld)[:, :n]
+    got = check_gemm(m, n, 96, out)
+    rng = np.random.default_rng(m * 7 + n * 3 + 96)
+    a_q, a_s, _ = fp4_ref.random_matrix(rng, m, 96, 3)
+    b_q, b_s, _ = fp4_ref.random_matrix(rng, n, 96, 3)
+    a_q, a_s, b_q, b_s = (torch.from_numpy(t).cuda() for t in (a_q, a_s, b_q, b_s))
+    assert pkg.mxfp4_gemm(a_q, b_q, a_s, b_s, out=view) is view
+    room = 96 * 2.0 ** -22 * 36 * 64 * 96 + 2 * HALF_STEP[out] * got.double().abs()   # two orders of one sum
+    assert ((view.double() - got.double()).abs() <= room).all()
+    rest = buf.clone()
+    rest[offset:offset + m * ld].view(m, ld)[:, :n] = -7.0
+    assert (rest == -7.0).all()
+
+
+def test_gemm_padded_rows_and_views():
+    """Operands that are column and row slices of larger matrices."""
+    rng = np.random.default_rng(11)
+    a_q, a_s, a = fp4_ref.random_matrix(rng, 30, 64)
+    b_q, b_s, b = fp4_ref.random_matrix(rng, 90, 64)
+    big_a = torch.full((30, 80), 0xFF, dtype=torch.uint8, device="cuda")
+    big_b = torch.full((128, 64), 0xFF, dtype=torch.uint8, device="cuda")
+    va, vb = big_a[:, 16:48], big_b[20:110, 32:]
+    va.copy_(torch.from_numpy(a_q)), vb.copy_(torch.from_numpy(b_q))
+    got = pkg.mxfp4_gemm(va, vb, torch.from_numpy(a_s).cuda(), torch.from_numpy(b_s).cuda())
+    want = pkg.mxfp4_gemm(torch.from_numpy(a_q).cuda(), torch.from_numpy(b_q).cuda(), torch.from_numpy(a_s).cuda(),
+                          torch.from_numpy(b_s).cuda())
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("m,n", [(3, 200), (150, 200), (2560, 2048)])
+def test_gemm_nan_blocks_reach_their_outputs_only(m, n):
+    rng = np.random.default_rng(m)
+    k = 256
+    a_codes, b_codes = (rng.integers(0, 16, (r, k)).astype(np.uint8) for r in (m, n))
+    a_scale, b_scale = (np.full((r, k // 32), 127, np.uint8) for r in (m, n))
+    a_scale[m - 1, 3] = 255
+    b_scale[5, 0] = 255
+    t = [torch.from_numpy(x).cuda() for x in (fp4_ref.pack_codes(a_codes), fp4_ref.pack_codes(b_codes),
+                                              fp4_ref.pack_scales(a_scale), fp4_ref.pack_scales(b_scale))]
+    got = pkg.mxfp4_gemm(*t)
+    nan = torch.zeros((m, n), dtype=torch.bool, device="cuda")
+    nan[m - 1] = True
+    nan[:, 5] = True
+    assert torch.equal(got.isnan(), nan)
+
+
+def test_gemm_extreme_scales():
+    """Scales at both ends of their range: 2^-127 * 2^127 products are ordinary numbers."""
+    codes = np.full((4, 64), 2, np.uint8)                 # 1.0
+    low, high = np.full((4, 2), 0, np.uint8), np.full((4, 2), 254, np.uint8)
+    q = torch.from_numpy(fp4_ref.pack_codes(codes)).cuda()
+    s_low, s_high = (torch.from_numpy(fp4_ref.pack_scales(s)).cuda() for s in (low, high))
+    assert (pkg.mxfp4_gemm(q, q, s_low, s_high) == 64.0).all()
+
+
+def test_gemm_empty():
+    z = torch.empty((0, 32), dtype=torch.uint8, device="cuda")
+    none = torch.empty(0, dtype=torch.uint8, device="cuda")
+    q, s = torch.zeros((4, 32), dtype=torch.uint8, device="cuda"), torch.zeros(512, dtype=torch.uint8, device="cuda")
+    assert pkg.mxfp4_gemm(z, q, none, s).shape == (0, 4)
+    assert pkg.mxfp4_gemm(q, z, s, none).shape == (4, 0)
+    assert (pkg.mxfp4_gemm(q[:, :0], q[:, :0], none, none) == 0).all()
+
+
+@pytest.mark.parametrize("m", [2, 100, 3000])
+def test_gemm_repeats_bit_for_bit_on_streams_and_in_graphs(m):
+    rng = np.random.default_rng(m)
+    sets = []
+    for i in range(2):
+        a_q, a_s, _ = fp4_ref.random_matrix(rng, m, 2048)
+        b_q, b_s, _ = fp4_ref.random_matrix(rng, 2048, 2048)
+        sets.append([torch.from_numpy(x).cuda() for x in (a_q, b_q, a_s, b_s)])
+    want = [pkg.mxfp4_gemm(*t) for t in sets]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    other = [pkg.mxfp4_gemm(*t, stream=side) for t in sets]
+    here = [pkg.mxfp4_gemm(*t) for t in sets]            # at the same time as the side stream's
+    torch.cuda.current_stream().wait_stream(side)
+    for w, o, h in zip(want, other, here):
+        assert torch.equal(w, o) and torch.equal(w, h)
+    graph = torch.cuda.CUDAGraph()
+    static = [t.clone() for t in sets[0]]
+    with torch.cuda.graph(graph):
+        c = pkg.mxfp4_gemm(*static)
+        c2 = pkg.mxfp4_gemm(*sets[1])
+    for t, w in zip((sets[1], sets[0]), (want[1], want[0])):
+        for dst, src in zip(static, t):
+            dst.copy_(src)
+        graph.replay()
+        assert torch.equal(c, w) and torch.equal(c2, want[1])
+    assert capi.device_status() == 0
+
+
+def test_quantize_then_product():
+    """x W^T through quantize_mxfp4 and mxfp4_gemm equals the product of the dequantized matrices."""
+    x = torch.randn((70, 500), device="cuda").bfloat16()
+    w = torch.randn((300, 500), device="cuda").bfloat16()
+    (xq, xs), (wq, ws) = pkg.quantize_mxfp4(x), pkg.quantize_mxfp4(w)
+    got = pkg.mxfp4_gemm(xq, wq, xs, ws)
+    a, b = (pkg.dequantize_mxfp4(*t).double() for t in ((xq, xs), (wq, ws)))
+    room = 512 * 2.0 ** -23 * (a.abs() @ b.abs().t())
+    assert ((got.double() - a @ b.t()).abs() <= room).all()
+
+
+def test_gemm_checked_build():
+    """The checked build's guards see every store of the product."""
+    checked = capi.checked_lib()
+    word = ctypes.c_uint32(0)
+    rng = np.random.default_rng(2)
+    for m, n, k in ((3, 100, 64), (77, 130, 2080), (2560, 2056, 96), (2560, 2051, 96)):
+        a_q, a_s, _ = fp4_ref.random_matrix(rng, m, k)
+        b_q, b_s, _ = fp4_ref.random_matrix(rng, n, k)
+        a_q, a_s, b_q, b_s = (torch.from_numpy(t).cuda() for t in (a_q, a_s, b_q, b_s))
+        want = pkg.mxfp4_gemm(a_q, b_q, a_s, b_s)
+        out = torch.zeros_like(want)
+        for slack, expect in ((0, 0), (4, 16)):
+            assert checked.mxfp8_checked_window_slack(slack) == 0
+            assert checked.mxfp4_gemm(a_q.data_ptr(), m, k // 2, a_s.data_ptr(), a_s.numel(), b_q.data_ptr(), n, k // 2,
+                                      b_s.data_ptr(), b_s.numel(), k, out.data_ptr(), 2, n,
+                                      torch.cuda.current_stream().cuda_stream) == 0
+            assert checked.mxfp8_device_status(ctypes.byref(word), 1) == 0
+            assert word.value == expect
+        assert checked.mxfp8_checked_window_slack(0) == 0
+        assert torch.equal(out, want)
