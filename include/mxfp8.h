@@ -42,7 +42,8 @@ enum mxfp8_status {
     MXFP8_ERR_SCALE_BUFFER = -5,   /* the scale buffer is smaller than required */
     MXFP8_ERR_CUDA = -6,           /* a CUDA runtime call failed (launch, attribute, ...) */
     MXFP8_ERR_TENSOR_MAP = -7,     /* the driver rejected a TMA descriptor */
-    MXFP8_ERR_DEVICE = -8          /* no usable sm_100 device is current */
+    MXFP8_ERR_DEVICE = -8,         /* no usable sm_100 device is current */
+    MXFP8_ERR_WORKSPACE = -9       /* the workspace is smaller than required */
 };
 
 /* Packed scale storage bytes for a (rows, cols) quantized matrix:
@@ -134,7 +135,8 @@ MXFP8_API int mxfp8_dequantize(const void* q, int64_t rows, int64_t cols, int64_
  * bit here and the kernel returns early.  Bits: 1 = payload tile wait,
  * 2 = stage-release wait, 4 = drain wait on exit, 8 = the self-test's wait,
  * 16 = a store outside its output was skipped (only the checked build,
- * include/mxfp8_checked.h, tests stores).  Reading waits for the device
+ * include/mxfp8_checked.h, tests stores), 32 = a wait of the MXFP4 product
+ * (mxfp4.h), 64 = a cache index that was not followed (mxfp8_cache.h).  Reading waits for the device
  * (cudaDeviceSynchronize); clear != 0 resets the word.  The word lives in a
  * small device buffer allocated on the first call on each device (and in
  * each new CUDA context of it).  Calls of mxfp8_quantize_noalloc report to

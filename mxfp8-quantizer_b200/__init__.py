@@ -4,6 +4,7 @@ CUDA, C ABI in include/mxfp8.h); this package is the Python host side that
 mirrors the reference's API (see quantizer.py)."""
 
 from . import _capi, shard
+from .kv_cache import MXFP8Cache, allocate_cache, cache_attention, cache_read, cache_write
 from .mxfp4 import FP4_E2M1_MAX, dequantize_mxfp4, mxfp4_gemm, quantize_mxfp4
 from .quantizer import (
     DEFAULT_E2E_SUITE,

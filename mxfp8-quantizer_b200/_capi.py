@@ -29,6 +29,7 @@ ERR_SCALE_BUFFER = -5
 ERR_CUDA = -6
 ERR_TENSOR_MAP = -7
 ERR_DEVICE = -8
+ERR_WORKSPACE = -9
 
 EXPORTS = (
     "mxfp8_scale_storage_bytes",
@@ -50,6 +51,23 @@ FP4_EXPORTS = (
     "mxfp4_dequantize",
     "mxfp4_gemm",
 )
+
+# include/mxfp8_cache.h
+CACHE_EXPORTS = (
+    "mxfp8_cache_write",
+    "mxfp8_cache_read",
+    "mxfp8_cache_attention_workspace",
+    "mxfp8_cache_attention",
+)
+
+
+class Cache(ctypes.Structure):
+    """struct mxfp8_cache."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scales", ctypes.c_void_p),
+                ("v_scales", ctypes.c_void_p), ("num_pages", ctypes.c_int64), ("heads", ctypes.c_int32),
+                ("page_size", ctypes.c_int32), ("dim", ctypes.c_int32)]
+
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
@@ -90,6 +108,15 @@ def configure(L: ctypes.CDLL) -> ctypes.CDLL:
     L.mxfp4_dequantize.restype = i32
     L.mxfp4_gemm.argtypes = [vp, i64, i64, vp, i64, vp, i64, i64, vp, i64, i64, vp, i32, i64, vp]
     L.mxfp4_gemm.restype = i32
+    cache, f32 = ctypes.POINTER(Cache), ctypes.c_float
+    L.mxfp8_cache_write.argtypes = [cache, vp, i64, i64, vp, i64, i64, i32, i64, vp, vp]
+    L.mxfp8_cache_write.restype = i32
+    L.mxfp8_cache_read.argtypes = [cache, vp, i64, i64, i64, vp, i64, vp, vp, i32, vp]
+    L.mxfp8_cache_read.restype = i32
+    L.mxfp8_cache_attention_workspace.argtypes = [cache, i64, i64]
+    L.mxfp8_cache_attention_workspace.restype = i64
+    L.mxfp8_cache_attention.argtypes = [cache, vp, i64, i64, i32, i64, i64, vp, i64, i64, vp, f32, vp, vp, vp, i64, vp]
+    L.mxfp8_cache_attention.restype = i32
     if hasattr(L, "mxfp8_checked_window_slack"):
         L.mxfp8_checked_window_slack.argtypes = [i64]
         L.mxfp8_checked_window_slack.restype = i32
@@ -197,6 +224,36 @@ def fp4_gemm(a_ptr: int, m: int, ld_a: int, a_s_ptr: int, a_s_bytes: int, b_ptr:
     rc = lib().mxfp4_gemm(a_ptr or None, m, ld_a, a_s_ptr or None, a_s_bytes, b_ptr or None, n, ld_b, b_s_ptr or None,
                           b_s_bytes, k, out_ptr or None, out_dtype, ld_out, stream or None)
     check(rc, "MXFP4 product launch")
+
+
+def cache_write(cache: Cache, k_ptr: int, k_token: int, k_head: int, v_ptr: int, v_token: int, v_head: int, dtype: int,
+                tokens: int, slots_ptr: int, stream: int) -> None:
+    rc = lib().mxfp8_cache_write(cache, k_ptr or None, k_token, k_head, v_ptr or None, v_token, v_head, dtype, tokens,
+                                 slots_ptr or None, stream or None)
+    check(rc, "cache write launch")
+
+
+def cache_read(cache: Cache, table_ptr: int, table_stride: int, max_pages: int, batch: int, starts_ptr: int, total: int,
+               k_out_ptr: int, v_out_ptr: int, out_dtype: int, stream: int) -> None:
+    rc = lib().mxfp8_cache_read(cache, table_ptr or None, table_stride, max_pages, batch, starts_ptr or None, total,
+                                k_out_ptr or None, v_out_ptr or None, out_dtype, stream or None)
+    check(rc, "cache read launch")
+
+
+def cache_attention_workspace(cache: Cache, batch: int, q_heads: int) -> int:
+    n = int(lib().mxfp8_cache_attention_workspace(cache, batch, q_heads))
+    if n < 0:
+        check(n, "cache attention workspace")
+    return n
+
+
+def cache_attention(cache: Cache, q_ptr: int, q_batch: int, q_head: int, dtype: int, batch: int, q_heads: int,
+                    table_ptr: int, table_stride: int, max_pages: int, lengths_ptr: int, scale: float, out_ptr: int,
+                    lse_ptr: int, workspace_ptr: int, workspace_bytes: int, stream: int) -> None:
+    rc = lib().mxfp8_cache_attention(cache, q_ptr or None, q_batch, q_head, dtype, batch, q_heads, table_ptr or None,
+                                     table_stride, max_pages, lengths_ptr or None, scale, out_ptr or None,
+                                     lse_ptr or None, workspace_ptr or None, workspace_bytes, stream or None)
+    check(rc, "cache attention launch")
 
 
 def device_status(clear: bool = False) -> int:

@@ -23,8 +23,10 @@ CSRC = PKG / "csrc"
 LIB = PKG / "libmxfp8.so"
 CHECKED_LIB = PKG / "libmxfp8_checked.so"
 SOURCES = ["capi.cu", "quantize_tma.cu", "quantize_generic.cu", "dequantize.cu", "selftest.cu",
-           "capi_mxfp4.cu", "mxfp4_convert.cu", "mxfp4_gemm.cu"]
-HEADERS = ["ptx.cuh", "recipe.cuh", "launch.h", "guard.cuh", "tile.cuh", "row_path.cuh", "stores.cuh", "mxfp4.cuh", "tcgen05.cuh"]
+           "capi_mxfp4.cu", "mxfp4_convert.cu", "mxfp4_gemm.cu", "capi_cache.cu", "cache_copy.cu",
+           "cache_attention.cu"]
+HEADERS = ["ptx.cuh", "recipe.cuh", "launch.h", "guard.cuh", "tile.cuh", "row_path.cuh", "stores.cuh", "mxfp4.cuh",
+           "tcgen05.cuh", "cache.cuh", "cache_index.h"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -38,7 +40,7 @@ def nvcc() -> str:
 def inputs() -> list[pathlib.Path]:
     return [CSRC / s for s in SOURCES] + [CSRC / h for h in HEADERS] + [
         ROOT / "include" / "mxfp8.h", ROOT / "include" / "mxfp8_checked.h", ROOT / "include" / "mxfp4.h",
-        pathlib.Path(__file__)]
+        ROOT / "include" / "mxfp8_cache.h", pathlib.Path(__file__)]
 
 
 def up_to_date(lib: pathlib.Path) -> bool:

@@ -1,0 +1,64 @@
+// cache_index.h -- index arithmetic of the paged cache: which row a position
+// lives in, which sequence an output row belongs to, and how the attention's
+// tiles are split over CTAs.  Plain C++, so that the CPU tests compile it too.
+#pragma once
+#include <stdint.h>
+
+#ifdef __CUDACC__
+#define MXFP8_HD __host__ __device__ __forceinline__
+#else
+#define MXFP8_HD inline
+#endif
+
+namespace mxfp8 {
+
+// Geometry of a cache; page_size = 1 << page_shift.
+struct CacheShape {
+    int64_t num_pages;
+    int heads;
+    int page_shift;
+    int dim;
+};
+
+constexpr int64_t kNoRow = -1;
+
+// Row (of dim bytes, of dim / 32 scale bytes) of a page's position for head
+// h, or kNoRow for a page outside the cache.
+MXFP8_HD int64_t cache_row(const CacheShape& c, int64_t page, int head, int offset) {
+    if (page < 0 || page >= c.num_pages) return kNoRow;
+    return ((page * c.heads + head) << c.page_shift) + offset;
+}
+
+// Page of position `at` of sequence b, or -1 if it lies past the table's row.
+MXFP8_HD int64_t table_page(const int32_t* table, int64_t stride, int64_t max_pages, int64_t b, int64_t at,
+                            int page_shift) {
+    const int64_t i = at >> page_shift;
+    return at < 0 || i >= max_pages ? -1 : table[b * stride + i];
+}
+
+// The sequence that covers output row `row`: the last b with starts[b] <=
+// row; batch if the row lies past the last sequence, -1 before the first.
+MXFP8_HD int64_t sequence_of(const int32_t* starts, int64_t batch, int64_t row) {
+    if (row < starts[0]) return -1;
+    if (row >= starts[batch]) return batch;
+    int64_t lo = 0, hi = batch;  // starts[lo] <= row < starts[hi]
+    while (hi - lo > 1) {
+        const int64_t mid = (lo + hi) >> 1;
+        if (starts[mid] <= row) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// `total` tiles over n parts: part i takes [split_begin(i), split_begin(i + 1)).
+MXFP8_HD int64_t split_begin(int64_t i, int64_t n, int64_t total) { return i * total / n; }
+// The part that holds tile x < total.
+MXFP8_HD int64_t split_part(int64_t x, int64_t n, int64_t total) { return ((x + 1) * n - 1) / total; }
+
+// Positions of a sequence that the attention visits.
+MXFP8_HD int64_t visible_length(int64_t length, int64_t max_pages, int page_shift) {
+    const int64_t room = max_pages << page_shift;
+    return length < 0 ? 0 : length < room ? length : room;
+}
+
+}  // namespace mxfp8

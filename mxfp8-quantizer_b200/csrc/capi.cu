@@ -381,6 +381,7 @@ extern "C" MXFP8_API const char* mxfp8_strerror(int status) {
         case MXFP8_ERR_CUDA: return "a CUDA runtime call failed";
         case MXFP8_ERR_TENSOR_MAP: return "the driver rejected a TMA descriptor";
         case MXFP8_ERR_DEVICE: return "no usable sm_100 device is current";
+        case MXFP8_ERR_WORKSPACE: return "the workspace is smaller than required";
         default: return "unknown status";
     }
 }
