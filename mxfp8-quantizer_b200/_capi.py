@@ -207,36 +207,36 @@ def dequantize(q_ptr: int, rows: int, cols: int, ld_q: int, s_ptr: int, s_bytes:
 
 def fp4_quantize(x_ptr: int, dtype: int, m: int, k: int, ld_x: int, q_ptr: int, ld_q: int, s_ptr: int, s_bytes: int,
                  stream: int) -> None:
-    rc = lib().mxfp4_quantize(x_ptr or None, dtype, m, k, ld_x, q_ptr or None, ld_q, s_ptr or None, s_bytes,
-                              stream or None)
+    rc = lib().mxfp4_quantize(x_ptr, dtype, m, k, ld_x, q_ptr, ld_q, s_ptr, s_bytes,
+                              stream)
     check(rc, "MXFP4 quantizer launch")
 
 
 def fp4_dequantize(q_ptr: int, rows: int, cols: int, ld_q: int, s_ptr: int, s_bytes: int, out_ptr: int,
                    out_dtype: int, ld_out: int, stream: int) -> None:
-    rc = lib().mxfp4_dequantize(q_ptr or None, rows, cols, ld_q, s_ptr or None, s_bytes, out_ptr or None, out_dtype,
-                                ld_out, stream or None)
+    rc = lib().mxfp4_dequantize(q_ptr, rows, cols, ld_q, s_ptr, s_bytes, out_ptr, out_dtype,
+                                ld_out, stream)
     check(rc, "MXFP4 dequantizer launch")
 
 
 def fp4_gemm(a_ptr: int, m: int, ld_a: int, a_s_ptr: int, a_s_bytes: int, b_ptr: int, n: int, ld_b: int, b_s_ptr: int,
              b_s_bytes: int, k: int, out_ptr: int, out_dtype: int, ld_out: int, stream: int) -> None:
-    rc = lib().mxfp4_gemm(a_ptr or None, m, ld_a, a_s_ptr or None, a_s_bytes, b_ptr or None, n, ld_b, b_s_ptr or None,
-                          b_s_bytes, k, out_ptr or None, out_dtype, ld_out, stream or None)
+    rc = lib().mxfp4_gemm(a_ptr, m, ld_a, a_s_ptr, a_s_bytes, b_ptr, n, ld_b, b_s_ptr,
+                          b_s_bytes, k, out_ptr, out_dtype, ld_out, stream)
     check(rc, "MXFP4 product launch")
 
 
 def cache_write(cache: Cache, k_ptr: int, k_token: int, k_head: int, v_ptr: int, v_token: int, v_head: int, dtype: int,
                 tokens: int, slots_ptr: int, stream: int) -> None:
-    rc = lib().mxfp8_cache_write(cache, k_ptr or None, k_token, k_head, v_ptr or None, v_token, v_head, dtype, tokens,
-                                 slots_ptr or None, stream or None)
+    rc = lib().mxfp8_cache_write(cache, k_ptr, k_token, k_head, v_ptr, v_token, v_head, dtype, tokens,
+                                 slots_ptr, stream)
     check(rc, "cache write launch")
 
 
 def cache_read(cache: Cache, table_ptr: int, table_stride: int, max_pages: int, batch: int, starts_ptr: int, total: int,
                k_out_ptr: int, v_out_ptr: int, out_dtype: int, stream: int) -> None:
-    rc = lib().mxfp8_cache_read(cache, table_ptr or None, table_stride, max_pages, batch, starts_ptr or None, total,
-                                k_out_ptr or None, v_out_ptr or None, out_dtype, stream or None)
+    rc = lib().mxfp8_cache_read(cache, table_ptr, table_stride, max_pages, batch, starts_ptr, total,
+                                k_out_ptr, v_out_ptr, out_dtype, stream)
     check(rc, "cache read launch")
 
 
@@ -250,9 +250,9 @@ def cache_attention_workspace(cache: Cache, batch: int, q_heads: int) -> int:
 def cache_attention(cache: Cache, q_ptr: int, q_batch: int, q_head: int, dtype: int, batch: int, q_heads: int,
                     table_ptr: int, table_stride: int, max_pages: int, lengths_ptr: int, scale: float, out_ptr: int,
                     lse_ptr: int, workspace_ptr: int, workspace_bytes: int, stream: int) -> None:
-    rc = lib().mxfp8_cache_attention(cache, q_ptr or None, q_batch, q_head, dtype, batch, q_heads, table_ptr or None,
-                                     table_stride, max_pages, lengths_ptr or None, scale, out_ptr or None,
-                                     lse_ptr or None, workspace_ptr or None, workspace_bytes, stream or None)
+    rc = lib().mxfp8_cache_attention(cache, q_ptr, q_batch, q_head, dtype, batch, q_heads, table_ptr,
+                                     table_stride, max_pages, lengths_ptr, scale, out_ptr,
+                                     lse_ptr, workspace_ptr, workspace_bytes, stream)
     check(rc, "cache attention launch")
 
 

@@ -10,6 +10,12 @@ from . import _capi
 
 _NOTHING = contextlib.nullcontext()
 
+# Handle of a device's current stream without a Stream object around it: a call
+# of these operators costs the host about as much as a small one costs the GPU,
+# and torch.cuda.current_stream alone took 2.2 of 16 us.
+_current_stream_handle = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
 IN_DTYPES = {torch.bfloat16: _capi.BF16, torch.float16: _capi.FP16}
 OUT_DTYPES = {torch.bfloat16: _capi.BF16, torch.float16: _capi.FP16, torch.float32: _capi.F32}
 
@@ -38,19 +44,19 @@ def on_stream(stream, first: torch.Tensor, *others: torch.Tensor):
     tensors are recorded on it: their memory is not reused before the launch
     is done, even if the caller drops them.  The caller orders the stream
     after the work that makes the inputs."""
-    device = first.device
-    if device.type != "cuda":
-        raise ValueError(f"the operator runs on CUDA tensors, got one on {device}")
+    index = first.get_device()
+    if index < 0:
+        raise ValueError(f"the operator runs on CUDA tensors, got one on {first.device}")
     for t in others:
-        if t.device != device:
-            raise ValueError(f"all tensors must be on {device}, got one on {t.device}")
+        if t.get_device() != index:
+            raise ValueError(f"all tensors must be on {first.device}, got one on {t.device}")
     if stream is None:
-        context = _NOTHING if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-        return context, torch.cuda.current_stream(device).cuda_stream
+        context = _NOTHING if torch.cuda.current_device() == index else torch.cuda.device(index)
+        return context, _current_stream_handle(index)
     if not isinstance(stream, torch.cuda.Stream):
-        stream = torch.cuda.ExternalStream(int(stream), device=device)
-    if stream.device != device:
-        raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
+        stream = torch.cuda.ExternalStream(int(stream), device=first.device)
+    if stream.device.index != index:
+        raise ValueError(f"the stream is on {stream.device}, the tensors on {first.device}")
     for t in (first, *others):
         t.record_stream(stream)
     return torch.cuda.stream(stream), stream.cuda_stream

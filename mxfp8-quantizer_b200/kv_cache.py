@@ -57,7 +57,7 @@ def _describe(cache: MXFP8Cache) -> _capi.Cache:
                          f"{tuple(v.shape)} {v.dtype}")
     pages, heads, page_size, dim = shape
     scale_shape = (pages, heads, page_size, dim // SCALE_BLOCK)
-    if dim % SCALE_BLOCK or tuple(k_scales.shape) != scale_shape or tuple(v_scales.shape) != scale_shape:
+    if dim % SCALE_BLOCK or k_scales.shape != scale_shape or v_scales.shape != scale_shape:
         raise ValueError(f"the scales must be {scale_shape} for dim a multiple of 32, got {tuple(k_scales.shape)} and "
                          f"{tuple(v_scales.shape)}")
     if k_scales.element_size() != 1 or v_scales.element_size() != 1:
@@ -69,23 +69,25 @@ def _describe(cache: MXFP8Cache) -> _capi.Cache:
 
 
 def _check_index(name: str, t: torch.Tensor, dtype: torch.dtype, dims: int) -> None:
-    if t.dtype != dtype or t.dim() != dims or (t.stride(-1) != 1 and t.shape[-1] > 1):
+    if t.dtype != dtype or t.dim() != dims or (t.stride()[-1] != 1 and t.shape[-1] > 1):
         raise ValueError(f"{name} must be a {dims}-D {dtype} tensor with a contiguous last dimension, got "
                          f"{tuple(t.shape)} {t.dtype}")
 
 
 def _check_rows(name: str, t: torch.Tensor, heads: int | None, dim: int) -> None:
-    if t.dim() != 3 or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{name} must be (rows, {'heads' if heads is None else heads}, {dim}), got {tuple(t.shape)}")
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != dim or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{name} must be (rows, {'heads' if heads is None else heads}, {dim}), got {tuple(shape)}")
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t with a contiguous last dimension."""
-    return t if t.stride(2) == 1 else t.contiguous()
+    return t if t.stride()[2] == 1 else t.contiguous()
 
 
 def _table_stride(table: torch.Tensor) -> int:
-    return table.stride(0) if table.shape[0] > 1 else table.shape[1]
+    batch, width = table.shape
+    return table.stride()[0] if batch > 1 else width
 
 
 def cache_write(cache: MXFP8Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, stream=None) -> None:
@@ -107,8 +109,10 @@ def cache_write(cache: MXFP8Cache, k: torch.Tensor, v: torch.Tensor, slots: torc
     context, handle = on_stream(stream, k, v, slots, *cache)
     with context:
         k, v = _rows(k), _rows(v)
-        _capi.cache_write(shape, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), code,
-                          tokens, slots.data_ptr(), handle)
+        k_token, k_head, _ = k.stride()
+        v_token, v_head, _ = v.stride()
+        _capi.cache_write(shape, k.data_ptr(), k_token, k_head, v.data_ptr(), v_token, v_head, code, tokens,
+                          slots.data_ptr(), handle)
 
 
 def cache_read(cache: MXFP8Cache, page_table: torch.Tensor, starts: torch.Tensor, total: int,
@@ -139,7 +143,8 @@ def cache_read(cache: MXFP8Cache, page_table: torch.Tensor, starts: torch.Tensor
     context, handle = on_stream(stream, page_table, starts, *cache, *(out or ()))
     with context:
         if out is None:
-            out = tuple(torch.empty(want, dtype=out_dtype, device=page_table.device) for _ in range(2))
+            k_out = torch.empty(*want, dtype=out_dtype, device=page_table.device)
+            out = k_out, torch.empty_like(k_out)
         _capi.cache_read(shape, page_table.data_ptr(), _table_stride(page_table), max_pages, batch, starts.data_ptr(),
                          total, out[0].data_ptr(), out[1].data_ptr(), code, handle)
     return out[0], out[1]
@@ -173,13 +178,14 @@ def cache_attention(q: torch.Tensor, cache: MXFP8Cache, page_table: torch.Tensor
     context, handle = on_stream(stream, q, page_table, lengths, *cache)
     with context:
         q = _rows(q)
+        q_batch, q_head, _ = q.stride()
         device = q.device
-        out = torch.empty((batch, q_heads, shape.dim), dtype=q.dtype, device=device)
-        lse = torch.empty((batch, q_heads), dtype=torch.float32, device=device) if return_lse else None
+        out = torch.empty(batch, q_heads, shape.dim, dtype=q.dtype, device=device)
+        lse = torch.empty(batch, q_heads, dtype=torch.float32, device=device) if return_lse else None
         size = _capi.cache_attention_workspace(shape, batch, q_heads)
-        workspace = torch.empty((size,), dtype=torch.uint8, device=device)
-        _capi.cache_attention(shape, q.data_ptr(), q.stride(0), q.stride(1), code, batch, q_heads,
-                              page_table.data_ptr(), _table_stride(page_table), page_table.shape[1],
-                              lengths.data_ptr(), 1.0 / math.sqrt(shape.dim) if scale is None else scale,
-                              out.data_ptr(), 0 if lse is None else lse.data_ptr(), workspace.data_ptr(), size, handle)
+        workspace = torch.empty(size, dtype=torch.uint8, device=device)
+        _capi.cache_attention(shape, q.data_ptr(), q_batch, q_head, code, batch, q_heads, page_table.data_ptr(),
+                              _table_stride(page_table), page_table.shape[1], lengths.data_ptr(),
+                              1.0 / math.sqrt(shape.dim) if scale is None else scale, out.data_ptr(),
+                              0 if lse is None else lse.data_ptr(), workspace.data_ptr(), size, handle)
     return (out, lse) if return_lse else out

@@ -21,11 +21,12 @@ _PAYLOAD_DTYPES = (torch.uint8, torch.int8, torch.float4_e2m1fn_x2)
 
 def _check_payload(name: str, q: torch.Tensor) -> tuple[int, int]:
     """(rows, cols) of an MXFP4 payload."""
-    if q.dim() != 2 or q.dtype not in _PAYLOAD_DTYPES or (q.stride(1) != 1 and q.shape[1] > 1):
+    if q.dim() != 2 or q.dtype not in _PAYLOAD_DTYPES or (q.stride()[1] != 1 and q.shape[1] > 1):
         raise ValueError(f"{name} must be a row-major matrix of bytes, got {tuple(q.shape)} {q.dtype}")
-    if q.shape[1] % 16:
-        raise ValueError(f"{name} must have a multiple of 32 columns (16 bytes), got {2 * q.shape[1]}")
-    return q.shape[0], 2 * q.shape[1]
+    rows, row_bytes = q.shape
+    if row_bytes % 16:
+        raise ValueError(f"{name} must have a multiple of 32 columns (16 bytes), got {2 * row_bytes}")
+    return rows, 2 * row_bytes
 
 
 def _check_scales(name: str, s: torch.Tensor) -> None:
@@ -36,7 +37,9 @@ def _check_scales(name: str, s: torch.Tensor) -> None:
 
 def _row_stride(t: torch.Tensor) -> int:
     """Row stride, also of a matrix whose single row carries none."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    rows, cols = t.shape
+    row = t.stride()[0]
+    return row if rows > 1 else max(row, cols)
 
 
 def quantize_mxfp4(x: torch.Tensor, q: torch.Tensor | None = None, s: torch.Tensor | None = None, stream=None):
@@ -53,18 +56,18 @@ def quantize_mxfp4(x: torch.Tensor, q: torch.Tensor | None = None, s: torch.Tens
     code = in_dtype("X", x.dtype)
     m, k = x.shape
     q_cols = -(-k // 32) * 32
-    given = [t for t in (q, s) if t is not None]
-    context, handle = on_stream(stream, x, *given)
+    context, handle = on_stream(stream, x, *(t for t in (q, s) if t is not None))
     with context:
-        if (x.stride(1) != 1 and k > 1) or (m > 1 and x.stride(0) < k):
+        row, col = x.stride()
+        if (col != 1 and k > 1) or (m > 1 and row < k):
             x = x.contiguous()
         if q is None:
-            q = torch.empty((m, q_cols // 2), dtype=torch.uint8, device=x.device)
+            q = torch.empty(m, q_cols // 2, dtype=torch.uint8, device=x.device)
         elif _check_payload("q", q) != (m, q_cols):
             raise ValueError(f"q must be ({m}, {q_cols // 2}) bytes, got {tuple(q.shape)}")
         need = -(-m // 128) * 128 * (-(-q_cols // 128) * 4)
         if s is None:
-            s = torch.empty((need,), dtype=torch.uint8, device=x.device)
+            s = torch.empty(need, dtype=torch.uint8, device=x.device)
         else:
             _check_scales("s", s)
         _capi.fp4_quantize(x.data_ptr(), code, m, k, _row_stride(x), q.data_ptr(), _row_stride(q), s.data_ptr(),
@@ -79,7 +82,7 @@ def dequantize_mxfp4(q: torch.Tensor, s: torch.Tensor, out_dtype: torch.dtype = 
     code = out_dtype_code(out_dtype)
     context, handle = on_stream(stream, q, s)
     with context:
-        out = torch.empty((rows, cols), dtype=out_dtype, device=q.device)
+        out = torch.empty(rows, cols, dtype=out_dtype, device=q.device)
         _capi.fp4_dequantize(q.data_ptr(), rows, cols, _row_stride(q), s.data_ptr(), s.numel(), out.data_ptr(), code,
                              cols, handle)
     return out
@@ -109,7 +112,7 @@ def mxfp4_gemm(a_q: torch.Tensor, b_q: torch.Tensor, a_s: torch.Tensor, b_s: tor
     context, handle = on_stream(stream, a_q, b_q, a_s, b_s, *(() if out is None else (out,)))
     with context:
         if out is None:
-            out = torch.empty((m, n), dtype=out_dtype, device=a_q.device)
+            out = torch.empty(m, n, dtype=out_dtype, device=a_q.device)
         _capi.fp4_gemm(a_q.data_ptr(), m, _row_stride(a_q), a_s.data_ptr(), a_s.numel(), b_q.data_ptr(), n,
                        _row_stride(b_q), b_s.data_ptr(), b_s.numel(), k, out.data_ptr(), code, _row_stride(out), handle)
     return out
