@@ -11,21 +11,22 @@
 //     (largest element in [2^14, 2^15)): a bf16 or fp16 value is exact there
 //     down to 2^-38 of the head's largest.
 //   sum_j p_j v_j: p_j 2^(sv - 127) is the operand, as p_j 2^(sv - R + 15) in
-//     f16 with R the largest V scale byte met so far: 2^-12 of relative error
-//     for every term within 29 binades of the largest possible one, terms below
-//     lose bits gradually; the accumulator is rescaled when R grows.
+//     f16 with R the largest V scale byte met so far: 2^-11 of relative error at
+//     most for every term within 29 binades of the largest possible one, terms
+//     below lose bits gradually; the accumulator is rescaled when R grows.
 // The m16n8k16 shapes are used because a decode step has at most 16 rows of
 // queries: a 128-row tcgen05 tile would be empty to 7/8 and would want K and V
 // converted into shared memory first.
 //
-// Work: tiles of 64 positions, of all sequences and KV heads in a row, are
-// split evenly over the CTAs whatever the lengths are.  A warp owns 16
-// positions of every tile: it fetches them (cp.async into a ring of its own,
-// no block-wide barriers), computes the scores with heads as rows and positions
-// as columns, which is the layout the second product takes its operand in, and
-// keeps its own running maximum and sums.  Where a CTA leaves a (sequence, KV
-// head) its warps join; if it did not hold all of its tiles, the unscaled sums go
-// to the workspace, and a second launch joins those.
+// Work: the tiles (POS positions) of all sequences and KV heads in a row are
+// split evenly over the warps, whatever the lengths are; a change of sequence
+// or head counts as kSegmentCost tiles.  A warp is on its own: it fetches its
+// tiles (cp.async into a ring of its own, no block-wide barrier anywhere),
+// computes the scores with heads as rows and positions as columns, which is
+// the layout the second product takes its operand in, and keeps its running
+// maximum and sums.  A (sequence, KV head) that one warp holds whole is
+// written at once; pieces of the others go to the workspace, unscaled, and a
+// second launch joins them in order, so the result does not depend on timing.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -43,10 +44,10 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kWarpPos = 16;                  // positions of a warp in a tile
-constexpr int kTilePos = kWarps * kWarpPos;
+constexpr int kSegmentCost = 1;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr uint32_t kNoRow32 = 0xFFFFFFFFu;
 
 // Heads in groups of 8 * NT rows: 16 where that saves a second pass over K and
 // V and the accumulators fit the registers.
@@ -55,40 +56,34 @@ inline int row_tiles(int dim, int group) { return group > 8 && dim <= 128 ? 2 : 
 template <int D, int NT>
 struct Config {
     static constexpr int rows = 8 * NT;
-    static constexpr int kv_bytes = kWarpPos * D;             // K (or V) payload of a warp's positions
-    static constexpr int sc_bytes = kWarpPos * D / 32;
+    static constexpr int pos = D <= 128 ? 32 : 16;            // positions of a tile
+    static constexpr int kv_bytes = pos * D;                  // K (or V) payload of a tile
+    static constexpr int sc_bytes = pos * D / 32;
     static constexpr int stage_bytes = 2 * kv_bytes + 2 * sc_bytes;
-    static constexpr int stages = D <= 64 ? 6 : D <= 128 ? 4 : 3;
-    static constexpr int f_floats = D / 32 * kWarpPos;        // scale factors of a warp's positions
-    static constexpr int warp_bytes = stages * stage_bytes + 2 * f_floats * 4;
-    static constexpr int join_off = kWarps * warp_bytes;
-    static constexpr int ml_off = join_off + rows * D * 4;    // then m and l of every warp and row
-    static constexpr int smem = ml_off + kWarps * rows * 8;
-    static constexpr int ctas_per_sm = smem * 3 <= 225 * 1024 ? 3 : 2;
+    static constexpr int stages = D <= 64 ? 4 : D <= 128 ? 2 : 3;
+    static constexpr int warp_bytes = stages * stage_bytes;
+    static constexpr int smem = kWarps * warp_bytes;
+    static constexpr int ctas_per_sm = D <= 128 && NT == 1 ? 3 : 2;
 };
 
 struct Params {
     CacheAttentionArgs a;
     int group;        // query heads of a KV head
     int row_groups;   // ceil(group / rows)
-    int64_t grid;     // CTAs
-    float* part_o;    // (2 * grid, rows, D): unscaled sums of the pieces
-    float2* part_ml;  // (2 * grid, rows): running maximum (log2) and sum
-    int2* meta;       // (batch * heads * row_groups): first and last CTA of a split segment
+    int64_t parts;    // warps
+    float* part_o;    // (2 * parts, rows, D): unscaled sums of the pieces
+    float2* part_ml;  // (2 * parts, rows): running maximum (log2) and sum
+    int2* meta;       // (batch * heads * row_groups): first and last warp of a split segment
 };
-
-// A place in the sequence of all tiles: sequence b, head group g (KV head and
-// row group), tile t of nt.
-struct Cursor {
-    int64_t b;
-    int g, t, nt, len;
-};
-
-__device__ __forceinline__ int tiles_of(int len) { return (len + kTilePos - 1) / kTilePos; }
 
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, d));
+    return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
     return v;
 }
 
@@ -96,20 +91,60 @@ __device__ __forceinline__ int length_of(const CacheAttentionArgs& a, int64_t b)
     return (int)visible_length(a.lengths[b], a.max_pages, a.c.page_shift);
 }
 
-// To the next tile; sequences without tiles are passed over.
-__device__ __forceinline__ void advance(const Params& p, Cursor& c, int groups) {
-    if (++c.t < c.nt) return;
-    c.t = 0;
-    if (++c.g < groups) return;
-    c.g = 0;
+// Cost of a sequence's segment: its tiles and the change to it, 0 if empty.
+template <int POS>
+__device__ __forceinline__ int cost_of(int len) {
+    return len == 0 ? 0 : (len + POS - 1) / POS + kSegmentCost;
+}
+
+// A warp's place: sequence b, head group g (KV head and row group), tile t of
+// its tiles t0 .. t1 - 1 of that segment's nt; `base` is the segment's place
+// in the sum of all costs, `end` the end of the warp's share of it.
+struct Cursor {
+    int64_t base, end, b;
+    const int32_t* pages;
+    int g, t, t0, t1, nt, len;
+    bool done;
+};
+
+// The warp's tiles of the cursor's segment; true if there are any.
+__device__ __forceinline__ bool enter(Cursor& c, int64_t begin) {
+    const int64_t first = c.base + kSegmentCost;
+    c.t0 = begin > first ? (int)(begin - first) : 0;
+    c.t1 = c.end - first < c.nt ? (int)(c.end - first) : c.nt;
+    c.t = c.t0;
+    return c.t0 < c.t1;
+}
+
+template <int POS>
+__device__ __forceinline__ void enter_sequence(const Params& p, Cursor& c) {
+    c.len = length_of(p.a, c.b);
+    c.nt = (c.len + POS - 1) / POS;
+    c.pages = p.a.table + c.b * p.a.table_stride;
+}
+
+// To the next segment in which the warp has tiles.
+template <int POS>
+__device__ __forceinline__ void next_segment(const Params& p, Cursor& c, int groups) {
     do {
-        if (++c.b >= p.a.batch) {
-            c.nt = 0;
+        c.base += c.nt + kSegmentCost;
+        if (c.base + kSegmentCost >= c.end) {
+            c.done = true;
             return;
         }
-        c.len = length_of(p.a, c.b);
-        c.nt = tiles_of(c.len);
-    } while (c.nt == 0);
+        if (++c.g == groups) {
+            c.g = 0;
+            do {  // total cost is not exhausted: there is another sequence with tiles
+                ++c.b;
+                enter_sequence<POS>(p, c);
+            } while (c.nt == 0);
+        }
+    } while (!enter(c, c.base));
+}
+
+template <int POS>
+__device__ __forceinline__ void advance(const Params& p, Cursor& c, int groups) {
+    if (++c.t == c.t1) next_segment<POS>(p, c, groups);
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
@@ -138,6 +173,14 @@ __device__ __forceinline__ void e4m3x4_to_half2(uint32_t w, uint32_t& lo, uint32
         : "r"(w));
 }
 
+// Four UE8M0 bytes as bf16 pairs: 2^(byte - 127), NaN for 255; exact.
+__device__ __forceinline__ void ue8m0x4_to_bf162(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
+        "cvt.rn.bf16x2.ue8m0x2 %0, a;\n\tcvt.rn.bf16x2.ue8m0x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
+}
+
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
@@ -150,8 +193,13 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     const __half2 t = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&t);
 }
+__device__ __forceinline__ uint32_t pack_out(bool bf16, float lo, float hi) {
+    if (!bf16) return pack_half2(lo, hi);
+    const __nv_bfloat162 t = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&t);
+}
 
-// Shared memory of a warp's 16 rows of D bytes: 32-byte groups of a row are
+// Shared memory of a tile's rows of D bytes: 32-byte groups of a row are
 // permuted so that the four rows that one access phase reads (K: rows r .. r +
 // 3, V: the same after v_place) fall on different banks.
 template <int D>
@@ -159,47 +207,53 @@ __device__ __forceinline__ uint32_t group_at(int row, int group) {
     const int key = D % 128 == 0 ? (row & 3) : ((row >> 1) & 1);
     return (uint32_t)(row * D + ((group ^ key) << 5));
 }
-// Row that position j of V is kept in: the positions 2c + i, c = 0 .. 3, that
-// a phase of the second product reads are neighbours.
-__device__ __forceinline__ int v_place(int j) { return (j >> 1) | ((j & 1) << 3); }
+// Row that position j of V is kept in: of each 16, the positions 2c + i, c = 0
+// .. 3, that a phase of the second product reads are neighbours.
+__device__ __forceinline__ int v_place(int j) { return (j & ~15) | ((j & 15) >> 1) | ((j & 1) << 3); }
 
-// Positions 16 w .. 16 w + 15 of the cursor's tile: the cache row of position
-// lane (kNoRow where there is none), for lanes below 16.
-__device__ __forceinline__ int64_t row_of_lane(const Params& p, const Cursor& c, int warp, int lane) {
-    if (c.nt == 0 || lane >= kWarpPos) return kNoRow;
-    const int at = c.t * kTilePos + warp * kWarpPos + lane;
-    if (at >= c.len) return kNoRow;
-    const int64_t page = table_page(p.a.table, p.a.table_stride, p.a.max_pages, c.b, at, p.a.c.page_shift);
-    const int64_t row = cache_row(p.a.c, page, c.g / p.row_groups, at & ((1 << p.a.c.page_shift) - 1));
-    if (row == kNoRow && p.a.status) atomicOr(p.a.status, kErrCacheIndex);
-    return row;
+// Cache row of position `lane` of the cursor's tile, kNoRow32 where there is none.
+template <int POS>
+__device__ __forceinline__ uint32_t row_of_lane(const Params& p, const Cursor& c, int lane) {
+    const int at = c.t * POS + lane;
+    if (c.done || lane >= POS || at >= c.len) return kNoRow32;
+    const uint32_t page = (uint32_t)c.pages[at >> p.a.c.page_shift];  // the length is within the table
+    if (page >= (uint64_t)p.a.c.num_pages) {
+        if (p.a.status) atomicOr(p.a.status, kErrCacheIndex);
+        return kNoRow32;
+    }
+    return (uint32_t)cache_row(p.a.c, page, c.g / p.row_groups, at & ((1 << p.a.c.page_shift) - 1));
 }
 
-// Fetch those positions into a stage: payloads 16 bytes a lane, scales four
-// bytes a lane (two positions' scale bytes are 4, 8, 12 or 16 contiguous ones:
-// pages hold an even number of positions).  Absent positions are zeros.
-template <int D>
-__device__ __forceinline__ void fetch(const Params& p, uint32_t stage, int64_t my_row, int lane) {
+// Fetch those rows into a stage: payloads 16 bytes a lane, scales four bytes a
+// lane (two positions' scale bytes are 4, 8, 12 or 16 contiguous ones: pages
+// hold an even number of positions).  Absent positions are zeros.
+template <int D, int POS>
+__device__ __forceinline__ void fetch(const Params& p, uint32_t stage, uint32_t my_row, int lane) {
     constexpr int kChunks = D / 16;  // of a row
-    constexpr int kKv = kWarpPos * D;
+    constexpr int kKv = POS * D;
 #pragma unroll
     for (int i = 0; i < kKv / 512; ++i) {
         const int idx = i * 32 + lane;
         const int j = idx / kChunks, ch = idx - j * kChunks;
-        const int64_t row = __shfl_sync(0xFFFFFFFFu, my_row, j);
-        const bool on = row != kNoRow;
-        const int64_t off = on ? row * D + ch * 16 : 0;
+        const uint32_t row = __shfl_sync(0xFFFFFFFFu, my_row, j);
+        const bool on = row != kNoRow32;
+        const uint64_t off = (uint64_t)(on ? row : 0u) * D + ch * 16;
         cp_async16(stage + group_at<D>(j, ch >> 1) + (ch & 1) * 16, p.a.k + off, on);
         cp_async16(stage + kKv + group_at<D>(v_place(j), ch >> 1) + (ch & 1) * 16, p.a.v + off, on);
     }
     constexpr int kPair = D / 64;    // 4-byte pieces of two positions' scales
-    const int pair = lane / kPair, in = lane - pair * kPair;
-    const int64_t even = __shfl_sync(0xFFFFFFFFu, my_row, (2 * pair) & 15);
-    if (lane < kWarpPos / 2 * kPair) {
-        const bool on = even != kNoRow;
-        const int64_t off = on ? even * (D / 32) + in * 4 : 0;
-        cp_async4(stage + 2 * kKv + lane * 4, p.a.k_scales + off, on);
-        cp_async4(stage + 2 * kKv + kWarpPos * D / 32 + lane * 4, p.a.v_scales + off, on);
+    constexpr int kPieces = POS / 2 * kPair;
+#pragma unroll
+    for (int i = 0; i < (kPieces + 31) / 32; ++i) {
+        const int idx = i * 32 + lane;
+        const int pair = idx / kPair, in = idx - pair * kPair;
+        const uint32_t even = __shfl_sync(0xFFFFFFFFu, my_row, (2 * pair) & (POS - 1));
+        if (kPieces % 32 == 0 || idx < kPieces) {
+            const bool on = even != kNoRow32;
+            const uint64_t off = (uint64_t)(on ? even : 0u) * (D / 32) + in * 4;
+            cp_async4(stage + 2 * kKv + idx * 4, p.a.k_scales + off, on);
+            cp_async4(stage + 2 * kKv + POS * D / 32 + idx * 4, p.a.v_scales + off, on);
+        }
     }
 }
 
@@ -256,23 +310,33 @@ __device__ __forceinline__ void load_query(const Params& p, const Cursor& c, int
     }
 }
 
+// Scale bytes of positions 2 q and 2 q + 1 of eight (those of the quad's
+// columns), as halves of two blocks each: w[0 .. NB/2 - 1] the first's.
+template <int NB>
+__device__ __forceinline__ void load_scale_pair(const uint8_t* src, uint32_t (&w)[NB / 2]) {
+#pragma unroll
+    for (int i = 0; i < NB / 2; ++i) w[i] = reinterpret_cast<const uint32_t*>(src)[i];
+}
+
 template <int D, int NT>
 __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_attention_kernel(const Params p) {
     using C = Config<D, NT>;
-    constexpr int kBlocks = D / 32;
+    constexpr int POS = C::pos, kCols = POS / 8;   // positions in columns of eight
+    constexpr int kBlocks = D / 32, kWords = kBlocks / 2;
+    constexpr uint32_t kFull = POS == 32 ? 0xFFFFFFFFu : (1u << POS) - 1u;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int64_t scan_s[kWarps];
-    __shared__ int64_t found_b, found_base;
+    __shared__ int64_t found_b[kWarps], found_base[kWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = lane >> 2, quad = lane & 3;
     const int groups = p.a.c.heads * p.row_groups;
 
     grid_wait_prerequisites();
-    // ---- this CTA's share of all tiles, and where it begins ----
+    // ---- the warps' shares of all costs, and the sequences where they begin ----
     const int64_t per = (p.a.batch + kThreads - 1) / kThreads;
     const int64_t b0 = min(p.a.batch, per * threadIdx.x), b1 = min(p.a.batch, b0 + per);
     int64_t mine = 0;
     for (int64_t b = b0; b < b1; ++b) {
-        mine += tiles_of(length_of(p.a, b));
+        mine += cost_of<POS>(length_of(p.a, b));
         if (blockIdx.x == 0 && p.a.status && (int64_t)p.a.lengths[b] > (p.a.max_pages << p.a.c.page_shift))
             atomicOr(p.a.status, kErrCacheIndex);
     }
@@ -284,57 +348,59 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
     }
     if (lane == 31) scan_s[warp] = upto;
     __syncthreads();
-    int64_t before = 0, tiles = 0;
+    int64_t before = 0, cost = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
         if (w < warp) before += scan_s[w];
-        tiles += scan_s[w];
+        cost += scan_s[w];
     }
-    const int64_t total = tiles * groups;
-    const int64_t parts = min(p.grid, total);
-    const int64_t cta = blockIdx.x;
-    if (cta >= parts) return;
-    const int64_t x0 = split_begin(cta, parts, total), x1 = split_begin(cta + 1, parts, total);
-    int64_t at = (before + upto - mine) * groups;  // first tile of this thread's first sequence
-    if (at <= x0 && x0 < at + mine * groups) {
-        int64_t b = b0;
-        for (;; ++b) {
-            const int64_t n = (int64_t)tiles_of(length_of(p.a, b)) * groups;
-            if (x0 < at + n) break;
-            at += n;
+    const int64_t total = cost * groups;
+    const int64_t parts = min(p.parts, total);
+    const int64_t first_part = (int64_t)blockIdx.x * kWarps;
+    if (first_part >= parts) return;
+    const int64_t from = (before + upto - mine) * groups;  // place of this thread's first sequence
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        const int64_t x = split_begin(first_part + w, parts, total);
+        if (first_part + w < parts && from <= x && x < from + mine * groups) {
+            int64_t at = from;
+            int64_t b = b0;
+            for (;; ++b) {
+                const int64_t n = (int64_t)cost_of<POS>(length_of(p.a, b)) * groups;
+                if (x < at + n) break;
+                at += n;
+            }
+            found_b[w] = b;
+            found_base[w] = at;
         }
-        found_b = b;
-        found_base = at;
     }
     __syncthreads();
+    const int64_t part = first_part + warp;
+    if (part >= parts) return;
     Cursor cur;  // the tile that is computed
-    cur.b = found_b;
-    cur.len = length_of(p.a, cur.b);
-    cur.nt = tiles_of(cur.len);
-    int64_t seg0 = found_base + (x0 - found_base) / cur.nt * cur.nt;  // first tile of the segment
-    cur.g = (int)((x0 - found_base) / cur.nt);
-    cur.t = (int)(x0 - seg0);
+    const int64_t begin = split_begin(part, parts, total);
+    cur.end = split_begin(part + 1, parts, total);
+    cur.b = found_b[warp];
+    enter_sequence<POS>(p, cur);
+    cur.g = (int)((begin - found_base[warp]) / (cur.nt + kSegmentCost));
+    cur.base = found_base[warp] + (int64_t)cur.g * (cur.nt + kSegmentCost);
+    cur.done = false;
+    if (!enter(cur, begin)) next_segment<POS>(p, cur, groups);
 
     uint8_t* const ring = smem + warp * C::warp_bytes;
     const uint32_t ring_u = smem_u32(ring);
-    float* const kf = reinterpret_cast<float*>(ring + C::stages * C::stage_bytes);  // [block][position]
-    float* const vf = kf + C::f_floats;
 
     // ---- fetch ahead: `next` is the tile whose rows are looked up in my_row ----
     Cursor next = cur;
-    int64_t next_x = x0;
-    int64_t my_row = row_of_lane(p, next, warp, lane);
+    uint32_t my_row = row_of_lane<POS>(p, next, lane);
     uint32_t present = 0;  // lane s: which positions of stage s are there
     auto issue = [&](int stage) {
-        if (next_x < x1) {
-            fetch<D>(p, ring_u + stage * C::stage_bytes, my_row, lane);
-            const uint32_t mask = __ballot_sync(0xFFFFFFFFu, my_row != kNoRow);
+        if (!next.done) {
+            const uint32_t mask = __ballot_sync(0xFFFFFFFFu, my_row != kNoRow32);
+            if (mask != 0) fetch<D, POS>(p, ring_u + stage * C::stage_bytes, my_row, lane);
             if (lane == stage) present = mask;
-            ++next_x;
-            if (next_x < x1) {
-                advance(p, next, groups);
-                my_row = row_of_lane(p, next, warp, lane);
-            }
+            advance<POS>(p, next, groups);
+            my_row = row_of_lane<POS>(p, next, lane);
         }
         cp_async_commit();
     };
@@ -344,14 +410,14 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
     uint32_t qf[D / 16][2 * NT];
     float mul[NT], m[NT], l[NT];
     float acc[NT][D / 16][4];
-    uint32_t ref = 0;  // R: the largest V scale byte so far
+    int ref = 15;  // R: the largest V scale byte so far, and at least 15
     bool fresh = true;
 
     int stage = 0;
-    for (int64_t x = x0; x < x1; ++x) {
+    while (!cur.done) {
         if (fresh) {
             load_query<D, NT>(p, cur, lane, qf, mul);
-            ref = 0;
+            ref = 15;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 m[n] = -INFINITY;
@@ -365,54 +431,28 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
         }
         cp_async_wait<C::stages - 2>();
         __syncwarp();  // also: the stage before this one is read, it can be filled again
-        const uint32_t mask = __shfl_sync(0xFFFFFFFFu, present, stage) & 0xFFFFu;
+        const uint32_t mask = __shfl_sync(0xFFFFFFFFu, present, stage);
         issue(stage == 0 ? C::stages - 1 : stage - 1);
         const uint8_t* st = ring + stage * C::stage_bytes;
         if (mask != 0) {
-            // ---- scale factors: f32 of K's, and the largest byte of V's ----
-            constexpr int kPer = kWarpPos * kBlocks / 32;  // bytes a lane
-            const uint8_t* ks = st + 2 * C::kv_bytes;
+            const uint8_t* ks = st + 2 * C::kv_bytes + quad * (2 * kBlocks);
             const uint8_t* vs = ks + C::sc_bytes;
-            uint32_t vb[kPer], top = 0;
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                const int idx = i * 32 + lane, j = idx / kBlocks, blk = idx - j * kBlocks;
-                kf[blk * kWarpPos + j] = ue8m0_value(ks[idx]);
-                vb[i] = (mask >> j) & 1 ? vs[idx] : 0u;
-                if (vb[i] != 255u) top = max(top, vb[i]);
-            }
-            top = __reduce_max_sync(0xFFFFFFFFu, top);
-            if (top > ref) {
-                const float down = exp2_fast(-(float)(top - ref));  // acc is in units of 2^(ref - 142)
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) acc[n][i][j] *= down;
-                ref = top;
-            }
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                const int idx = i * 32 + lane, j = idx / kBlocks, blk = idx - j * kBlocks;
-                const int e = (int)vb[i] - (int)ref + 15 + 127;
-                const float f = __uint_as_float(vb[i] == 255u ? 0x7FC00000u : (uint32_t)max(e, 0) << 23);
-                vf[blk * kWarpPos + j] = f;
-            }
-            __syncwarp();
-
             // ---- scores: rows are heads, columns positions 8 nt + 2 quad + {0, 1} ----
-            float s[2][4];
+            float s[kCols][2 * NT];
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt) {
+            for (int nt = 0; nt < kCols; ++nt) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) s[nt][j] = 0.0f;
+                for (int j = 0; j < 2 * NT; ++j) s[nt][j] = 0.0f;
+                uint32_t w[kWords], f[kBlocks];  // f: bf16 factors, blocks in pairs, both positions
+                load_scale_pair<kBlocks>(ks + nt * 8 * kBlocks, w);
+#pragma unroll
+                for (int i = 0; i < kWords; ++i) ue8m0x4_to_bf162(w[i], f[2 * i], f[2 * i + 1]);
 #pragma unroll
                 for (int blk = 0; blk < kBlocks; ++blk) {
-                    const uint2 w = *reinterpret_cast<const uint2*>(st + group_at<D>(nt * 8 + row, blk) + quad * 8);
+                    const uint2 b = *reinterpret_cast<const uint2*>(st + group_at<D>(nt * 8 + row, blk) + quad * 8);
                     uint32_t b0, b1, b2, b3;
-                    e4m3x4_to_half2(w.x, b0, b1);
-                    e4m3x4_to_half2(w.y, b2, b3);
+                    e4m3x4_to_half2(b.x, b0, b1);
+                    e4m3x4_to_half2(b.y, b2, b3);
                     float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                     if constexpr (NT == 1) {
                         mma_f16(d, qf[2 * blk][0], 0u, qf[2 * blk][1], 0u, b0, b1);
@@ -422,37 +462,47 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
                         mma_f16(d, qf[2 * blk + 1][0], qf[2 * blk + 1][2], qf[2 * blk + 1][1], qf[2 * blk + 1][3], b2,
                                 b3);
                     }
-                    const float2 f = *reinterpret_cast<const float2*>(kf + blk * kWarpPos + nt * 8 + 2 * quad);
+                    const uint32_t f0 = f[blk / 2], f1 = f[kWords + blk / 2];
+                    const float fx = __uint_as_float(blk & 1 ? f0 & 0xFFFF0000u : f0 << 16);
+                    const float fy = __uint_as_float(blk & 1 ? f1 & 0xFFFF0000u : f1 << 16);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        s[nt][2 * n] = fmaf(d[2 * n], f.x, s[nt][2 * n]);
-                        s[nt][2 * n + 1] = fmaf(d[2 * n + 1], f.y, s[nt][2 * n + 1]);
+                        s[nt][2 * n] = fmaf(d[2 * n], fx, s[nt][2 * n]);
+                        s[nt][2 * n + 1] = fmaf(d[2 * n + 1], fy, s[nt][2 * n + 1]);
                     }
                 }
+            }
+#pragma unroll
+            for (int nt = 0; nt < kCols; ++nt)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    s[nt][2 * n] *= mul[n];
+                    s[nt][2 * n + 1] *= mul[n];
+                }
+            if (mask != kFull) {
+#pragma unroll
+                for (int nt = 0; nt < kCols; ++nt)
+#pragma unroll
+                    for (int j = 0; j < 2 * NT; ++j)
+                        if (!((mask >> (nt * 8 + 2 * quad + (j & 1))) & 1)) s[nt][j] = -INFINITY;
             }
             // ---- softmax, in log2 ----
             float corr[NT];
             bool moved = false;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                float top_s = -INFINITY;
+                float top = -INFINITY;
 #pragma unroll
-                for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        float& v = s[nt][2 * n + j];
-                        v = (mask >> (nt * 8 + 2 * quad + j)) & 1 ? v * mul[n] : -INFINITY;
-                        top_s = fmaxf(top_s, v);
-                    }
-                top_s = fmaxf(top_s, __shfl_xor_sync(0xFFFFFFFFu, top_s, 1));
-                top_s = fmaxf(top_s, __shfl_xor_sync(0xFFFFFFFFu, top_s, 2));
-                const float m_new = fmaxf(m[n], top_s);
-                corr[n] = exp2_fast(m[n] - m_new);
+                for (int nt = 0; nt < kCols; ++nt) top = fmaxf(top, fmaxf(s[nt][2 * n], s[nt][2 * n + 1]));
+                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+                const float m_new = fmaxf(m[n], top);
+                corr[n] = m_new > m[n] ? exp2_fast(m[n] - m_new) : 1.0f;
                 moved |= m_new > m[n];
                 m[n] = m_new;
-                l[n] *= m_new > -INFINITY ? corr[n] : 1.0f;
+                l[n] *= corr[n];
 #pragma unroll
-                for (int nt = 0; nt < 2; ++nt)
+                for (int nt = 0; nt < kCols; ++nt)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         float& v = s[nt][2 * n + j];
@@ -460,11 +510,49 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
                         l[n] += v;
                     }
             }
+            // ---- V's scale bytes and the largest of them ----
+            uint32_t vw[kCols][kWords];
+            uint32_t most = 0;
+#pragma unroll
+            for (int nt = 0; nt < kCols; ++nt) {
+                load_scale_pair<kBlocks>(vs + nt * 8 * kBlocks, vw[nt]);
+                if (mask != kFull) {  // an absent position may share its four bytes with one that is there
+                    uint16_t h[kBlocks];
+#pragma unroll
+                    for (int i = 0; i < kBlocks; ++i) {
+                        h[i] = (uint16_t)(vw[nt][i / 2] >> (16 * (i & 1)));
+                        if (!((mask >> (nt * 8 + 2 * quad + (i >= kWords))) & 1)) h[i] = 0;
+                    }
+#pragma unroll
+                    for (int i = 0; i < kWords; ++i) vw[nt][i] = h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
+                }
+#pragma unroll
+                for (int i = 0; i < kWords; ++i) most = __vmaxu4(most, vw[nt][i]);
+            }
+            if (__any_sync(0xFFFFFFFFu, __vcmpeq4(most, 0xFFFFFFFFu) != 0)) {
+                // NaN scales reach the result as they are; R is the largest of the others
+                most = 0;
+#pragma unroll
+                for (int nt = 0; nt < kCols; ++nt)
+#pragma unroll
+                    for (int i = 0; i < kWords; ++i)
+                        most = __vmaxu4(most, vw[nt][i] & ~__vcmpeq4(vw[nt][i], 0xFFFFFFFFu));
+            }
+            most = __vmaxu4(most, most >> 16);
+            most = max(most & 0xFFu, (most >> 8) & 0xFFu);
+            most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
+            most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
+            float down = 1.0f;
+            if ((int)most > ref) {  // acc is in units of 2^(ref - 142)
+                down = exp2_fast((float)(ref - (int)most));
+                ref = (int)most;
+                moved = true;
+            }
             if (__any_sync(0xFFFFFFFFu, moved)) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const float c0 = __shfl_sync(0xFFFFFFFFu, corr[n], 8 * quad);
-                    const float c1 = __shfl_sync(0xFFFFFFFFu, corr[n], 8 * quad + 4);
+                    const float c0 = __shfl_sync(0xFFFFFFFFu, corr[n], 8 * quad) * down;
+                    const float c1 = __shfl_sync(0xFFFFFFFFu, corr[n], 8 * quad + 4) * down;
 #pragma unroll
                     for (int i = 0; i < D / 16; ++i) {
                         acc[n][i][0] *= c0;
@@ -475,205 +563,183 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
                 }
             }
             // ---- second product: rows are elements of V, columns heads ----
+            const float up = __uint_as_float((uint32_t)(142 - ref + 127) << 23);  // 2^(142 - ref)
+#pragma unroll
+            for (int nt = 0; nt < kCols; ++nt)
+#pragma unroll
+                for (int j = 0; j < 2 * NT; ++j) s[nt][j] *= up;
             const uint8_t* vsm = st + C::kv_bytes;
 #pragma unroll
-            for (int blk = 0; blk < kBlocks; ++blk) {
-                const float2 f0 = *reinterpret_cast<const float2*>(vf + blk * kWarpPos + 2 * quad);
-                const float2 f1 = *reinterpret_cast<const float2*>(vf + blk * kWarpPos + 8 + 2 * quad);
-                uint32_t pb[NT][2];
+            for (int half = 0; half < POS / 16; ++half) {
+                uint32_t f[2][kBlocks];
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    pb[n][0] = pack_half2(s[0][2 * n] * f0.x, s[0][2 * n + 1] * f0.y);
-                    pb[n][1] = pack_half2(s[1][2 * n] * f1.x, s[1][2 * n + 1] * f1.y);
-                }
-                // positions 2 quad, 2 quad + 1, 8 + 2 quad, 9 + 2 quad; elements 4 row .. 4 row + 3 of the block
-                uint32_t w[4];
+                for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    w[i] = *reinterpret_cast<const uint32_t*>(vsm + group_at<D>(quad + 4 * (i >> 1) + 8 * (i & 1), blk) +
-                                                              4 * row);
-                uint32_t h[2][4];  // [positions low or high][element]: pairs of neighbouring positions
+                    for (int i = 0; i < kWords; ++i)
+                        ue8m0x4_to_bf162(vw[2 * half + t][i], f[t][2 * i], f[t][2 * i + 1]);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    e4m3x4_to_half2(__byte_perm(w[2 * i], w[2 * i + 1], 0x5140), h[i][0], h[i][1]);
-                    e4m3x4_to_half2(__byte_perm(w[2 * i], w[2 * i + 1], 0x7362), h[i][2], h[i][3]);
-                }
+                for (int blk = 0; blk < kBlocks; ++blk) {
+                    uint32_t pb[NT][2];
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    mma_f16(acc[n][2 * blk], h[0][0], h[0][1], h[1][0], h[1][1], pb[n][0], pb[n][1]);
-                    mma_f16(acc[n][2 * blk + 1], h[0][2], h[0][3], h[1][2], h[1][3], pb[n][0], pb[n][1]);
+                    for (int t = 0; t < 2; ++t) {
+                        const uint32_t f0 = f[t][blk / 2], f1 = f[t][kWords + blk / 2];
+                        const float fx = __uint_as_float(blk & 1 ? f0 & 0xFFFF0000u : f0 << 16);
+                        const float fy = __uint_as_float(blk & 1 ? f1 & 0xFFFF0000u : f1 << 16);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+                            pb[n][t] = pack_half2(s[2 * half + t][2 * n] * fx, s[2 * half + t][2 * n + 1] * fy);
+                    }
+                    // positions 2 quad, 2 quad + 1, 8 + 2 quad, 9 + 2 quad; elements 4 row .. 4 row + 3 of the block
+                    uint32_t w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        w[i] = *reinterpret_cast<const uint32_t*>(
+                            vsm + group_at<D>(16 * half + quad + 4 * (i >> 1) + 8 * (i & 1), blk) + 4 * row);
+                    uint32_t h[2][4];  // [positions low or high][element]: pairs of neighbouring positions
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        e4m3x4_to_half2(__byte_perm(w[2 * i], w[2 * i + 1], 0x5140), h[i][0], h[i][1]);
+                        e4m3x4_to_half2(__byte_perm(w[2 * i], w[2 * i + 1], 0x7362), h[i][2], h[i][3]);
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        mma_f16(acc[n][2 * blk], h[0][0], h[0][1], h[1][0], h[1][1], pb[n][0], pb[n][1]);
+                        mma_f16(acc[n][2 * blk + 1], h[0][2], h[0][3], h[1][2], h[1][3], pb[n][0], pb[n][1]);
+                    }
                 }
             }
         }
         stage = stage + 1 == C::stages ? 0 : stage + 1;
 
-        // ---- the last tile of a segment, or of this CTA: join the warps ----
-        const bool ends = cur.t + 1 == cur.nt;
-        if (ends || x + 1 == x1) {
-            float* join = reinterpret_cast<float*>(smem + C::join_off);           // [row][D]
-            float2* ml = reinterpret_cast<float2*>(smem + C::ml_off);             // [warp][row]
+        if (cur.t + 1 == cur.t1) {  // the warp's last tile of this segment
+            const bool begins = cur.t0 == 0, ends = cur.t1 == cur.nt;
+            const int64_t seg = cur.b * groups + cur.g;
+            // slot 1 of the warp: the segment begins here and goes on; slot 0: it began before
+            const int64_t slot = 2 * part + (begins ? 1 : 0);
+            if (begins && lane == 0) {
+                const int64_t last = split_part(cur.base + kSegmentCost + cur.nt - 1, parts, total);
+                gstore_plain(p.meta + seg, ends ? make_int2(0, -1) : make_int2((int)part, (int)last), p.a.ww,
+                             p.a.status);
+            }
+            const int sub = cur.g % p.row_groups;
+            const int64_t head0 = (int64_t)(cur.g / p.row_groups) * p.group + sub * C::rows;
+            const int rows = min(C::rows, p.group - sub * C::rows);
+            const float unit = exp2f((float)(ref - 142));
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 l[n] += __shfl_xor_sync(0xFFFFFFFFu, l[n], 1);
                 l[n] += __shfl_xor_sync(0xFFFFFFFFu, l[n], 2);
-                if (quad == 0) ml[warp * C::rows + n * 8 + row] = make_float2(m[n], l[n]);
-            }
-            __syncthreads();
-            // acc holds rows (heads) 2 quad, 2 quad + 1: their joint maxima and this warp's factors
-            float fac[NT][2];
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
+                // rows as in the scores: 8 n + row
+                if (quad == 0 && n * 8 + row < rows) {
+                    if (!(begins && ends))
+                        gstore_plain(p.part_ml + slot * C::rows + n * 8 + row, make_float2(m[n], l[n]), p.a.ww,
+                                     p.a.status);
+                    else if (p.a.lse)
+                        gstore_plain(p.a.lse + cur.b * p.a.q_heads + head0 + n * 8 + row, (m[n] + log2f(l[n])) * kLn2,
+                                     p.a.lw, p.a.status);
+                }
+                // rows as in acc: 8 n + 2 quad + {0, 1}; per block the elements 4 row .. 4 row + 3
+                const float inv = l[n] == 0.0f ? 0.0f : 1.0f / l[n];
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
+                    const float inv_j = __shfl_sync(0xFFFFFFFFu, inv, 8 * quad + 4 * j);
                     const int r = n * 8 + 2 * quad + j;
-                    float all = -INFINITY;
+                    if (r >= rows) continue;
 #pragma unroll
-                    for (int w = 0; w < kWarps; ++w) all = fmaxf(all, ml[w * C::rows + r].x);
-                    const float2 own = ml[warp * C::rows + r];
-                    fac[n][j] = own.y == 0.0f ? 0.0f : exp2_fast(own.x - all) * exp2f((float)((int)ref - 142));
-                }
-            for (int w = 0; w < kWarps; ++w) {
-                if (warp == w) {
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                // tile i of block i / 2: elements 4 row + 2 (i % 2) + (j / 2)
-                                const int d = (i >> 1) * 32 + 4 * row + 2 * (i & 1) + (j >> 1);
-                                float* dst = join + (n * 8 + 2 * quad + (j & 1)) * D + d;
-                                const float v = acc[n][i][j] * fac[n][j & 1];
-                                *dst = w == 0 ? v : *dst + v;
-                            }
-                }
-                __syncthreads();
-            }
-            const bool whole = ends && x0 <= seg0;
-            // slot 1: the segment begins in this CTA; slot 0: it began before
-            const int64_t slot = 2 * cta + (x0 <= seg0 ? 1 : 0);
-            const int64_t seg = cur.b * groups + cur.g;
-            if (threadIdx.x == 0 && x0 <= seg0)
-                gstore_plain(p.meta + seg,
-                             whole ? make_int2(0, -1)
-                                   : make_int2((int)cta, (int)split_part(seg0 + cur.nt - 1, parts, total)),
-                             p.a.ww, p.a.status);
-            const int sub = cur.g % p.row_groups;
-            const int64_t head0 = (int64_t)(cur.g / p.row_groups) * p.group + sub * C::rows;
-            const int rows = min(C::rows, p.group - sub * C::rows);
-            for (int r = warp; r < rows; r += kWarps) {
-                float all = -INFINITY, sum = 0.0f;
-#pragma unroll
-                for (int w = 0; w < kWarps; ++w) all = fmaxf(all, ml[w * C::rows + r].x);
-#pragma unroll
-                for (int w = 0; w < kWarps; ++w) {
-                    const float2 v = ml[w * C::rows + r];
-                    if (v.y != 0.0f) sum += v.y * exp2_fast(v.x - all);
-                }
-                if (whole) {
-                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                    const int64_t o = (cur.b * p.a.q_heads + head0 + r) * D;
-                    for (int d = 2 * lane; d < D; d += 64) {
-                        const float v0 = join[r * D + d] * inv, v1 = join[r * D + d + 1] * inv;
-                        uint32_t h;
-                        if (p.a.q_bf16) {
-                            const __nv_bfloat162 t = __floats2bfloat162_rn(v0, v1);
-                            h = *reinterpret_cast<const uint32_t*>(&t);
+                    for (int blk = 0; blk < kBlocks; ++blk) {
+                        const float o0 = acc[n][2 * blk][j] * unit, o1 = acc[n][2 * blk][2 + j] * unit;
+                        const float o2 = acc[n][2 * blk + 1][j] * unit, o3 = acc[n][2 * blk + 1][2 + j] * unit;
+                        const int d = blk * 32 + 4 * row;
+                        if (begins && ends) {
+                            const int64_t o = (cur.b * p.a.q_heads + head0 + r) * D + d;
+                            gstore_plain(reinterpret_cast<uint2*>(p.a.out + o),
+                                         make_uint2(pack_out(p.a.q_bf16, o0 * inv_j, o1 * inv_j),
+                                                    pack_out(p.a.q_bf16, o2 * inv_j, o3 * inv_j)),
+                                         p.a.ow, p.a.status);
                         } else {
-                            h = pack_half2(v0, v1);
+                            gstore_plain(reinterpret_cast<float4*>(p.part_o + (slot * C::rows + r) * D + d),
+                                         make_float4(o0, o1, o2, o3), p.a.ww, p.a.status);
                         }
-                        gstore_plain(reinterpret_cast<uint32_t*>(p.a.out + o + d), h, p.a.ow, p.a.status);
                     }
-                    if (p.a.lse && lane == 0)
-                        gstore_plain(p.a.lse + cur.b * p.a.q_heads + head0 + r, (all + log2f(sum)) * kLn2, p.a.lw,
-                                     p.a.status);
-                } else {
-                    float* o = p.part_o + (slot * C::rows + r) * D;
-                    for (int d = 2 * lane; d < D; d += 64)
-                        gstore_plain(reinterpret_cast<float2*>(o + d),
-                                     make_float2(join[r * D + d], join[r * D + d + 1]), p.a.ww, p.a.status);
-                    if (lane == 0)
-                        gstore_plain(p.part_ml + slot * C::rows + r, make_float2(all, sum), p.a.ww, p.a.status);
                 }
             }
-            __syncthreads();
-            seg0 += cur.nt;
             fresh = true;
         }
-        if (x + 1 < x1) advance(p, cur, groups);
+        advance<POS>(p, cur, groups);
     }
     cp_async_wait<0>();
     grid_launch_dependents();
 }
 
-// Second launch: one CTA per (sequence, head group).  Empty sequences get
-// their zeros here; segments that one CTA held are done; the pieces of the others are
-// joined in the order of the CTAs.
+// Second launch: one CTA per (sequence, query head).  Empty sequences get
+// their zeros here; segments that one warp held are done; the pieces of the
+// others are joined, every fourth by one of four warps.
 template <int D, int NT>
-__global__ void __launch_bounds__(128) cache_attention_join_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads) cache_attention_join_kernel(const Params p) {
     using C = Config<D, NT>;
+    constexpr int kVecs = D / 64;
+    __shared__ float2 sums[kWarps][D / 2];
     grid_wait_prerequisites();
-    const int groups = p.a.c.heads * p.row_groups;
-    const int64_t seg = blockIdx.x;
-    const int64_t b = seg / groups;
-    const int g = (int)(seg - b * groups), sub = g % p.row_groups;
-    const int rows = min(C::rows, p.group - sub * C::rows);
-    const int64_t head0 = b * p.a.q_heads + (int64_t)(g / p.row_groups) * p.group + sub * C::rows;
-    const bool empty = length_of(p.a, b) == 0;
-    int2 ctas = make_int2(0, -1);
-    if (!empty) {
-        ctas = p.meta[seg];
-        if (ctas.y < ctas.x) return;
+    const int64_t b = blockIdx.x / p.a.q_heads;
+    const int head = (int)(blockIdx.x - b * p.a.q_heads);
+    const int in = head % p.group, sub = in / C::rows, r = in - sub * C::rows;
+    int2 parts = make_int2(0, -1);
+    if (length_of(p.a, b) != 0) {
+        parts = p.meta[(b * p.a.c.heads + head / p.group) * p.row_groups + sub];
+        if (parts.y < parts.x) return;
     }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int r = warp; r < rows; r += 4) {
-        float all = -INFINITY;
-        for (int i = ctas.x + lane; i <= ctas.y; i += 32)
-            all = fmaxf(all, p.part_ml[(2 * (int64_t)i + (i == ctas.x)) * C::rows + r].x);
-        all = warp_max(all);
-        float sum = 0.0f;
-        float2 o[D / 64];
-#pragma unroll
-        for (int k = 0; k < D / 64; ++k) o[k] = make_float2(0.0f, 0.0f);
-        for (int i = ctas.x; i <= ctas.y; ++i) {
-            const int64_t at = (2 * (int64_t)i + (i == ctas.x)) * C::rows + r;
-            const float2 ml = p.part_ml[at];
-            if (ml.y == 0.0f) continue;  // no position of the piece was there
-            const float f = exp2_fast(ml.x - all);
-            sum += ml.y * f;
-#pragma unroll
-            for (int k = 0; k < D / 64; ++k) {
-                const float2 v = *reinterpret_cast<const float2*>(p.part_o + at * D + 2 * lane + 64 * k);
-                o[k].x += v.x * f;
-                o[k].y += v.y * f;
-            }
-        }
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-        for (int k = 0; k < D / 64; ++k) {
-            uint32_t h;
-            if (p.a.q_bf16) {
-                const __nv_bfloat162 t = __floats2bfloat162_rn(o[k].x * inv, o[k].y * inv);
-                h = *reinterpret_cast<const uint32_t*>(&t);
-            } else {
-                h = pack_half2(o[k].x * inv, o[k].y * inv);
-            }
-            gstore_plain(reinterpret_cast<uint32_t*>(p.a.out + (head0 + r) * D + 2 * lane + 64 * k), h, p.a.ow,
-                         p.a.status);
-        }
-        if (p.a.lse && lane == 0)
-            gstore_plain(p.a.lse + head0 + r, (all + log2f(sum)) * kLn2, p.a.lw, p.a.status);
+    auto slot_of = [&](int i) { return (2 * (int64_t)i + (i == parts.x)) * C::rows + r; };
+    float top = -INFINITY;
+    for (int i = parts.x + lane; i <= parts.y; i += 32) top = fmaxf(top, p.part_ml[slot_of(i)].x);
+    top = warp_max(top);
+    float sum = 0.0f;
+    for (int i = parts.x + lane; i <= parts.y; i += 32) {
+        const float2 ml = p.part_ml[slot_of(i)];
+        if (ml.y != 0.0f) sum += ml.y * exp2_fast(ml.x - top);  // 0: no position of the piece was there
     }
+    sum = warp_sum(sum);
+    float2 o[kVecs];
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) o[k] = make_float2(0.0f, 0.0f);
+#pragma unroll 4
+    for (int i = parts.x + warp; i <= parts.y; i += kWarps) {
+        const int64_t at = slot_of(i);
+        const float2 ml = p.part_ml[at];
+        const float f = ml.y != 0.0f ? exp2_fast(ml.x - top) : 0.0f;
+#pragma unroll
+        for (int k = 0; k < kVecs; ++k) {
+            const float2 v = *reinterpret_cast<const float2*>(p.part_o + at * D + 2 * lane + 64 * k);
+            o[k].x += v.x * f;
+            o[k].y += v.y * f;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) sums[warp][lane + 32 * k] = o[k];
+    __syncthreads();
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    for (int d = threadIdx.x; d < D / 2; d += kThreads) {
+        float2 v = sums[0][d];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) {
+            v.x += sums[w][d].x;
+            v.y += sums[w][d].y;
+        }
+        gstore_plain(reinterpret_cast<uint32_t*>(p.a.out + (int64_t)blockIdx.x * D + 2 * d),
+                     pack_out(p.a.q_bf16, v.x * inv, v.y * inv), p.a.ow, p.a.status);
+    }
+    if (p.a.lse && threadIdx.x == 0)
+        gstore_plain(p.a.lse + blockIdx.x, (top + log2f(sum)) * kLn2, p.a.lw, p.a.status);
 }
 
 template <int D, int NT>
-int64_t grid_of(int sm_count) {
+int64_t ctas_of(int sm_count) {
     return (int64_t)sm_count * Config<D, NT>::ctas_per_sm;
 }
 
 template <int D, int NT>
 int64_t workspace_of(int64_t segments, int sm_count) {
-    const int64_t slots = 2 * grid_of<D, NT>(sm_count) * Config<D, NT>::rows;
+    const int64_t slots = 2 * kWarps * ctas_of<D, NT>(sm_count) * Config<D, NT>::rows;
     return slots * (D * 4 + 8) + segments * 8;
 }
 
@@ -702,12 +768,14 @@ int launch_typed(const CacheAttentionArgs& a, int sm_count, cudaStream_t stream)
     p.group = a.q_heads / a.c.heads;
     p.row_groups = (p.group + C::rows - 1) / C::rows;
     const int64_t segments = a.batch * a.c.heads * p.row_groups;
-    const int64_t most = segments * (((a.max_pages << a.c.page_shift) + kTilePos - 1) / kTilePos);
-    const int64_t ctas = grid_of<D, NT>(sm_count);
-    p.grid = ctas < most ? ctas : most;
+    // no more warps than the longest lengths that the table allows would use
+    const int64_t most = segments * (((a.max_pages << a.c.page_shift) + C::pos - 1) / C::pos + kSegmentCost);
+    const int64_t ctas = ctas_of<D, NT>(sm_count), slots = 2 * kWarps * ctas * C::rows;
+    const int64_t grid = a.max_pages == 0 ? 0 : most < ctas * kWarps ? (most + kWarps - 1) / kWarps : ctas;
+    p.parts = grid * kWarps;
     p.part_o = static_cast<float*>(a.workspace);
-    p.part_ml = reinterpret_cast<float2*>(p.part_o + 2 * ctas * C::rows * D);
-    p.meta = reinterpret_cast<int2*>(p.part_ml + 2 * ctas * C::rows);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + slots * D);
+    p.meta = reinterpret_cast<int2*>(p.part_ml + slots);
 
     cudaLaunchConfig_t cfg = {};
     cfg.stream = stream;
@@ -716,15 +784,15 @@ int launch_typed(const CacheAttentionArgs& a, int sm_count, cudaStream_t stream)
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (p.grid > 0) {
-        cfg.gridDim = dim3((unsigned)p.grid);
+    if (grid > 0) {
+        cfg.gridDim = dim3((unsigned)grid);
         cfg.blockDim = dim3(kThreads);
         cfg.dynamicSmemBytes = C::smem;
         e = cudaLaunchKernelEx(&cfg, kernel, p);
     }
     if (e == cudaSuccess) {
-        cfg.gridDim = dim3((unsigned)segments);
-        cfg.blockDim = dim3(128);
+        cfg.gridDim = dim3((unsigned)(a.batch * a.q_heads));
+        cfg.blockDim = dim3(kThreads);
         cfg.dynamicSmemBytes = 0;
         e = cudaLaunchKernelEx(&cfg, cache_attention_join_kernel<D, NT>, p);
     }

@@ -21,7 +21,7 @@ int check_cache(const mxfp8_cache* cache, CacheShape* c) {
     if (!cache) return MXFP8_ERR_NULL_POINTER;
     const int s = cache->page_size;
     if (cache->num_pages < 0 || cache->heads < 1 || s < 1 || s > 4096 || (s & (s - 1)) != 0 || cache->dim < 32 ||
-        cache->dim > 1024 || cache->dim % 32 != 0 || cache->num_pages > (int64_t(1) << 32) / cache->heads / s)
+        cache->dim > 1024 || cache->dim % 32 != 0 || cache->num_pages > ((int64_t(1) << 32) - 1) / cache->heads / s)
         return MXFP8_ERR_SHAPE;
     if (cache->num_pages > 0) {
         if (!cache->k || !cache->v || !cache->k_scales || !cache->v_scales) return MXFP8_ERR_NULL_POINTER;
