@@ -44,7 +44,9 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kSegmentCost = 1;
+constexpr int kJoinWarps = 8;
+constexpr int kJoinThreads = 32 * kJoinWarps;
+constexpr int kSegmentCost = 2;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr uint32_t kNoRow32 = 0xFFFFFFFFu;
@@ -60,10 +62,10 @@ struct Config {
     static constexpr int kv_bytes = pos * D;                  // K (or V) payload of a tile
     static constexpr int sc_bytes = pos * D / 32;
     static constexpr int stage_bytes = 2 * kv_bytes + 2 * sc_bytes;
-    static constexpr int stages = D <= 64 ? 4 : D <= 128 ? 2 : 3;
+    static constexpr int stages = D <= 64 ? 3 : 2;
     static constexpr int warp_bytes = stages * stage_bytes;
     static constexpr int smem = kWarps * warp_bytes;
-    static constexpr int ctas_per_sm = D <= 128 && NT == 1 ? 3 : 2;
+    static constexpr int ctas_per_sm = 2;
 };
 
 struct Params {
@@ -117,8 +119,8 @@ __device__ __forceinline__ bool enter(Cursor& c, int64_t begin) {
 }
 
 template <int POS>
-__device__ __forceinline__ void enter_sequence(const Params& p, Cursor& c) {
-    c.len = length_of(p.a, c.b);
+__device__ __forceinline__ void enter_sequence(const Params& p, Cursor& c, int len) {
+    c.len = len;
     c.nt = (c.len + POS - 1) / POS;
     c.pages = p.a.table + c.b * p.a.table_stride;
 }
@@ -136,7 +138,7 @@ __device__ __forceinline__ void next_segment(const Params& p, Cursor& c, int gro
             c.g = 0;
             do {  // total cost is not exhausted: there is another sequence with tiles
                 ++c.b;
-                enter_sequence<POS>(p, c);
+                enter_sequence<POS>(p, c, length_of(p.a, c.b));
             } while (c.nt == 0);
         }
     } while (!enter(c, c.base));
@@ -200,28 +202,45 @@ __device__ __forceinline__ uint32_t pack_out(bool bf16, float lo, float hi) {
 }
 
 // Shared memory of a tile's rows of D bytes: 32-byte groups of a row are
-// permuted so that the four rows that one access phase reads (K: rows r .. r +
-// 3, V: the same after v_place) fall on different banks.
+// permuted (xor with a key of the row) so that the four rows that one access
+// phase reads (K: rows r .. r + 3, V: the same after v_place) fall on different
+// banks.
 template <int D>
-__device__ __forceinline__ uint32_t group_at(int row, int group) {
-    const int key = D % 128 == 0 ? (row & 3) : ((row >> 1) & 1);
-    return (uint32_t)(row * D + ((group ^ key) << 5));
+__device__ __forceinline__ constexpr int key_of(int row) {
+    return D % 128 == 0 ? (row & 3) : ((row >> 1) & 1);
+}
+template <int D>
+__device__ __forceinline__ constexpr uint32_t group_at(int row, int group) {
+    return (uint32_t)(row * D + ((group ^ key_of<D>(row)) << 5));
+}
+// The same place as `at` (in group 0 of its row), in group blk: the key's bits
+// are exchanged, the others added; a row's start has none of the key's bits.
+template <int D>
+__device__ __forceinline__ constexpr uint32_t in_block(uint32_t at, int blk) {
+    constexpr int kKey = D % 128 == 0 ? 3 : 1;
+    return (at ^ (uint32_t)((blk & kKey) << 5)) + (uint32_t)((blk & ~kKey) << 5);
 }
 // Row that position j of V is kept in: of each 16, the positions 2c + i, c = 0
 // .. 3, that a phase of the second product reads are neighbours.
-__device__ __forceinline__ int v_place(int j) { return (j & ~15) | ((j & 15) >> 1) | ((j & 1) << 3); }
+__device__ __forceinline__ constexpr int v_place(int j) { return (j & ~15) | ((j & 15) >> 1) | ((j & 1) << 3); }
+
+// Page of position `lane` of the cursor's tile, as the table has it.  The load
+// is consumed a tile later (row_of_lane): waiting for it here would cost a
+// memory latency a tile.
+template <int POS>
+__device__ __forceinline__ int page_of_lane(const Params& p, const Cursor& c, int lane) {
+    const int at = c.t * POS + lane;
+    return c.done || lane >= POS || at >= c.len ? -1 : c.pages[at >> p.a.c.page_shift];  // at is within the table
+}
 
 // Cache row of position `lane` of the cursor's tile, kNoRow32 where there is none.
 template <int POS>
-__device__ __forceinline__ uint32_t row_of_lane(const Params& p, const Cursor& c, int lane) {
+__device__ __forceinline__ uint32_t row_of_lane(const Params& p, const Cursor& c, int page, int lane) {
     const int at = c.t * POS + lane;
-    if (c.done || lane >= POS || at >= c.len) return kNoRow32;
-    const uint32_t page = (uint32_t)c.pages[at >> p.a.c.page_shift];  // the length is within the table
-    if (page >= (uint64_t)p.a.c.num_pages) {
-        if (p.a.status) atomicOr(p.a.status, kErrCacheIndex);
-        return kNoRow32;
-    }
-    return (uint32_t)cache_row(p.a.c, page, c.g / p.row_groups, at & ((1 << p.a.c.page_shift) - 1));
+    if (lane >= POS || at >= c.len) return kNoRow32;
+    const int64_t row = cache_row(p.a.c, page, c.g / p.row_groups, at & ((1 << p.a.c.page_shift) - 1));
+    if (row == kNoRow && p.a.status) atomicOr(p.a.status, kErrCacheIndex);
+    return row == kNoRow ? kNoRow32 : (uint32_t)row;
 }
 
 // Fetch those rows into a stage: payloads 16 bytes a lane, scales four bytes a
@@ -231,15 +250,35 @@ template <int D, int POS>
 __device__ __forceinline__ void fetch(const Params& p, uint32_t stage, uint32_t my_row, int lane) {
     constexpr int kChunks = D / 16;  // of a row
     constexpr int kKv = POS * D;
+    if constexpr ((kChunks & (kChunks - 1)) == 0) {
+        // A lane keeps its chunk; step i takes row i * kRows + j0.  Both the row of V and the keys split into a
+        // part of i and a part of j0 that share no bits, so a step's address is the lane's own, xor a constant, plus
+        // a constant.
+        constexpr int kRows = 32 / kChunks;
+        const int j0 = lane / kChunks, ch = lane % kChunks;
+        const uint32_t k_at = group_at<D>(j0, ch >> 1) + (ch & 1) * 16;
+        const uint32_t v_at = group_at<D>(v_place(j0), ch >> 1) + (ch & 1) * 16;
+        const uint8_t* k = p.a.k + ch * 16;
+        const uint8_t* v = p.a.v + ch * 16;
 #pragma unroll
-    for (int i = 0; i < kKv / 512; ++i) {
-        const int idx = i * 32 + lane;
-        const int j = idx / kChunks, ch = idx - j * kChunks;
-        const uint32_t row = __shfl_sync(0xFFFFFFFFu, my_row, j);
-        const bool on = row != kNoRow32;
-        const uint64_t off = (uint64_t)(on ? row : 0u) * D + ch * 16;
-        cp_async16(stage + group_at<D>(j, ch >> 1) + (ch & 1) * 16, p.a.k + off, on);
-        cp_async16(stage + kKv + group_at<D>(v_place(j), ch >> 1) + (ch & 1) * 16, p.a.v + off, on);
+        for (int i = 0; i < POS / kRows; ++i) {
+            const uint32_t row = __shfl_sync(0xFFFFFFFFu, my_row, i * kRows + j0);
+            const bool on = row != kNoRow32;
+            const uint64_t off = (uint64_t)(on ? row : 0u) * D;
+            cp_async16(stage + i * kRows * D + (k_at ^ (key_of<D>(i * kRows) << 5)), k + off, on);
+            cp_async16(stage + kKv + v_place(i * kRows) * D + (v_at ^ (key_of<D>(v_place(i * kRows)) << 5)), v + off, on);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kKv / 512; ++i) {
+            const int idx = i * 32 + lane;
+            const int j = idx / kChunks, ch = idx - j * kChunks;
+            const uint32_t row = __shfl_sync(0xFFFFFFFFu, my_row, j);
+            const bool on = row != kNoRow32;
+            const uint64_t off = (uint64_t)(on ? row : 0u) * D + ch * 16;
+            cp_async16(stage + group_at<D>(j, ch >> 1) + (ch & 1) * 16, p.a.k + off, on);
+            cp_async16(stage + kKv + group_at<D>(v_place(j), ch >> 1) + (ch & 1) * 16, p.a.v + off, on);
+        }
     }
     constexpr int kPair = D / 64;    // 4-byte pieces of two positions' scales
     constexpr int kPieces = POS / 2 * kPair;
@@ -327,9 +366,11 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int64_t scan_s[kWarps];
     __shared__ int64_t found_b[kWarps], found_base[kWarps];
+    __shared__ int found_len[kWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = lane >> 2, quad = lane & 3;
     const int groups = p.a.c.heads * p.row_groups;
 
+    grid_launch_dependents();  // the second launch may take its place: it waits for this one's end
     grid_wait_prerequisites();
     // ---- the warps' shares of all costs, and the sequences where they begin ----
     const int64_t per = (p.a.batch + kThreads - 1) / kThreads;
@@ -358,49 +399,57 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
     const int64_t parts = min(p.parts, total);
     const int64_t first_part = (int64_t)blockIdx.x * kWarps;
     if (first_part >= parts) return;
+    const Split split = make_split(parts, total);
     const int64_t from = (before + upto - mine) * groups;  // place of this thread's first sequence
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-        const int64_t x = split_begin(first_part + w, parts, total);
+        const int64_t x = split_begin(split, first_part + w);
         if (first_part + w < parts && from <= x && x < from + mine * groups) {
             int64_t at = from;
             int64_t b = b0;
+            int len;
             for (;; ++b) {
-                const int64_t n = (int64_t)cost_of<POS>(length_of(p.a, b)) * groups;
+                len = length_of(p.a, b);
+                const int64_t n = (int64_t)cost_of<POS>(len) * groups;
                 if (x < at + n) break;
                 at += n;
             }
             found_b[w] = b;
             found_base[w] = at;
+            found_len[w] = len;
         }
     }
     __syncthreads();
     const int64_t part = first_part + warp;
     if (part >= parts) return;
     Cursor cur;  // the tile that is computed
-    const int64_t begin = split_begin(part, parts, total);
-    cur.end = split_begin(part + 1, parts, total);
+    const int64_t begin = split_begin(split, part);
+    cur.end = split_begin(split, part + 1);
     cur.b = found_b[warp];
-    enter_sequence<POS>(p, cur);
+    enter_sequence<POS>(p, cur, found_len[warp]);
     cur.g = (int)((begin - found_base[warp]) / (cur.nt + kSegmentCost));
     cur.base = found_base[warp] + (int64_t)cur.g * (cur.nt + kSegmentCost);
     cur.done = false;
     if (!enter(cur, begin)) next_segment<POS>(p, cur, groups);
 
+    // this lane's part of K (row `row` of eight) and V (place `quad` of four); the keys of the rows that it reads are
+    // those of these two
+    const uint32_t k_at = group_at<D>(row, 0) + quad * 8, v_at = group_at<D>(quad, 0) + 4 * row;
     uint8_t* const ring = smem + warp * C::warp_bytes;
     const uint32_t ring_u = smem_u32(ring);
 
-    // ---- fetch ahead: `next` is the tile whose rows are looked up in my_row ----
+    // ---- fetch ahead: `next` is the tile whose pages are being looked up ----
     Cursor next = cur;
-    uint32_t my_row = row_of_lane<POS>(p, next, lane);
+    int my_page = page_of_lane<POS>(p, next, lane);
     uint32_t present = 0;  // lane s: which positions of stage s are there
     auto issue = [&](int stage) {
         if (!next.done) {
+            const uint32_t my_row = row_of_lane<POS>(p, next, my_page, lane);
             const uint32_t mask = __ballot_sync(0xFFFFFFFFu, my_row != kNoRow32);
             if (mask != 0) fetch<D, POS>(p, ring_u + stage * C::stage_bytes, my_row, lane);
             if (lane == stage) present = mask;
             advance<POS>(p, next, groups);
-            my_row = row_of_lane<POS>(p, next, lane);
+            my_page = page_of_lane<POS>(p, next, lane);
         }
         cp_async_commit();
     };
@@ -449,7 +498,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
                 for (int i = 0; i < kWords; ++i) ue8m0x4_to_bf162(w[i], f[2 * i], f[2 * i + 1]);
 #pragma unroll
                 for (int blk = 0; blk < kBlocks; ++blk) {
-                    const uint2 b = *reinterpret_cast<const uint2*>(st + group_at<D>(nt * 8 + row, blk) + quad * 8);
+                    const uint2 b = *reinterpret_cast<const uint2*>(st + in_block<D>(k_at, blk) + nt * 8 * D);
                     uint32_t b0, b1, b2, b3;
                     e4m3x4_to_half2(b.x, b0, b1);
                     e4m3x4_to_half2(b.y, b2, b3);
@@ -594,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         w[i] = *reinterpret_cast<const uint32_t*>(
-                            vsm + group_at<D>(16 * half + quad + 4 * (i >> 1) + 8 * (i & 1), blk) + 4 * row);
+                            vsm + in_block<D>(v_at, blk) + (16 * half + 4 * (i >> 1) + 8 * (i & 1)) * D);
                     uint32_t h[2][4];  // [positions low or high][element]: pairs of neighbouring positions
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
@@ -617,7 +666,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
             // slot 1 of the warp: the segment begins here and goes on; slot 0: it began before
             const int64_t slot = 2 * part + (begins ? 1 : 0);
             if (begins && lane == 0) {
-                const int64_t last = split_part(cur.base + kSegmentCost + cur.nt - 1, parts, total);
+                const int64_t last = split_part(split, cur.base + kSegmentCost + cur.nt - 1);
                 gstore_plain(p.meta + seg, ends ? make_int2(0, -1) : make_int2((int)part, (int)last), p.a.ww,
                              p.a.status);
             }
@@ -668,60 +717,60 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
         advance<POS>(p, cur, groups);
     }
     cp_async_wait<0>();
-    grid_launch_dependents();
 }
 
 // Second launch: one CTA per (sequence, query head).  Empty sequences get
 // their zeros here; segments that one warp held are done; the pieces of the
-// others are joined, every fourth by one of four warps.
+// others are joined, every eighth by one of eight warps.
 template <int D, int NT>
-__global__ void __launch_bounds__(kThreads) cache_attention_join_kernel(const Params p) {
+__global__ void __launch_bounds__(kJoinThreads) cache_attention_join_kernel(const Params p) {
     using C = Config<D, NT>;
     constexpr int kVecs = D / 64;
-    __shared__ float2 sums[kWarps][D / 2];
+    __shared__ float2 sums[kJoinWarps][D / 2];
+    grid_launch_dependents();
     grid_wait_prerequisites();
     const int64_t b = blockIdx.x / p.a.q_heads;
     const int head = (int)(blockIdx.x - b * p.a.q_heads);
     const int in = head % p.group, sub = in / C::rows, r = in - sub * C::rows;
-    int2 parts = make_int2(0, -1);
-    if (length_of(p.a, b) != 0) {
-        parts = p.meta[(b * p.a.c.heads + head / p.group) * p.row_groups + sub];
-        if (parts.y < parts.x) return;
-    }
+    int2 parts = p.meta[(b * p.a.c.heads + head / p.group) * p.row_groups + sub];  // not written for an empty sequence
+    if (length_of(p.a, b) == 0) parts = make_int2(0, -1);
+    else if (parts.y < parts.x) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    auto slot_of = [&](int i) { return (2 * (int64_t)i + (i == parts.x)) * C::rows + r; };
+    const int pieces = parts.y - parts.x + 1;
+    auto slot_of = [&](int i) { return (2 * (int64_t)(parts.x + i) + (i == 0)) * C::rows + r; };
     float top = -INFINITY;
-    for (int i = parts.x + lane; i <= parts.y; i += 32) top = fmaxf(top, p.part_ml[slot_of(i)].x);
+    for (int i = lane; i < pieces; i += 32) top = fmaxf(top, p.part_ml[slot_of(i)].x);
     top = warp_max(top);
     float sum = 0.0f;
-    for (int i = parts.x + lane; i <= parts.y; i += 32) {
-        const float2 ml = p.part_ml[slot_of(i)];
-        if (ml.y != 0.0f) sum += ml.y * exp2_fast(ml.x - top);  // 0: no position of the piece was there
-    }
-    sum = warp_sum(sum);
     float2 o[kVecs];
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) o[k] = make_float2(0.0f, 0.0f);
-#pragma unroll 4
-    for (int i = parts.x + warp; i <= parts.y; i += kWarps) {
-        const int64_t at = slot_of(i);
-        const float2 ml = p.part_ml[at];
-        const float f = ml.y != 0.0f ? exp2_fast(ml.x - top) : 0.0f;
+    for (int i0 = 0; i0 < pieces; i0 += 32) {  // a lane has the weight of one of 32 pieces
+        const float2 ml = i0 + lane < pieces ? p.part_ml[slot_of(i0 + lane)] : make_float2(0.0f, 0.0f);
+        const float weight = ml.y != 0.0f ? exp2_fast(ml.x - top) : 0.0f;  // 0: no position of the piece was there
+        sum += ml.y * weight;
+        const int here = min(32, pieces - i0);
+#pragma unroll 8
+        for (int i = warp; i < here; i += kJoinWarps) {
+            const float f = __shfl_sync(0xFFFFFFFFu, weight, i);
+            const float* src = p.part_o + slot_of(i0 + i) * D + 2 * lane;
 #pragma unroll
-        for (int k = 0; k < kVecs; ++k) {
-            const float2 v = *reinterpret_cast<const float2*>(p.part_o + at * D + 2 * lane + 64 * k);
-            o[k].x += v.x * f;
-            o[k].y += v.y * f;
+            for (int k = 0; k < kVecs; ++k) {
+                const float2 v = *reinterpret_cast<const float2*>(src + 64 * k);
+                o[k].x += v.x * f;
+                o[k].y += v.y * f;
+            }
         }
     }
+    sum = warp_sum(sum);
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) sums[warp][lane + 32 * k] = o[k];
     __syncthreads();
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    for (int d = threadIdx.x; d < D / 2; d += kThreads) {
+    for (int d = threadIdx.x; d < D / 2; d += kJoinThreads) {
         float2 v = sums[0][d];
 #pragma unroll
-        for (int w = 1; w < kWarps; ++w) {
+        for (int w = 1; w < kJoinWarps; ++w) {
             v.x += sums[w][d].x;
             v.y += sums[w][d].y;
         }
@@ -792,7 +841,7 @@ int launch_typed(const CacheAttentionArgs& a, int sm_count, cudaStream_t stream)
     }
     if (e == cudaSuccess) {
         cfg.gridDim = dim3((unsigned)(a.batch * a.q_heads));
-        cfg.blockDim = dim3(kThreads);
+        cfg.blockDim = dim3(kJoinThreads);
         cfg.dynamicSmemBytes = 0;
         e = cudaLaunchKernelEx(&cfg, cache_attention_join_kernel<D, NT>, p);
     }

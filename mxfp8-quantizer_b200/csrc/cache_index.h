@@ -1,6 +1,6 @@
 // cache_index.h -- index arithmetic of the paged cache: which row a position
 // lives in, which sequence an output row belongs to, and how the attention's
-// tiles are split over CTAs.  Plain C++, so that the CPU tests compile it too.
+// tiles are split over warps.  Plain C++, so that the CPU tests compile it too.
 #pragma once
 #include <stdint.h>
 
@@ -50,10 +50,25 @@ MXFP8_HD int64_t sequence_of(const int32_t* starts, int64_t batch, int64_t row) 
     return lo;
 }
 
-// `total` tiles over n parts: part i takes [split_begin(i), split_begin(i + 1)).
-MXFP8_HD int64_t split_begin(int64_t i, int64_t n, int64_t total) { return i * total / n; }
-// The part that holds tile x < total.
-MXFP8_HD int64_t split_part(int64_t x, int64_t n, int64_t total) { return ((x + 1) * n - 1) / total; }
+// `total` units over n parts, the first total % n parts one unit longer: part i
+// takes [begin(i), begin(i + 1)).
+struct Split {
+    int64_t each, longer;
+};
+MXFP8_HD Split make_split(int64_t n, int64_t total) {
+    if (total <= 0xFFFFFFFFll) {  // the common case: a 32-bit division
+        const uint32_t each = (uint32_t)total / (uint32_t)n;
+        return Split{each, total - (int64_t)each * n};
+    }
+    const int64_t each = total / n;
+    return Split{each, total - each * n};
+}
+MXFP8_HD int64_t split_begin(const Split& s, int64_t i) { return i * s.each + (i < s.longer ? i : s.longer); }
+// The part that holds unit x < total.
+MXFP8_HD int64_t split_part(const Split& s, int64_t x) {
+    const int64_t edge = s.longer * (s.each + 1);  // end of the longer parts
+    return x < edge ? x / (s.each + 1) : s.longer + (x - edge) / s.each;
+}
 
 // Positions of a sequence that the attention visits.
 MXFP8_HD int64_t visible_length(int64_t length, int64_t max_pages, int page_shift) {

@@ -12,7 +12,7 @@ int64_t probe_table(const int32_t* table, int64_t stride, int64_t max_pages, int
     return table_page(table, stride, max_pages, b, at, shift);
 }
 int64_t probe_sequence(const int32_t* starts, int64_t batch, int64_t row) { return sequence_of(starts, batch, row); }
-int64_t probe_begin(int64_t i, int64_t n, int64_t total) { return split_begin(i, n, total); }
-int64_t probe_part(int64_t x, int64_t n, int64_t total) { return split_part(x, n, total); }
+int64_t probe_begin(int64_t i, int64_t n, int64_t total) { return split_begin(make_split(n, total), i); }
+int64_t probe_part(int64_t x, int64_t n, int64_t total) { return split_part(make_split(n, total), x); }
 int64_t probe_visible(int64_t length, int64_t max_pages, int shift) { return visible_length(length, max_pages, shift); }
 }
