@@ -53,4 +53,22 @@ __device__ __forceinline__ void gstore_plain(T* p, T v, const StoreWindow& w, un
     *p = v;
 }
 
+// Same guard for 32 bytes at a 32-byte aligned address: one whole sector a
+// thread.  Write-back, as the consumers of these outputs come next.
+__device__ __forceinline__ void gstore32(void* p, const uint32_t* v, const StoreWindow& w, unsigned int* status) {
+#ifdef MXFP8_CHECKED
+    const uint8_t* a = static_cast<const uint8_t*>(p);
+    if (a < w.lo || a + 32 > w.hi || (reinterpret_cast<uintptr_t>(p) & 31) != 0) {
+        if (status) atomicOr(status, kErrBoundsStore);
+        return;
+    }
+#else
+    (void)w;
+    (void)status;
+#endif
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+
 }  // namespace mxfp8

@@ -129,23 +129,6 @@ __device__ __forceinline__ void store1(void* out, int64_t at, float v, const Sto
     }
 }
 
-// 32 bytes to a 32-byte aligned address: one whole sector a thread.
-__device__ __forceinline__ void store32(void* p, const uint32_t* v, const StoreWindow& w, unsigned int* status) {
-#ifdef MXFP8_CHECKED
-    const uint8_t* a = static_cast<const uint8_t*>(p);
-    if (a < w.lo || a + 32 > w.hi || (reinterpret_cast<uintptr_t>(p) & 31) != 0) {
-        if (status) atomicOr(status, kErrBoundsStore);
-        return;
-    }
-#else
-    (void)w;
-    (void)status;
-#endif
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
-                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-                 : "memory");
-}
-
 // NC f32 of one row of C, columns col .. col + NC - 1 (those below n), to out.
 template <int OUT, int NC>
 __device__ __forceinline__ void store_row(const GemmParams& p, int64_t row, int col, int n, const uint32_t* acc,
@@ -157,13 +140,13 @@ __device__ __forceinline__ void store_row(const GemmParams& p, int64_t row, int 
 #pragma unroll
         for (int i = 0; i < NC; i += kPer) {
             if constexpr (OUT == MXFP8_F32) {
-                store32(static_cast<float*>(p.out) + at + i, acc + i, p.ow, p.status);
+                gstore32(static_cast<float*>(p.out) + at + i, acc + i, p.ow, p.status);
             } else {
                 uint32_t h[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     h[j] = pack2<OUT>(__uint_as_float(acc[i + 2 * j]), __uint_as_float(acc[i + 2 * j + 1]));
-                store32(static_cast<unsigned short*>(p.out) + at + i, h, p.ow, p.status);
+                gstore32(static_cast<unsigned short*>(p.out) + at + i, h, p.ow, p.status);
             }
         }
     } else {
