@@ -9,14 +9,15 @@
 //
 // Quantizing is also near the ALUs' limit, so a lane holds 16 elements of a
 // row, half a block: one shuffle for the block's amax, one scale for 16 codes.
-// 8192x8192 bf16: 49.3 us with 8 elements a lane and 64-bit index divisions.
+// Measured, 8192x8192 bf16: 26.7 us = 6.36 TB/s (49.3 with 8 elements a lane and
+// 64-bit index divisions); inverted to bf16 27.1 us, to f32 47.6 us (68.5 with
+// 16-byte stores).  Rows off a 32-byte boundary (4096x8191): 20.2 us = 4.2 TB/s.
 #include <cuda_runtime.h>
 
 #include "../../include/mxfp4.h"
 #include "launch.h"
 #include "mxfp4.cuh"
 #include "ptx.cuh"
-#include "stores.cuh"
 
 namespace mxfp8 {
 
@@ -39,55 +40,71 @@ __device__ __forceinline__ WarpUnit warp_unit(uint32_t segs, int cols) {
                     (int64_t)(blockIdx.x - line * segs) * cols};
 }
 
-// How an X row starts, decided for all rows by the base and the row stride.
-enum RowAlign { kAny, kAligned16, kAligned32 };
+__device__ __forceinline__ void load32(const uint8_t* p, uint32_t* w) {
+    asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                 : "l"(p));
+}
 
-// Elements col .. col + 15 of an X row as eight words, zeros from column k on.
-// kAny: the row starts at any even address; every lane loads the two 16-byte
-// chunks that hold its first elements and takes the rest from the next lane's
-// chunk; only chunks that hold one of the row's own elements are read.  Called
-// by whole warps.
-template <RowAlign ALIGN>
-__device__ __forceinline__ void load_row16(const uint8_t* row, int64_t col, int64_t k, uint32_t (&w)[8]) {
+__device__ __forceinline__ void load16(const uint8_t* p, uint32_t* w) {
+    asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "l"(p));
+}
+
+// Elements col .. col + 15 of an X row, in two steps so that the loads of all of a
+// warp's rows are in flight before the first is touched.
+// load: ALIGNED rows start on 32 bytes, and a lane loads its 32.  Otherwise it
+// loads the two aligned 16-byte chunks from the one that holds its first
+// element on, and the last lane the one after them; only chunks that hold one of
+// the row's own elements are read.
+template <bool ALIGNED>
+__device__ __forceinline__ void load_row16(const uint8_t* row, int64_t col, int64_t k, uint32_t (&w)[8],
+                                           uint32_t (&next)[ALIGNED ? 1 : 4]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[i] = 0u;
-    if constexpr (ALIGN == kAligned32) {
-        if (col + 16 <= k) {
-            asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]),
-                           "=r"(w[7])
-                         : "l"(row + 2 * col));
-            return;
-        }
-    }
-    uint4 v[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
-    if constexpr (ALIGN != kAny) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if (col + 8 * i < k) v[i] = __ldcs(reinterpret_cast<const uint4*>(row + 2 * col) + i);
+    if constexpr (ALIGNED) {
+        if (col < k) load32(row + 2 * col, w);
     } else {
         const uint32_t h = (uint32_t)(reinterpret_cast<uintptr_t>(row) & 15);
-        const uint8_t* base = row - h;                     // 16-byte aligned
-        const int64_t end = h + 2 * k;                     // bytes of the row from base
-        const int64_t at = 2 * col;
-        uint4 next = make_uint4(0u, 0u, 0u, 0u);
+        const int64_t end = k > 0 ? h + 2 * k : 0;  // bytes of the row from row - h
+        const uint8_t* at = row - h + 2 * col;
+        if (2 * col < end) load16(at, w);
+        if (2 * col + 16 < end) load16(at + 16, w + 4);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if (at + 16 * i < end) v[i] = __ldcs(reinterpret_cast<const uint4*>(base + at) + i);
-        if ((threadIdx.x & 31) == 31 && at + 32 < end) next = __ldcs(reinterpret_cast<const uint4*>(base + at + 32));
+        for (int i = 0; i < 4; ++i) next[i] = 0u;
+        if ((threadIdx.x & 31) == 31 && 2 * col + 32 < end) load16(at + 32, next);
+    }
+}
+
+// settle: the lane's elements as eight words, zeros from column k on.  The
+// shift is the same for the whole warp; called by whole warps.
+template <bool ALIGNED>
+__device__ __forceinline__ void settle_row16(const uint8_t* row, int64_t col, int64_t k, uint32_t (&w)[8],
+                                             uint32_t (&next)[ALIGNED ? 1 : 4]) {
+    if constexpr (!ALIGNED) {
+        const uint32_t h = (uint32_t)(reinterpret_cast<uintptr_t>(row) & 15);
         if (h != 0) {
-            uint4 nb;
-            nb.x = __shfl_down_sync(0xFFFFFFFFu, v[0].x, 1);
-            nb.y = __shfl_down_sync(0xFFFFFFFFu, v[0].y, 1);
-            nb.z = __shfl_down_sync(0xFFFFFFFFu, v[0].z, 1);
-            nb.w = __shfl_down_sync(0xFFFFFFFFu, v[0].w, 1);
-            if ((threadIdx.x & 31) == 31) nb = next;
-            v[0] = bytes_from<-1>(v[0], v[1], h);
-            v[1] = bytes_from<-1>(v[1], nb, h);
+            uint32_t t[12];
+            const bool last = (threadIdx.x & 31) == 31;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t[i] = w[i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                t[8 + i] = __shfl_down_sync(0xFFFFFFFFu, w[i], 1);
+                if (last) t[8 + i] = next[i];
+            }
+#pragma unroll
+            for (int step = 2; step >= 1; step >>= 1) {  // whole words: 2, 1
+                if (h & (4 * step)) {
+#pragma unroll
+                    for (int i = 0; i + step < 12; ++i) t[i] = t[i + step];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = __funnelshift_r(t[i], t[i + 1], 8u * (h & 3u));
         }
     }
-    w[0] = v[0].x; w[1] = v[0].y; w[2] = v[0].z; w[3] = v[0].w;
-    w[4] = v[1].x; w[5] = v[1].y; w[6] = v[1].z; w[7] = v[1].w;
     if (col + 16 > k) {  // the row ends inside: clear what lies behind it
         const int64_t left = k - col;
 #pragma unroll
@@ -116,7 +133,7 @@ __device__ __forceinline__ void scale4(uint32_t w0, uint32_t w1, float inv, floa
     mul2(c, d, inv, f[2], f[3]);
 }
 
-template <int DT, RowAlign ALIGN>
+template <int DT, bool ALIGNED>
 __global__ void __launch_bounds__(kConvertThreads) mxfp4_quantize_kernel(
     const uint8_t* __restrict__ x, int64_t m, int64_t k, int64_t row_bytes, uint8_t* __restrict__ q, int64_t q_cols,
     int64_t ld_q, uint8_t* __restrict__ s, int64_t col_chunks, uint32_t segs, StoreWindow qw, StoreWindow sw,
@@ -126,16 +143,17 @@ __global__ void __launch_bounds__(kConvertThreads) mxfp4_quantize_kernel(
     const WarpUnit u = warp_unit(segs, kQuantCols);
     const int lane = threadIdx.x & 31;
     const int64_t col = u.c0 + lane * 16;
-    uint32_t w[kRowsPerWarp][8];
+    uint32_t w[kRowsPerWarp][8], next[kRowsPerWarp][ALIGNED ? 1 : 4];
 #pragma unroll
     for (int i = 0; i < kRowsPerWarp; ++i) {
         const int64_t row = u.row0 + 32 * i;
-        load_row16<ALIGN>(x + row * row_bytes, col, row < m ? k : 0, w[i]);
+        load_row16<ALIGNED>(x + row * row_bytes, col, row < m ? k : 0, w[i], next[i]);
     }
     uint32_t words[kRowsPerWarp];
 #pragma unroll
     for (int i = 0; i < kRowsPerWarp; ++i) {
         const int64_t row = u.row0 + 32 * i;
+        settle_row16<ALIGNED>(x + row * row_bytes, col, row < m ? k : 0, w[i], next[i]);
         uint32_t a = w[i][0] & 0x7FFF7FFFu;
 #pragma unroll
         for (int j = 1; j < 8; ++j) a = __vmaxu2(a, w[i][j] & 0x7FFF7FFFu);
@@ -280,14 +298,10 @@ int launch_mxfp4_quantize(const Fp4QuantizeArgs& a, cudaStream_t stream) {
     const int64_t col_chunks = (a.q_cols + 127) / 128;
     const int64_t blocks = convert_blocks(row_blocks, segs);
     if (blocks < 0) return MXFP8_ERR_SHAPE;
-    const uint64_t start = reinterpret_cast<uintptr_t>(a.x) | (uint64_t)(a.m > 1 ? a.ld_x * 2 : 0);
-    const RowAlign align = start % 32 == 0 ? kAligned32 : start % 16 == 0 ? kAligned16 : kAny;
-    auto kernel = a.dtype == MXFP8_BF16 ? (align == kAligned32   ? mxfp4_quantize_kernel<kBF16, kAligned32>
-                                           : align == kAligned16 ? mxfp4_quantize_kernel<kBF16, kAligned16>
-                                                                 : mxfp4_quantize_kernel<kBF16, kAny>)
-                                        : (align == kAligned32   ? mxfp4_quantize_kernel<kFP16, kAligned32>
-                                           : align == kAligned16 ? mxfp4_quantize_kernel<kFP16, kAligned16>
-                                                                 : mxfp4_quantize_kernel<kFP16, kAny>);
+    const bool aligned = ((reinterpret_cast<uintptr_t>(a.x) | (uint64_t)(a.m > 1 ? a.ld_x * 2 : 0)) & 31) == 0;
+    auto kernel = a.dtype == MXFP8_BF16
+                      ? (aligned ? mxfp4_quantize_kernel<kBF16, true> : mxfp4_quantize_kernel<kBF16, false>)
+                      : (aligned ? mxfp4_quantize_kernel<kFP16, true> : mxfp4_quantize_kernel<kFP16, false>);
     return launch_convert(kernel, blocks, stream, "mxfp4_quantize_kernel launch", static_cast<const uint8_t*>(a.x), a.m,
                           a.k, a.ld_x * 2, a.q, a.q_cols, a.ld_q, a.s, col_chunks, (uint32_t)segs, a.qw, a.sw,
                           a.status);

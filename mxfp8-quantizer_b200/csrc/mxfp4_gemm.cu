@@ -2,15 +2,18 @@
 // block-scaled tensor cores (tcgen05.mma kind::mxf4): 64 products of E2M1
 // values a step, each block of 32 scaled by 2^(sa + sb - 254), summed in f32.
 //
-// One matrix supplies the 128 rows of a tile (P), the other its BN columns
-// (Q).  A CTA has one warp that streams 256-column stages of both (TMA tiles
-// with the 128-byte swizzle, scale chunks as untiled copies: a 128-row block's
-// chunks are contiguous along K), one that copies the scales to tensor memory
-// and issues the MMAs, and four or eight that read the accumulators back.
+// One matrix supplies the rows of a tile (P, the lanes of tensor memory), the
+// other its columns (Q).  A CTA has one warp that streams 256-column stages of
+// both (TMA tiles with the 128-byte swizzle, scale chunks as untiled copies: a
+// 128-row block's chunks are contiguous along K), one that copies the scales to
+// tensor memory and issues the MMAs, and four or eight that read the
+// accumulators back.  Two forms:
 //
-// SWAP = false: P is A.  A lane of tensor memory is a row of C, its columns
-//   are contiguous in memory: 32-byte stores.
-// SWAP = true: P is B.  A lane is a column of C, so a warp's stores are
+// wide: P is A, Q is B.  The two CTAs of a cluster pair compute one 256 x 256
+//   tile (cta_group::2): each loads its 128 rows of A and half of the 256 rows
+//   of B, 35 KB a stage for 4 MMAs where a CTA on its own would load 51.  A lane
+//   is a row of C, its columns are contiguous in memory: 32-byte stores.
+// narrow: P is B, Q is A.  A lane is a column of C, so a warp's stores are
 //   contiguous for any alignment, and few rows of A make a narrow tile: the
 //   form for single tokens, where streaming B is the whole cost.  If there are
 //   fewer tiles than SMs, a cluster of CTAs shares a tile: each takes a part of
@@ -37,32 +40,49 @@ namespace {
 constexpr int kTileP = 128;        // rows of P in a tile: the MMA's M
 constexpr int kStageK = 256;       // elements of K in a stage: 128 bytes a row
 constexpr int kStepK = 64;         // elements of K in one MMA
+constexpr int kPBytes = kTileP * 128;
 constexpr int kChunk = 512;        // bytes of one 128-row x 4-block scale chunk
 constexpr uint64_t kWaitNs = 1000000000ull;
 constexpr unsigned kErrGemmWait = 32u;   // bit of the device status word
 
-template <int BN, bool SWAP>
-struct Config {
-    static constexpr int row_blocks_q = (BN + 127) / 128;
-    static constexpr int p_bytes = kTileP * 128;
+template <int BN>
+struct Narrow {
     static constexpr int q_bytes = BN * 128;
-    static constexpr int sp_off = p_bytes + q_bytes;
+    static constexpr int sp_off = kPBytes + q_bytes;
     static constexpr int sq_off = sp_off + 2 * kChunk;
-    static constexpr int stage_bytes = sq_off + row_blocks_q * 2 * kChunk;
-    static constexpr int stages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
-    static constexpr int acc = BN <= 128 ? 2 : 1;              // accumulators in tensor memory
-    static constexpr int epi_warps = BN <= 128 ? 4 : 8;
+    static constexpr int stage_bytes = sq_off + 2 * kChunk;
+    static constexpr int stages = BN == 128 ? 6 : 8;
+    static constexpr int acc = 2;                               // accumulators in tensor memory
+    static constexpr int epi_warps = 4;
     static constexpr int threads = 32 * (epi_warps + 2);
-    // tensor memory: accumulators, then two sets of scales (A's and B's of one stage)
-    static constexpr int sf_cols = 2 * 4 + 2 * 4 * row_blocks_q;
+    // tensor memory: accumulators, then two sets of scales (P's and Q's of one stage)
+    static constexpr int sf_cols = 16;
     static constexpr int cols_used = acc * BN + 2 * sf_cols;
     static constexpr int tmem_cols = cols_used <= 64 ? 64 : cols_used <= 128 ? 128 : cols_used <= 256 ? 256 : 512;
     static constexpr int bar_off = stages * stage_bytes;
     static constexpr int n_bars = 2 * stages + 2 * acc;
     static constexpr int ctl_off = bar_off + 8 * n_bars;
     static constexpr int smem = ctl_off + 16 + 1024;            // and room to align the base to 1024
-    static_assert(cols_used <= 512 && stage_bytes % 1024 == 0);
-    static_assert(!SWAP || BN <= 128, "the join of a split K holds one BN x 128 f32 tile in the stages");
+    static_assert(BN <= 128 && cols_used <= 512 && stage_bytes % 1024 == 0);
+    static_assert(BN * 512 <= stages * stage_bytes, "the join of a split K holds a BN x 128 f32 tile in the stages");
+};
+
+struct Wide {
+    static constexpr int bn = 256;
+    static constexpr int q_bytes = bn / 2 * 128;                // this CTA's half of Q
+    static constexpr int sp_off = kPBytes + q_bytes;
+    static constexpr int sq_off = sp_off + 2 * kChunk;          // scales of all 256 rows of Q
+    static constexpr int stage_bytes = sq_off + 4 * kChunk;
+    static constexpr int stages = 6;
+    static constexpr int epi_warps = 8;
+    static constexpr int threads = 32 * (epi_warps + 2);
+    static constexpr int sf_cols = 8 + 16;
+    static constexpr int tmem_cols = 512;                       // 256 + 2 * 24 of them used
+    static constexpr int bar_off = stages * stage_bytes;
+    static constexpr int n_bars = 2 * stages + 2;
+    static constexpr int ctl_off = bar_off + 8 * n_bars;
+    static constexpr int smem = ctl_off + 16 + 1024;
+    static_assert(stage_bytes % 1024 == 0 && smem <= 227 * 1024);
 };
 
 struct GemmParams {
@@ -74,7 +94,7 @@ struct GemmParams {
     int k;
     int n_stages;               // ceil(k / 256)
     int tiles_p, n_tiles;
-    int split;                  // CTAs of a cluster that share a tile
+    int split;                  // narrow: CTAs of a cluster that share a tile
     void* out;
     int64_t ld_out;
     StoreWindow ow;
@@ -82,11 +102,13 @@ struct GemmParams {
 };
 
 // Wait for a barrier's phase, at most kWaitNs, or until another role gave up.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, volatile int* abort, unsigned int* status) {
-    if (mbar_try_wait(bar, parity)) return true;
+    auto done = [&] { return CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity); };
+    if (done()) return true;
     const uint64_t t0 = global_timer_ns();
     for (uint32_t i = 1;; ++i) {
-        if (mbar_try_wait(bar, parity)) return true;
+        if (done()) return true;
         if ((i & 255u) == 0) {
             if (*abort) return false;
             if (global_timer_ns() - t0 > kWaitNs) {
@@ -95,6 +117,19 @@ __device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, volati
                 return false;
             }
         }
+    }
+}
+
+// The load thread's end: wait until the last use of every stage is over, so that
+// nothing arrives on its barriers later.  After an abort nobody may release
+// the stages: then the copies themselves are waited for, as they still target this CTA.
+template <int STAGES>
+__device__ __forceinline__ void drain_stages(uint32_t full0, uint32_t empty0, int issued, volatile int* ctl,
+                                             unsigned int* status) {
+    for (int i = max(0, issued - STAGES); i < issued; ++i) {
+        const int s = i % STAGES;
+        const uint32_t parity = (i / STAGES) & 1;
+        if (ctl[0] || !wait_phase(empty0 + 8 * s, parity, ctl, status)) mbar_wait_bounded(full0 + 8 * s, parity, kWaitNs);
     }
 }
 
@@ -129,6 +164,25 @@ __device__ __forceinline__ void store1(void* out, int64_t at, float v, const Sto
     }
 }
 
+// Four f32 of one row of C, columns col .. col + 3 (those below n = rows_p).
+template <int OUT>
+__device__ __forceinline__ void store_quad(const GemmParams& p, int64_t row, int col, const float4& v) {
+    constexpr int kEs = OUT == MXFP8_F32 ? 4 : 2;
+    const int64_t at = row * p.ld_out + col;
+    if (((reinterpret_cast<uintptr_t>(p.out) + (uint64_t)at * kEs) & (4 * kEs - 1)) == 0 && col + 4 <= p.rows_p) {
+        if constexpr (OUT == MXFP8_F32)
+            gstore_plain(reinterpret_cast<float4*>(static_cast<float*>(p.out) + at), v, p.ow, p.status);
+        else
+            gstore_plain(reinterpret_cast<uint2*>(static_cast<unsigned short*>(p.out) + at),
+                         make_uint2(pack2<OUT>(v.x, v.y), pack2<OUT>(v.z, v.w)), p.ow, p.status);
+        return;
+    }
+    const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (col + i < p.rows_p) store1<OUT>(p.out, at + i, f[i], p.ow, p.status);
+}
+
 // NC f32 of one row of C, columns col .. col + NC - 1 (those below n), to out.
 template <int OUT, int NC>
 __device__ __forceinline__ void store_row(const GemmParams& p, int64_t row, int col, int n, const uint32_t* acc,
@@ -156,17 +210,17 @@ __device__ __forceinline__ void store_row(const GemmParams& p, int64_t row, int 
     }
 }
 
-template <int BN, bool SWAP, int OUT>
-__global__ void __launch_bounds__(Config<BN, SWAP>::threads, 1)
-    mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
+template <int BN, int OUT>
+__global__ void __launch_bounds__(Narrow<BN>::threads, 1)
+    mxfp4_gemm_narrow_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
                       const GemmParams p) {
-    using C = Config<BN, SWAP>;
+    using C = Narrow<BN>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t base = smem_u32(smem);
     const uint32_t full0 = base + C::bar_off, empty0 = full0 + 8 * C::stages;
     const uint32_t acc_full0 = empty0 + 8 * C::stages, acc_empty0 = acc_full0 + 8 * C::acc;
-    volatile int* ctl = reinterpret_cast<volatile int*>(smem + C::ctl_off);  // abort, consumed stages, TMEM address
+    volatile int* ctl = reinterpret_cast<volatile int*>(smem + C::ctl_off);  // abort, -, TMEM address
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int kLoadWarp = C::epi_warps, kMmaWarp = C::epi_warps + 1;
 
@@ -180,10 +234,9 @@ __global__ void __launch_bounds__(Config<BN, SWAP>::threads, 1)
             mbar_init(acc_empty0 + 8 * i, C::epi_warps);
         }
         ctl[0] = 0;
-        ctl[1] = 0;
         fence_mbar_init();
     }
-    if (warp == kMmaWarp) tmem_alloc(base + C::ctl_off + 8, C::tmem_cols);
+    if (warp == kMmaWarp) tmem_alloc<1>(base + C::ctl_off + 8, C::tmem_cols);
     if (warp == kLoadWarp && lane == 0) {
         prefetch_tensormap(&map_p);
         prefetch_tensormap(&map_q);
@@ -217,16 +270,13 @@ __global__ void __launch_bounds__(Config<BN, SWAP>::threads, 1)
                     }
                     const uint32_t dst = base + s * C::stage_bytes, bar = full0 + 8 * s;
                     const int chunks = min(2, p.col_chunks - 2 * ks);
-                    const int rbq = tq * BN / 128;
-                    const int nrbq = min(C::row_blocks_q, p.row_blocks_q - rbq);
-                    mbar_arrive_expect_tx(bar, C::p_bytes + C::q_bytes + (1 + nrbq) * chunks * kChunk);
+                    mbar_arrive_expect_tx(bar, kPBytes + C::q_bytes + 2 * chunks * kChunk);
                     tma_load_2d(dst, &map_p, ks * (kStageK / 2), tp * kTileP, bar);
-                    tma_load_2d(dst + C::p_bytes, &map_q, ks * (kStageK / 2), tq * BN, bar);
+                    tma_load_2d(dst + kPBytes, &map_q, ks * (kStageK / 2), tq * BN, bar);
                     bulk_load(dst + C::sp_off, p.sp + ((int64_t)tp * p.col_chunks + 2 * ks) * kChunk, chunks * kChunk,
                               bar);
-                    for (int r = 0; r < nrbq; ++r)
-                        bulk_load(dst + C::sq_off + r * 2 * kChunk,
-                                  p.sq + ((int64_t)(rbq + r) * p.col_chunks + 2 * ks) * kChunk, chunks * kChunk, bar);
+                    bulk_load(dst + C::sq_off, p.sq + ((int64_t)tq * p.col_chunks + 2 * ks) * kChunk, chunks * kChunk,
+                              bar);
                 }
             }
         }
@@ -250,27 +300,22 @@ __global__ void __launch_bounds__(Config<BN, SWAP>::threads, 1)
                     const uint32_t sfp = tmem_sf + (it & 1) * C::sf_cols, sfq = sfp + 8;
                     const int chunks = min(2, p.col_chunks - 2 * ks);
                     for (int c = 0; c < chunks; ++c) {
-                        tmem_copy_scales(sfp + 4 * c, desc_scale_chunk(src + C::sp_off + c * kChunk));
-#pragma unroll
-                        for (int r = 0; r < C::row_blocks_q; ++r)
-                            tmem_copy_scales(sfq + 4 * (c * C::row_blocks_q + r),
-                                             desc_scale_chunk(src + C::sq_off + (2 * r + c) * kChunk));
+                        tmem_copy_scales<1>(sfp + 4 * c, desc_scale_chunk(src + C::sp_off + c * kChunk));
+                        tmem_copy_scales<1>(sfq + 4 * c, desc_scale_chunk(src + C::sq_off + c * kChunk));
                     }
                     const int steps = min(kStageK / kStepK, (p.k - ks * kStageK + kStepK - 1) / kStepK);
                     for (int j = 0; j < steps; ++j) {
                         const int c = j >> 1, sf = 2 * (j & 1);
-                        mma_mxf4(d, desc_sw128(src + 32 * j), desc_sw128(src + C::p_bytes + 32 * j),
-                                 mxf4_idesc(kTileP, BN, sf), sfp + 4 * c, sfq + 4 * c * C::row_blocks_q,
-                                 ks > ks0 || j > 0);
+                        mma_mxf4<1>(d, desc_sw128(src + 32 * j), desc_sw128(src + kPBytes + 32 * j),
+                                    mxf4_idesc(kTileP, BN, sf), sfp + 4 * c, sfq + 4 * c, ks > ks0 || j > 0);
                     }
-                    tcgen05_commit(empty0 + 8 * s);
+                    tcgen05_commit<1>(empty0 + 8 * s);
                 }
-                if (ok) tcgen05_commit(acc_full0 + 8 * slot);
+                if (ok) tcgen05_commit<1>(acc_full0 + 8 * slot);
             }
-            ctl[1] = it;
             // an abort leaves MMAs in flight: let them end before the tensor memory goes
             if (ctl[0]) {
-                tcgen05_commit(acc_full0);
+                tcgen05_commit<1>(acc_full0);
                 mbar_wait_bounded(acc_full0, 0, kWaitNs);
             }
         }
@@ -286,28 +331,7 @@ __global__ void __launch_bounds__(Config<BN, SWAP>::threads, 1)
             int tp, tq;
             tile_of(p, t, tp, tq);
             const uint32_t d = tmem + slot * BN + lane_off;
-            if constexpr (!SWAP) {
-                // eight warps: two for each quarter of the lanes, 128 columns each
-                const int col0 = (warp >> 2) * 128;
-                uint32_t v[4][32];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) tmem_load_32(d + col0 + 32 * i, v[i]);
-                tmem_wait_loads();
-#pragma unroll
-                for (int i = 0; i < 4; ++i) tmem_loaded(v[i]);
-                // the accumulator is in registers: the next tile's MMAs may overwrite it
-                tcgen05_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(acc_empty0 + 8 * slot);
-                const int64_t row = (int64_t)tp * kTileP + q4 * 32 + lane;
-                constexpr int kEs = OUT == MXFP8_F32 ? 4 : 2;
-                const bool vec = ((reinterpret_cast<uintptr_t>(p.out) | (uint64_t)(p.ld_out * kEs)) & 31) == 0;
-                if (row < p.rows_p) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        store_row<OUT, 32>(p, row, tq * BN + col0 + 32 * i, p.rows_q, v[i], vec);
-                }
-            } else {
+            {
                 const int64_t n = (int64_t)tp * kTileP + q4 * 32 + lane;
                 const int left = min(BN, p.rows_q - tq * BN);
                 float* red = reinterpret_cast<float*>(smem);
@@ -333,35 +357,216 @@ __global__ void __launch_bounds__(Config<BN, SWAP>::threads, 1)
             }
         }
     }
+    if (warp == kLoadWarp && lane == 0) drain_stages<C::stages>(full0, empty0, issued, ctl, p.status);
     __syncwarp();
-    if constexpr (SWAP) {
-        if (p.split > 1) {  // one tile a cluster: add the parts up, each CTA its share of the columns
-            cluster_sync();
-            if (warp < C::epi_warps && !ctl[0]) {
-                int tp, tq;
-                tile_of(p, first_tile, tp, tq);
-                const int64_t n = (int64_t)tp * kTileP + threadIdx.x;
-                const int left = min(BN, p.rows_q - tq * BN);
-                for (int c = rank; c < left; c += p.split) {
-                    const uint32_t at = base + (uint32_t)(c * 128 + threadIdx.x) * 4u;
-                    float sum = 0.0f;
-                    for (int r = 0; r < p.split; ++r) sum += cluster_load_f32(cluster_map(at, r));
-                    if (n < p.rows_p)
-                        store1<OUT>(p.out, ((int64_t)tq * BN + c) * p.ld_out + n, sum, p.ow, p.status);
+    if (p.split > 1) {  // one tile a cluster: add the parts up, each CTA its share of the columns
+        cluster_sync();
+        if (warp < C::epi_warps && !ctl[0]) {
+            int tp, tq;
+            tile_of(p, first_tile, tp, tq);
+            const int left = min(BN, p.rows_q - tq * BN);
+            // a warp takes a column, a lane four of its rows; four columns at a time keep the remote loads in flight
+            for (int c0 = rank + p.split * warp; c0 < left; c0 += 4 * C::epi_warps * p.split) {
+                float4 sum[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for (int r = 0; r < p.split; ++r) {
+                    const uint32_t at = cluster_map(base, r) + (uint32_t)lane * 16u;
+                    float4 v[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)  // columns past `left` read what the tile left there, below BN
+                        v[i] = cluster_load_f32x4(at + (uint32_t)min(c0 + i * C::epi_warps * p.split, left - 1) * 512u);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        sum[i].x += v[i].x;
+                        sum[i].y += v[i].y;
+                        sum[i].z += v[i].z;
+                        sum[i].w += v[i].w;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int c = c0 + i * C::epi_warps * p.split;
+                    if (c < left) store_quad<OUT>(p, (int64_t)tq * BN + c, tp * kTileP + 4 * lane, sum[i]);
                 }
             }
-            cluster_sync();  // nobody leaves while its part is still read
         }
+        cluster_sync();  // nobody leaves while its part is still read
     }
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
-    if (warp == kLoadWarp && lane == 0) {
-        // loads that nobody waited for (only after an abort) still target this CTA
-        for (int i = ctl[1]; i < issued; ++i)
-            if (!mbar_wait_bounded(full0 + 8 * (i % C::stages), (i / C::stages) & 1, kWaitNs)) break;
+    if (warp == kMmaWarp) tmem_dealloc<1>(tmem, C::tmem_cols);
+}
+
+
+// The wide form: a cluster pair a tile.  The odd CTA loads its share and reads
+// its half of the rows back; its MMA thread only tells the even one, which
+// issues for both, when a stage of its own has landed.
+template <int OUT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide::threads, 1)
+    mxfp4_gemm_wide_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
+                           const GemmParams p) {
+    using C = Wide;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    const uint32_t base = smem_u32(smem);
+    const uint32_t full0 = base + C::bar_off, empty0 = full0 + 8 * C::stages;
+    const uint32_t acc_full = empty0 + 8 * C::stages, acc_empty = acc_full + 8;
+    volatile int* ctl = reinterpret_cast<volatile int*>(smem + C::ctl_off);  // abort, -, TMEM address
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int kLoadWarp = C::epi_warps, kMmaWarp = C::epi_warps + 1;
+    const int rank = blockIdx.x & 1;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::stages; ++i) {
+            mbar_init(full0 + 8 * i, rank == 0 ? 2 : 1);  // the even CTA's: its own stage and the odd CTA's
+            mbar_init(empty0 + 8 * i, 1);
+        }
+        mbar_init(acc_full, 1);
+        mbar_init(acc_empty, 2 * C::epi_warps);           // used in the even CTA: both CTAs' readers
+        ctl[0] = 0;
+        fence_mbar_init();
     }
-    if (warp == kMmaWarp) tmem_dealloc(tmem, C::tmem_cols);
+    if (warp == kMmaWarp) tmem_alloc<2>(base + C::ctl_off + 8, C::tmem_cols);
+    if (warp == kLoadWarp && lane == 0) {
+        prefetch_tensormap(&map_p);
+        prefetch_tensormap(&map_q);
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    cluster_sync();  // the other CTA's barriers are ready, too
+    tcgen05_fence_after();
+    const uint32_t tmem = (uint32_t)ctl[2];
+    const uint32_t tmem_sf = tmem + C::bn;
+    grid_launch_dependents();
+    grid_wait_prerequisites();
+
+    const int first_tile = blockIdx.x >> 1, tile_step = gridDim.x >> 1;
+    int issued = 0;  // stages loaded by the load thread
+
+    if (warp == kLoadWarp) {
+        if (lane == 0) {
+            bool ok = true;
+            for (int t = first_tile; ok && t < p.n_tiles; t += tile_step) {
+                int tp, tq;
+                tile_of(p, t, tp, tq);
+                const int row_block = 2 * tp + rank;
+                // the last pair's odd CTA may have no rows: its payload is zeros, its scales any bytes
+                const bool has_rows = row_block * kTileP < p.rows_p;
+                const int nrbq = min(2, p.row_blocks_q - 2 * tq);
+                for (int ks = 0; ks < p.n_stages; ++ks, ++issued) {
+                    const int s = issued % C::stages;
+                    if (issued >= C::stages &&
+                        !wait_phase(empty0 + 8 * s, ((issued / C::stages) - 1) & 1, ctl, p.status)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t dst = base + s * C::stage_bytes, bar = full0 + 8 * s;
+                    const int chunks = min(2, p.col_chunks - 2 * ks);
+                    mbar_arrive_expect_tx(bar, kPBytes + C::q_bytes + ((has_rows ? 1 : 0) + nrbq) * chunks * kChunk);
+                    tma_load_2d(dst, &map_p, ks * (kStageK / 2), row_block * kTileP, bar);
+                    tma_load_2d(dst + kPBytes, &map_q, ks * (kStageK / 2), tq * C::bn + rank * (C::bn / 2), bar);
+                    if (has_rows)
+                        bulk_load(dst + C::sp_off, p.sp + ((int64_t)row_block * p.col_chunks + 2 * ks) * kChunk,
+                                  chunks * kChunk, bar);
+                    for (int r = 0; r < nrbq; ++r)
+                        bulk_load(dst + C::sq_off + r * 2 * kChunk,
+                                  p.sq + ((int64_t)(2 * tq + r) * p.col_chunks + 2 * ks) * kChunk, chunks * kChunk, bar);
+                }
+            }
+        }
+    } else if (warp == kMmaWarp) {
+        if (lane == 0 && rank == 1) {
+            const uint32_t peer_full0 = cluster_map(full0, 0);
+            int it = 0;
+            bool ok = true;
+            for (int t = first_tile; ok && t < p.n_tiles; t += tile_step)
+                for (int ks = 0; ks < p.n_stages; ++ks, ++it) {
+                    const int s = it % C::stages;
+                    if (!wait_phase(full0 + 8 * s, (it / C::stages) & 1, ctl, p.status)) {
+                        ok = false;
+                        break;
+                    }
+                    cluster_arrive(peer_full0 + 8 * s);
+                }
+        } else if (lane == 0) {
+            int it = 0, a = 0;
+            bool ok = true;
+            for (int t = first_tile; ok && t < p.n_tiles; t += tile_step, ++a) {
+                if (a > 0 && !wait_phase<true>(acc_empty, (a - 1) & 1, ctl, p.status)) break;
+                tcgen05_fence_after();
+                for (int ks = 0; ks < p.n_stages; ++ks, ++it) {
+                    const int s = it % C::stages;
+                    if (!wait_phase<true>(full0 + 8 * s, (it / C::stages) & 1, ctl, p.status)) {
+                        ok = false;
+                        break;
+                    }
+                    tcgen05_fence_after();
+                    const uint32_t src = base + s * C::stage_bytes;
+                    const uint32_t sfp = tmem_sf + (it & 1) * C::sf_cols, sfq = sfp + 8;
+                    const int chunks = min(2, p.col_chunks - 2 * ks);
+                    for (int c = 0; c < chunks; ++c) {
+                        tmem_copy_scales<2>(sfp + 4 * c, desc_scale_chunk(src + C::sp_off + c * kChunk));
+#pragma unroll
+                        for (int r = 0; r < 2; ++r)
+                            tmem_copy_scales<2>(sfq + 8 * c + 4 * r,
+                                                desc_scale_chunk(src + C::sq_off + (2 * r + c) * kChunk));
+                    }
+                    const int steps = min(kStageK / kStepK, (p.k - ks * kStageK + kStepK - 1) / kStepK);
+                    for (int j = 0; j < steps; ++j) {
+                        const int c = j >> 1, sf = 2 * (j & 1);
+                        mma_mxf4<2>(tmem, desc_sw128(src + 32 * j), desc_sw128(src + kPBytes + 32 * j),
+                                    mxf4_idesc(2 * kTileP, C::bn, sf), sfp + 4 * c, sfq + 8 * c, ks > 0 || j > 0);
+                    }
+                    tcgen05_commit<2>(empty0 + 8 * s);
+                }
+                if (ok) tcgen05_commit<2>(acc_full);
+            }
+            // an abort leaves MMAs in flight: let them end before the tensor memory goes
+            if (ctl[0]) {
+                tcgen05_commit<2>(acc_full);
+                mbar_wait_bounded(acc_full, 0, kWaitNs);
+            }
+        }
+    } else {
+        // two warps for each quarter of the lanes, 128 columns each
+        const int q4 = warp & 3, col0 = (warp >> 2) * 128;
+        const uint32_t d = tmem + col0 + ((uint32_t)(q4 * 32) << 16);
+        const uint32_t peer_acc_empty = cluster_map(acc_empty, 0);
+        constexpr int kEs = OUT == MXFP8_F32 ? 4 : 2;
+        const bool vec = ((reinterpret_cast<uintptr_t>(p.out) | (uint64_t)(p.ld_out * kEs)) & 31) == 0;
+        int a = 0;
+        for (int t = first_tile; t < p.n_tiles; t += tile_step, ++a) {
+            if (!__all_sync(0xFFFFFFFFu, wait_phase(acc_full, a & 1, ctl, p.status))) break;
+            tcgen05_fence_after();
+            int tp, tq;
+            tile_of(p, t, tp, tq);
+            uint32_t v[4][32];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) tmem_load_32(d + 32 * i, v[i]);
+            tmem_wait_loads();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) tmem_loaded(v[i]);
+            // the accumulator is in registers: the next tile's MMAs may overwrite it
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) cluster_arrive(peer_acc_empty);
+            const int64_t row = (int64_t)(2 * tp + rank) * kTileP + q4 * 32 + lane;
+            if (row < p.rows_p) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    store_row<OUT, 32>(p, row, tq * C::bn + col0 + 32 * i, p.rows_q, v[i], vec);
+            }
+        }
+    }
+    if (warp == kLoadWarp && lane == 0) drain_stages<C::stages>(full0, empty0, issued, ctl, p.status);
+    __syncwarp();
+    tcgen05_fence_before();
+    __syncthreads();
+    cluster_sync();  // the other CTA's barriers and tensor memory are no longer in use
+    tcgen05_fence_after();
+    if (warp == kMmaWarp) tmem_dealloc<2>(tmem, C::tmem_cols);
 }
 
 // Tensor map of a payload: bytes (rows, cols / 2), boxes of 128 bytes by
@@ -386,28 +591,26 @@ int encode_payload(CUtensorMap* map, const void* q, int64_t rows, int64_t bytes,
     return MXFP8_OK;
 }
 
-template <int BN, bool SWAP, int OUT>
-int launch_typed(const Fp4GemmArgs& g, int sm_count, cudaStream_t stream) {
-    using C = Config<BN, SWAP>;
-    auto kernel = mxfp4_gemm_kernel<BN, SWAP, OUT>;
-    // once per device: later launches, captured ones among them, make no such call
-    static std::atomic<uint64_t> attr_set{0};
+// A kernel's shared memory opt-in, once per device: later launches, captured
+// ones among them, make no such call.
+template <typename K>
+cudaError_t opt_in(K* kernel, int smem, std::atomic<uint64_t>& done) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     const uint64_t bit = 1ull << (dev & 63);
-    if (e == cudaSuccess && !(attr_set.load(std::memory_order_acquire) & bit)) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem);
-        if (e == cudaSuccess) attr_set.fetch_or(bit, std::memory_order_acq_rel);
+    if (e == cudaSuccess && !(done.load(std::memory_order_acquire) & bit)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_acq_rel);
     }
-    if (e != cudaSuccess) {
-        set_last_error("cudaFuncSetAttribute", (int)e);
-        return MXFP8_ERR_CUDA;
-    }
-    const Fp4Operand& P = SWAP ? g.b : g.a;
-    const Fp4Operand& Q = SWAP ? g.a : g.b;
-    CUtensorMap map_p, map_q;
-    if (int rc = encode_payload(&map_p, P.q, P.rows, g.k / 2, P.ld, kTileP)) return rc;
-    if (int rc = encode_payload(&map_q, Q.q, Q.rows, g.k / 2, Q.ld, BN)) return rc;
+    return e;
+}
+
+int launch_failed(const char* what, cudaError_t e) {
+    set_last_error(what, (int)e);
+    return MXFP8_ERR_CUDA;
+}
+
+GemmParams params_of(const Fp4GemmArgs& g, const Fp4Operand& P, const Fp4Operand& Q, int tile_p, int tile_q) {
     GemmParams p;
     p.sp = P.s;
     p.sq = Q.s;
@@ -417,20 +620,58 @@ int launch_typed(const Fp4GemmArgs& g, int sm_count, cudaStream_t stream) {
     p.rows_q = (int)Q.rows;
     p.k = (int)g.k;
     p.n_stages = (int)((g.k + kStageK - 1) / kStageK);
-    p.tiles_p = (int)((P.rows + kTileP - 1) / kTileP);
-    const int64_t tiles = (int64_t)p.tiles_p * ((Q.rows + BN - 1) / BN);
-    if (tiles > (1 << 24)) return MXFP8_ERR_SHAPE;
-    p.n_tiles = (int)tiles;
+    p.tiles_p = (int)((P.rows + tile_p - 1) / tile_p);
+    p.n_tiles = p.tiles_p * (int)((Q.rows + tile_q - 1) / tile_q);
     p.split = 1;
-    if (SWAP)  // double the CTAs of a tile while they fit the SMs and each keeps two stages
-        while (p.split < 8 && tiles * p.split * 2 <= sm_count && p.n_stages >= 4 * p.split) p.split *= 2;
     p.out = g.out;
     p.ld_out = g.ld_out;
     p.ow = g.ow;
     p.status = g.status;
+    return p;
+}
 
+template <int OUT>
+int launch_wide(const Fp4GemmArgs& g, int sm_count, cudaStream_t stream) {
+    using C = Wide;
+    static std::atomic<uint64_t> done{0};
+    auto kernel = mxfp4_gemm_wide_kernel<OUT>;
+    cudaError_t e = opt_in(kernel, C::smem, done);
+    if (e != cudaSuccess) return launch_failed("cudaFuncSetAttribute", e);
+    CUtensorMap map_p, map_q;
+    if (int rc = encode_payload(&map_p, g.a.q, g.a.rows, g.k / 2, g.a.ld, kTileP)) return rc;
+    if (int rc = encode_payload(&map_q, g.b.q, g.b.rows, g.k / 2, g.b.ld, C::bn / 2)) return rc;
+    const GemmParams p = params_of(g, g.a, g.b, 2 * kTileP, C::bn);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(p.split > 1 ? tiles * p.split : tiles < sm_count ? tiles : sm_count));
+    const int pairs = sm_count / 2;
+    cfg.gridDim = dim3(2u * (unsigned)(p.n_tiles < pairs ? p.n_tiles : pairs));
+    cfg.blockDim = dim3(C::threads);
+    cfg.dynamicSmemBytes = C::smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, kernel, map_p, map_q, p);
+    if (e == cudaSuccess) e = cudaGetLastError();
+    return e == cudaSuccess ? MXFP8_OK : launch_failed("mxfp4_gemm_wide_kernel launch", e);
+}
+
+template <int BN, int OUT>
+int launch_narrow(const Fp4GemmArgs& g, int sm_count, cudaStream_t stream) {
+    using C = Narrow<BN>;
+    static std::atomic<uint64_t> done{0};
+    auto kernel = mxfp4_gemm_narrow_kernel<BN, OUT>;
+    cudaError_t e = opt_in(kernel, C::smem, done);
+    if (e != cudaSuccess) return launch_failed("cudaFuncSetAttribute", e);
+    CUtensorMap map_p, map_q;
+    if (int rc = encode_payload(&map_p, g.b.q, g.b.rows, g.k / 2, g.b.ld, kTileP)) return rc;
+    if (int rc = encode_payload(&map_q, g.a.q, g.a.rows, g.k / 2, g.a.ld, BN)) return rc;
+    GemmParams p = params_of(g, g.b, g.a, kTileP, BN);
+    // double the CTAs of a tile while they fit the SMs and each keeps two stages
+    while (p.split < 8 && (int64_t)p.n_tiles * p.split * 2 <= sm_count && p.n_stages >= 4 * p.split) p.split *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(p.split > 1 ? p.n_tiles * p.split : p.n_tiles < sm_count ? p.n_tiles : sm_count));
     cfg.blockDim = dim3(C::threads);
     cfg.dynamicSmemBytes = C::smem;
     cfg.stream = stream;
@@ -445,33 +686,31 @@ int launch_typed(const Fp4GemmArgs& g, int sm_count, cudaStream_t stream) {
     cfg.numAttrs = p.split > 1 ? 2 : 1;
     e = cudaLaunchKernelEx(&cfg, kernel, map_p, map_q, p);
     if (e == cudaSuccess) e = cudaGetLastError();
-    if (e != cudaSuccess) {
-        set_last_error("mxfp4_gemm_kernel launch", (int)e);
-        return MXFP8_ERR_CUDA;
-    }
-    return MXFP8_OK;
+    return e == cudaSuccess ? MXFP8_OK : launch_failed("mxfp4_gemm_narrow_kernel launch", e);
 }
 
-template <int BN, bool SWAP>
+template <int OUT>
 int launch_out(const Fp4GemmArgs& g, int sm_count, cudaStream_t stream) {
-    switch (g.out_dtype) {
-        case MXFP8_F32: return launch_typed<BN, SWAP, MXFP8_F32>(g, sm_count, stream);
-        case MXFP8_BF16: return launch_typed<BN, SWAP, MXFP8_BF16>(g, sm_count, stream);
-        default: return launch_typed<BN, SWAP, MXFP8_FP16>(g, sm_count, stream);
-    }
+    if (g.a.rows <= 16) return launch_narrow<16, OUT>(g, sm_count, stream);
+    if (g.a.rows <= 32) return launch_narrow<32, OUT>(g, sm_count, stream);
+    if (g.a.rows <= 64) return launch_narrow<64, OUT>(g, sm_count, stream);
+    const int es = OUT == MXFP8_F32 ? 4 : 2;
+    const bool vec = ((reinterpret_cast<uintptr_t>(g.out) | (uint64_t)(g.ld_out * es)) & 31) == 0;
+    const int64_t wide_tiles = ((g.a.rows + 255) / 256) * ((g.b.rows + 255) / 256);
+    if (vec && wide_tiles >= sm_count / 4) return launch_wide<OUT>(g, sm_count, stream);
+    return launch_narrow<128, OUT>(g, sm_count, stream);
 }
 
 }  // namespace
 
 int launch_mxfp4_gemm(const Fp4GemmArgs& g, int sm_count, cudaStream_t stream) {
-    if (g.a.rows <= 16) return launch_out<16, true>(g, sm_count, stream);
-    if (g.a.rows <= 32) return launch_out<32, true>(g, sm_count, stream);
-    if (g.a.rows <= 64) return launch_out<64, true>(g, sm_count, stream);
-    const int es = g.out_dtype == MXFP8_F32 ? 4 : 2;
-    const bool vec = ((reinterpret_cast<uintptr_t>(g.out) | (uint64_t)(g.ld_out * es)) & 31) == 0;
-    const int64_t wide_tiles = ((g.a.rows + 127) / 128) * ((g.b.rows + 255) / 256);
-    if (vec && wide_tiles >= sm_count) return launch_out<256, false>(g, sm_count, stream);
-    return launch_out<128, true>(g, sm_count, stream);
+    // tiles are counted in 32 bits
+    if (((g.a.rows + 127) / 128) * ((g.b.rows + 127) / 128) > (1 << 24)) return MXFP8_ERR_SHAPE;
+    switch (g.out_dtype) {
+        case MXFP8_F32: return launch_out<MXFP8_F32>(g, sm_count, stream);
+        case MXFP8_BF16: return launch_out<MXFP8_BF16>(g, sm_count, stream);
+        default: return launch_out<MXFP8_FP16>(g, sm_count, stream);
+    }
 }
 
 }  // namespace mxfp8

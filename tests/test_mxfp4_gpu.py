@@ -219,7 +219,8 @@ def test_gemm(m, n, k, out):
 
 @pytest.mark.parametrize("m,n,k,out", [(4096, 1280, 512, "fp16"), (4096, 1280, 96, "f32"), (2048, 2304, 288, "bf16"),
                                        (4000, 1296, 544, "bf16"), (4095, 1301, 256, "fp16"), (2500, 2500, 1024, "f32"),
-                                       (10000, 520, 320, "bf16")])
+                                       (10000, 520, 320, "bf16"), (2600, 1024, 2080, "bf16"), (2600, 1000, 4096, "f32"),
+                                       (300, 10000, 160, "fp16"), (700, 4096, 2048, "bf16")])
 def test_gemm_many_tiles(m, n, k, out):
     check_gemm(m, n, k, out)
 
