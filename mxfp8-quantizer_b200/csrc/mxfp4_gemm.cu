@@ -89,7 +89,6 @@ struct GemmParams {
     const uint8_t* sp;          // scales of P and Q
     const uint8_t* sq;
     int col_chunks;             // scale chunks along K, the same for both
-    int row_blocks_q;           // 128-row blocks in Q's scale storage
     int rows_p, rows_q;
     int k;
     int n_stages;               // ceil(k / 256)
@@ -102,25 +101,25 @@ struct GemmParams {
 };
 
 // Wait for a barrier's phase, at most kWaitNs, or until another role gave up.
-template <bool CLUSTER = false>
+// Called by whole warps; the answer is the warp's.
 __device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, volatile int* abort, unsigned int* status) {
-    auto done = [&] { return CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity); };
-    if (done()) return true;
-    const uint64_t t0 = global_timer_ns();
+    uint64_t t0 = 0;
     for (uint32_t i = 1;; ++i) {
-        if (done()) return true;
+        if (__all_sync(0xFFFFFFFFu, mbar_try_wait(bar, parity))) return true;
         if ((i & 255u) == 0) {
-            if (*abort) return false;
-            if (global_timer_ns() - t0 > kWaitNs) {
+            const uint64_t now = global_timer_ns();
+            if (t0 == 0) t0 = now;
+            const bool late = now - t0 > kWaitNs;
+            if (late && !*abort) {
                 if (status) atomicOr(status, kErrGemmWait);
                 *abort = 1;
-                return false;
             }
+            if (__any_sync(0xFFFFFFFFu, *abort != 0)) return false;
         }
     }
 }
 
-// The load thread's end: wait until the last use of every stage is over, so that
+// The load warp's end: wait until the last use of every stage is over, so that
 // nothing arrives on its barriers later.  After an abort nobody may release
 // the stages: then the copies themselves are waited for, as they still target this CTA.
 template <int STAGES>
@@ -129,7 +128,7 @@ __device__ __forceinline__ void drain_stages(uint32_t full0, uint32_t empty0, in
     for (int i = max(0, issued - STAGES); i < issued; ++i) {
         const int s = i % STAGES;
         const uint32_t parity = (i / STAGES) & 1;
-        if (ctl[0] || !wait_phase(empty0 + 8 * s, parity, ctl, status)) mbar_wait_bounded(full0 + 8 * s, parity, kWaitNs);
+        if (!wait_phase(empty0 + 8 * s, parity, ctl, status)) mbar_wait_bounded(full0 + 8 * s, parity, kWaitNs);
     }
 }
 
@@ -142,6 +141,20 @@ __device__ __forceinline__ void tile_of(const GemmParams& p, int t, int& tp, int
     const int wide = min(16, p.tiles_p - group * 16);
     tq = in / wide;
     tp = group * 16 + in - tq * wide;
+}
+
+// The MMAs of one stage, K = 64 each; sfp and sfq hold the scales of its (at
+// most two) chunks, `q_cols` columns of tensor memory a chunk of Q's.
+template <int GROUP, int N>
+__device__ __forceinline__ void issue_stage(uint32_t d, uint32_t rows_p, uint32_t rows_q, uint32_t sfp, uint32_t sfq,
+                                            int q_cols, int steps, bool accumulate) {
+    const uint64_t a = desc_sw128(rows_p), b = desc_sw128(rows_q);
+#pragma unroll
+    for (int j = 0; j < kStageK / kStepK; ++j) {
+        if (j < steps)
+            mma_mxf4<GROUP>(d, a + 2 * j, b + 2 * j, mxf4_idesc(GROUP * kTileP, N, 2 * (j & 1)), sfp + 4 * (j >> 1),
+                            sfq + q_cols * (j >> 1), accumulate || j > 0);
+    }
 }
 
 template <int OUT>
@@ -256,68 +269,67 @@ __global__ void __launch_bounds__(Narrow<BN>::threads, 1)
     int issued = 0;  // stages loaded by the load thread
 
     if (warp == kLoadWarp) {
-        if (lane == 0) {
-            bool ok = true;
-            for (int t = first_tile; ok && t < p.n_tiles; t += tile_step) {
-                int tp, tq;
-                tile_of(p, t, tp, tq);
-                for (int ks = ks0; ks < ks1; ++ks, ++issued) {
-                    const int s = issued % C::stages;
-                    if (issued >= C::stages &&
-                        !wait_phase(empty0 + 8 * s, ((issued / C::stages) - 1) & 1, ctl, p.status)) {
-                        ok = false;
-                        break;
-                    }
+        bool ok = true;
+        for (int t = first_tile; ok && t < p.n_tiles; t += tile_step) {
+            int tp, tq;
+            tile_of(p, t, tp, tq);
+            for (int ks = ks0; ks < ks1; ++ks, ++issued) {
+                const int s = issued % C::stages;
+                if (issued >= C::stages &&
+                    !wait_phase(empty0 + 8 * s, ((issued / C::stages) - 1) & 1, ctl, p.status)) {
+                    ok = false;
+                    break;
+                }
+                if (elect_one()) {
                     const uint32_t dst = base + s * C::stage_bytes, bar = full0 + 8 * s;
-                    const int chunks = min(2, p.col_chunks - 2 * ks);
-                    mbar_arrive_expect_tx(bar, kPBytes + C::q_bytes + 2 * chunks * kChunk);
+                    const uint32_t scales = min(2, p.col_chunks - 2 * ks) * kChunk;
+                    mbar_arrive_expect_tx(bar, kPBytes + C::q_bytes + 2 * scales);
                     tma_load_2d(dst, &map_p, ks * (kStageK / 2), tp * kTileP, bar);
                     tma_load_2d(dst + kPBytes, &map_q, ks * (kStageK / 2), tq * BN, bar);
-                    bulk_load(dst + C::sp_off, p.sp + ((int64_t)tp * p.col_chunks + 2 * ks) * kChunk, chunks * kChunk,
-                              bar);
-                    bulk_load(dst + C::sq_off, p.sq + ((int64_t)tq * p.col_chunks + 2 * ks) * kChunk, chunks * kChunk,
-                              bar);
+                    bulk_load(dst + C::sp_off, p.sp + ((int64_t)tp * p.col_chunks + 2 * ks) * kChunk, scales, bar);
+                    bulk_load(dst + C::sq_off, p.sq + ((int64_t)tq * p.col_chunks + 2 * ks) * kChunk, scales, bar);
                 }
+                __syncwarp();
             }
         }
     } else if (warp == kMmaWarp) {
-        if (lane == 0) {
-            int it = 0, a = 0;
-            bool ok = true;
-            for (int t = first_tile; ok && t < p.n_tiles; t += tile_step, ++a) {
-                const int slot = a % C::acc;
-                if (a >= C::acc && !wait_phase(acc_empty0 + 8 * slot, ((a / C::acc) - 1) & 1, ctl, p.status)) break;
+        int it = 0, a = 0;
+        bool ok = true;
+        for (int t = first_tile; ok && t < p.n_tiles; t += tile_step, ++a) {
+            const int slot = a % C::acc;
+            if (a >= C::acc && !wait_phase(acc_empty0 + 8 * slot, ((a / C::acc) - 1) & 1, ctl, p.status)) break;
+            tcgen05_fence_after();
+            for (int ks = ks0; ks < ks1; ++ks, ++it) {
+                const int s = it % C::stages;
+                if (!wait_phase(full0 + 8 * s, (it / C::stages) & 1, ctl, p.status)) {
+                    ok = false;
+                    break;
+                }
                 tcgen05_fence_after();
-                const uint32_t d = tmem + slot * BN;
-                for (int ks = ks0; ks < ks1; ++ks, ++it) {
-                    const int s = it % C::stages;
-                    if (!wait_phase(full0 + 8 * s, (it / C::stages) & 1, ctl, p.status)) {
-                        ok = false;
-                        break;
-                    }
-                    tcgen05_fence_after();
+                if (elect_one()) {
                     const uint32_t src = base + s * C::stage_bytes;
                     const uint32_t sfp = tmem_sf + (it & 1) * C::sf_cols, sfq = sfp + 8;
                     const int chunks = min(2, p.col_chunks - 2 * ks);
-                    for (int c = 0; c < chunks; ++c) {
-                        tmem_copy_scales<1>(sfp + 4 * c, desc_scale_chunk(src + C::sp_off + c * kChunk));
-                        tmem_copy_scales<1>(sfq + 4 * c, desc_scale_chunk(src + C::sq_off + c * kChunk));
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        if (c < chunks) {
+                            tmem_copy_scales<1>(sfp + 4 * c, desc_scale_chunk(src + C::sp_off + c * kChunk));
+                            tmem_copy_scales<1>(sfq + 4 * c, desc_scale_chunk(src + C::sq_off + c * kChunk));
+                        }
                     }
-                    const int steps = min(kStageK / kStepK, (p.k - ks * kStageK + kStepK - 1) / kStepK);
-                    for (int j = 0; j < steps; ++j) {
-                        const int c = j >> 1, sf = 2 * (j & 1);
-                        mma_mxf4<1>(d, desc_sw128(src + 32 * j), desc_sw128(src + kPBytes + 32 * j),
-                                    mxf4_idesc(kTileP, BN, sf), sfp + 4 * c, sfq + 4 * c, ks > ks0 || j > 0);
-                    }
+                    issue_stage<1, BN>(tmem + slot * BN, src, src + kPBytes, sfp, sfq, 4,
+                                       (p.k - ks * kStageK + kStepK - 1) / kStepK, ks > ks0);
                     tcgen05_commit<1>(empty0 + 8 * s);
+                    if (ks + 1 == ks1) tcgen05_commit<1>(acc_full0 + 8 * slot);
                 }
-                if (ok) tcgen05_commit<1>(acc_full0 + 8 * slot);
+                __syncwarp();
             }
-            // an abort leaves MMAs in flight: let them end before the tensor memory goes
-            if (ctl[0]) {
-                tcgen05_commit<1>(acc_full0);
-                mbar_wait_bounded(acc_full0, 0, kWaitNs);
-            }
+        }
+        // an abort leaves MMAs in flight: let them end before the tensor memory goes
+        if (ctl[0]) {
+            if (elect_one()) tcgen05_commit<1>(acc_full0);
+            __syncwarp();
+            mbar_wait_bounded(acc_full0, 0, kWaitNs);
         }
     } else {
         const int q4 = warp & 3;
@@ -325,8 +337,7 @@ __global__ void __launch_bounds__(Narrow<BN>::threads, 1)
         int a = 0;
         for (int t = first_tile; t < p.n_tiles; t += tile_step, ++a) {
             const int slot = a % C::acc;
-            const bool ok = __all_sync(0xFFFFFFFFu, wait_phase(acc_full0 + 8 * slot, (a / C::acc) & 1, ctl, p.status));
-            if (!ok) break;
+            if (!wait_phase(acc_full0 + 8 * slot, (a / C::acc) & 1, ctl, p.status)) break;
             tcgen05_fence_after();
             int tp, tq;
             tile_of(p, t, tp, tq);
@@ -357,7 +368,7 @@ __global__ void __launch_bounds__(Narrow<BN>::threads, 1)
             }
         }
     }
-    if (warp == kLoadWarp && lane == 0) drain_stages<C::stages>(full0, empty0, issued, ctl, p.status);
+    if (warp == kLoadWarp) drain_stages<C::stages>(full0, empty0, issued, ctl, p.status);
     __syncwarp();
     if (p.split > 1) {  // one tile a cluster: add the parts up, each CTA its share of the columns
         cluster_sync();
@@ -400,12 +411,13 @@ __global__ void __launch_bounds__(Narrow<BN>::threads, 1)
 }
 
 
-// The wide form: a cluster pair a tile.  The odd CTA loads its share and reads
-// its half of the rows back; its MMA thread only tells the even one, which
-// issues for both, when a stage of its own has landed.
+// The wide form: a cluster pair a tile.  Each CTA loads its share, all of it
+// signalled on the even CTA's barriers; that one issues for both, and each
+// reads its half of the rows back.
 template <int OUT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide::threads, 1)
     mxfp4_gemm_wide_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
+                           const __grid_constant__ CUtensorMap map_sp, const __grid_constant__ CUtensorMap map_sq,
                            const GemmParams p) {
     using C = Wide;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -420,7 +432,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide::threads, 1)
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::stages; ++i) {
-            mbar_init(full0 + 8 * i, rank == 0 ? 2 : 1);  // the even CTA's: its own stage and the odd CTA's
+            mbar_init(full0 + 8 * i, 1);                  // used in the even CTA: both CTAs' copies
             mbar_init(empty0 + 8 * i, 1);
         }
         mbar_init(acc_full, 1);
@@ -432,6 +444,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide::threads, 1)
     if (warp == kLoadWarp && lane == 0) {
         prefetch_tensormap(&map_p);
         prefetch_tensormap(&map_q);
+        prefetch_tensormap(&map_sp);
+        prefetch_tensormap(&map_sq);
     }
     tcgen05_fence_before();
     __syncthreads();
@@ -443,91 +457,71 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide::threads, 1)
     grid_wait_prerequisites();
 
     const int first_tile = blockIdx.x >> 1, tile_step = gridDim.x >> 1;
-    int issued = 0;  // stages loaded by the load thread
+    int issued = 0;  // stages loaded by the load warp
 
     if (warp == kLoadWarp) {
-        if (lane == 0) {
-            bool ok = true;
-            for (int t = first_tile; ok && t < p.n_tiles; t += tile_step) {
-                int tp, tq;
-                tile_of(p, t, tp, tq);
-                const int row_block = 2 * tp + rank;
-                // the last pair's odd CTA may have no rows: its payload is zeros, its scales any bytes
-                const bool has_rows = row_block * kTileP < p.rows_p;
-                const int nrbq = min(2, p.row_blocks_q - 2 * tq);
-                for (int ks = 0; ks < p.n_stages; ++ks, ++issued) {
-                    const int s = issued % C::stages;
-                    if (issued >= C::stages &&
-                        !wait_phase(empty0 + 8 * s, ((issued / C::stages) - 1) & 1, ctl, p.status)) {
-                        ok = false;
-                        break;
-                    }
-                    const uint32_t dst = base + s * C::stage_bytes, bar = full0 + 8 * s;
-                    const int chunks = min(2, p.col_chunks - 2 * ks);
-                    mbar_arrive_expect_tx(bar, kPBytes + C::q_bytes + ((has_rows ? 1 : 0) + nrbq) * chunks * kChunk);
-                    tma_load_2d(dst, &map_p, ks * (kStageK / 2), row_block * kTileP, bar);
-                    tma_load_2d(dst + kPBytes, &map_q, ks * (kStageK / 2), tq * C::bn + rank * (C::bn / 2), bar);
-                    if (has_rows)
-                        bulk_load(dst + C::sp_off, p.sp + ((int64_t)row_block * p.col_chunks + 2 * ks) * kChunk,
-                                  chunks * kChunk, bar);
-                    for (int r = 0; r < nrbq; ++r)
-                        bulk_load(dst + C::sq_off + r * 2 * kChunk,
-                                  p.sq + ((int64_t)(2 * tq + r) * p.col_chunks + 2 * ks) * kChunk, chunks * kChunk, bar);
+        const uint32_t even_full0 = cluster_map(full0, 0);
+        bool ok = true;
+        for (int t = first_tile; ok && t < p.n_tiles; t += tile_step) {
+            int tp, tq;
+            tile_of(p, t, tp, tq);
+            for (int ks = 0; ks < p.n_stages; ++ks, ++issued) {
+                const int s = issued % C::stages;
+                if (issued >= C::stages &&
+                    !wait_phase(empty0 + 8 * s, ((issued / C::stages) - 1) & 1, ctl, p.status)) {
+                    ok = false;
+                    break;
                 }
+                if (elect_one()) {
+                    const uint32_t dst = base + s * C::stage_bytes, bar = even_full0 + 8 * s;
+                    // whole boxes count, zero-filled where the matrices end
+                    if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, 2 * C::stage_bytes);
+                    tma_load_2d_pair(dst, &map_p, ks * (kStageK / 2), (2 * tp + rank) * kTileP, bar);
+                    tma_load_2d_pair(dst + kPBytes, &map_q, ks * (kStageK / 2), tq * C::bn + rank * (C::bn / 2), bar);
+                    tma_load_2d_pair(dst + C::sp_off, &map_sp, ks * 2 * (kChunk / 4), 2 * tp + rank, bar);
+                    tma_load_2d_pair(dst + C::sq_off, &map_sq, ks * 2 * (kChunk / 4), 2 * tq, bar);
+                }
+                __syncwarp();
             }
         }
     } else if (warp == kMmaWarp) {
-        if (lane == 0 && rank == 1) {
-            const uint32_t peer_full0 = cluster_map(full0, 0);
-            int it = 0;
-            bool ok = true;
-            for (int t = first_tile; ok && t < p.n_tiles; t += tile_step)
-                for (int ks = 0; ks < p.n_stages; ++ks, ++it) {
-                    const int s = it % C::stages;
-                    if (!wait_phase(full0 + 8 * s, (it / C::stages) & 1, ctl, p.status)) {
-                        ok = false;
-                        break;
-                    }
-                    cluster_arrive(peer_full0 + 8 * s);
+        int it = 0, a = 0;
+        bool ok = rank == 0;
+        for (int t = first_tile; ok && t < p.n_tiles; t += tile_step, ++a) {
+            if (a > 0 && !wait_phase(acc_empty, (a - 1) & 1, ctl, p.status)) break;
+            tcgen05_fence_after();
+            for (int ks = 0; ks < p.n_stages; ++ks, ++it) {
+                const int s = it % C::stages;
+                if (!wait_phase(full0 + 8 * s, (it / C::stages) & 1, ctl, p.status)) {
+                    ok = false;
+                    break;
                 }
-        } else if (lane == 0) {
-            int it = 0, a = 0;
-            bool ok = true;
-            for (int t = first_tile; ok && t < p.n_tiles; t += tile_step, ++a) {
-                if (a > 0 && !wait_phase<true>(acc_empty, (a - 1) & 1, ctl, p.status)) break;
                 tcgen05_fence_after();
-                for (int ks = 0; ks < p.n_stages; ++ks, ++it) {
-                    const int s = it % C::stages;
-                    if (!wait_phase<true>(full0 + 8 * s, (it / C::stages) & 1, ctl, p.status)) {
-                        ok = false;
-                        break;
-                    }
-                    tcgen05_fence_after();
+                if (elect_one()) {
                     const uint32_t src = base + s * C::stage_bytes;
                     const uint32_t sfp = tmem_sf + (it & 1) * C::sf_cols, sfq = sfp + 8;
                     const int chunks = min(2, p.col_chunks - 2 * ks);
-                    for (int c = 0; c < chunks; ++c) {
-                        tmem_copy_scales<2>(sfp + 4 * c, desc_scale_chunk(src + C::sp_off + c * kChunk));
 #pragma unroll
-                        for (int r = 0; r < 2; ++r)
-                            tmem_copy_scales<2>(sfq + 8 * c + 4 * r,
-                                                desc_scale_chunk(src + C::sq_off + (2 * r + c) * kChunk));
+                    for (int c = 0; c < 2; ++c) {
+                        if (c < chunks) {
+                            tmem_copy_scales<2>(sfp + 4 * c, desc_scale_chunk(src + C::sp_off + c * kChunk));
+                            tmem_copy_scales<2>(sfq + 8 * c, desc_scale_chunk(src + C::sq_off + c * kChunk));
+                            tmem_copy_scales<2>(sfq + 8 * c + 4, desc_scale_chunk(src + C::sq_off + (2 + c) * kChunk));
+                        }
                     }
-                    const int steps = min(kStageK / kStepK, (p.k - ks * kStageK + kStepK - 1) / kStepK);
-                    for (int j = 0; j < steps; ++j) {
-                        const int c = j >> 1, sf = 2 * (j & 1);
-                        mma_mxf4<2>(tmem, desc_sw128(src + 32 * j), desc_sw128(src + kPBytes + 32 * j),
-                                    mxf4_idesc(2 * kTileP, C::bn, sf), sfp + 4 * c, sfq + 8 * c, ks > 0 || j > 0);
-                    }
+                    issue_stage<2, C::bn>(tmem, src, src + kPBytes, sfp, sfq, 8,
+                                          (p.k - ks * kStageK + kStepK - 1) / kStepK, ks > 0);
                     tcgen05_commit<2>(empty0 + 8 * s);
+                    if (ks + 1 == p.n_stages) tcgen05_commit<2>(acc_full);
                 }
-                if (ok) tcgen05_commit<2>(acc_full);
+                __syncwarp();
             }
-            // an abort leaves MMAs in flight: let them end before the tensor memory goes
-            if (ctl[0]) {
-                tcgen05_commit<2>(acc_full);
-                mbar_wait_bounded(acc_full, 0, kWaitNs);
-            }
+        }
+        // an abort leaves MMAs in flight: let them end before the tensor memory goes
+        if (rank == 0 && ctl[0]) {
+            if (elect_one()) tcgen05_commit<2>(acc_full);
+            __syncwarp();
+            mbar_wait_bounded(acc_full, 0, kWaitNs);
         }
     } else {
         // two warps for each quarter of the lanes, 128 columns each
@@ -538,7 +532,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide::threads, 1)
         const bool vec = ((reinterpret_cast<uintptr_t>(p.out) | (uint64_t)(p.ld_out * kEs)) & 31) == 0;
         int a = 0;
         for (int t = first_tile; t < p.n_tiles; t += tile_step, ++a) {
-            if (!__all_sync(0xFFFFFFFFu, wait_phase(acc_full, a & 1, ctl, p.status))) break;
+            if (!wait_phase(acc_full, a & 1, ctl, p.status)) break;
             tcgen05_fence_after();
             int tp, tq;
             tile_of(p, t, tp, tq);
@@ -560,7 +554,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide::threads, 1)
             }
         }
     }
-    if (warp == kLoadWarp && lane == 0) drain_stages<C::stages>(full0, empty0, issued, ctl, p.status);
+    if (warp == kLoadWarp) drain_stages<C::stages>(full0, empty0, issued, ctl, p.status);
     __syncwarp();
     tcgen05_fence_before();
     __syncthreads();
@@ -569,26 +563,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide::threads, 1)
     if (warp == kMmaWarp) tmem_dealloc<2>(tmem, C::tmem_cols);
 }
 
-// Tensor map of a payload: bytes (rows, cols / 2), boxes of 128 bytes by
-// `box_rows`, 128-byte swizzle, zeros outside.
-int encode_payload(CUtensorMap* map, const void* q, int64_t rows, int64_t bytes, int64_t ld, int box_rows) {
+// A 2-D tensor map with zeros outside.
+int encode_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, uint64_t cols, uint64_t rows,
+               uint64_t stride_bytes, uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
     auto encode = get_encode_fn();
     if (!encode) {
         set_last_error("cuTensorMapEncodeTiled entry point unavailable", 0);
         return MXFP8_ERR_TENSOR_MAP;
     }
-    cuuint64_t dims[2] = {(cuuint64_t)bytes, (cuuint64_t)rows};
-    cuuint64_t strides[1] = {(cuuint64_t)ld};
-    cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+    cuuint64_t dims[2] = {cols, rows};
+    cuuint64_t strides[1] = {stride_bytes};
+    cuuint32_t box[2] = {box_cols, box_rows};
     cuuint32_t step[2] = {1, 1};
-    CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(q), dims, strides, box, step,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    CUresult r = encode(map, type, 2, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
         set_last_error("cuTensorMapEncodeTiled failed", (int)r);
         return MXFP8_ERR_TENSOR_MAP;
     }
     return MXFP8_OK;
+}
+
+// A payload: boxes of 128 bytes (256 elements of K) by box_rows, 128-byte swizzle.
+int encode_payload(CUtensorMap* map, const Fp4Operand& m, int64_t k, int box_rows) {
+    return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, m.q, (uint64_t)(k / 2), (uint64_t)m.rows, (uint64_t)m.ld, 128,
+                      (uint32_t)box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// Its scales: a row of words per 128-row block, boxes of two chunks by box_blocks.
+int encode_scales(CUtensorMap* map, const Fp4Operand& m, int64_t k, int box_blocks) {
+    const uint64_t words = (uint64_t)((k + 127) / 128) * (kChunk / 4);
+    return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, m.s, words, (uint64_t)((m.rows + 127) / 128), words * 4,
+                      2 * (kChunk / 4), (uint32_t)box_blocks, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 // A kernel's shared memory opt-in, once per device: later launches, captured
@@ -615,7 +621,6 @@ GemmParams params_of(const Fp4GemmArgs& g, const Fp4Operand& P, const Fp4Operand
     p.sp = P.s;
     p.sq = Q.s;
     p.col_chunks = (int)((g.k + 127) / 128);
-    p.row_blocks_q = (int)((Q.rows + 127) / 128);
     p.rows_p = (int)P.rows;
     p.rows_q = (int)Q.rows;
     p.k = (int)g.k;
@@ -637,9 +642,11 @@ int launch_wide(const Fp4GemmArgs& g, int sm_count, cudaStream_t stream) {
     auto kernel = mxfp4_gemm_wide_kernel<OUT>;
     cudaError_t e = opt_in(kernel, C::smem, done);
     if (e != cudaSuccess) return launch_failed("cudaFuncSetAttribute", e);
-    CUtensorMap map_p, map_q;
-    if (int rc = encode_payload(&map_p, g.a.q, g.a.rows, g.k / 2, g.a.ld, kTileP)) return rc;
-    if (int rc = encode_payload(&map_q, g.b.q, g.b.rows, g.k / 2, g.b.ld, C::bn / 2)) return rc;
+    CUtensorMap map_p, map_q, map_sp, map_sq;
+    if (int rc = encode_payload(&map_p, g.a, g.k, kTileP)) return rc;
+    if (int rc = encode_payload(&map_q, g.b, g.k, C::bn / 2)) return rc;
+    if (int rc = encode_scales(&map_sp, g.a, g.k, 1)) return rc;
+    if (int rc = encode_scales(&map_sq, g.b, g.k, 2)) return rc;
     const GemmParams p = params_of(g, g.a, g.b, 2 * kTileP, C::bn);
     cudaLaunchConfig_t cfg = {};
     const int pairs = sm_count / 2;
@@ -652,7 +659,7 @@ int launch_wide(const Fp4GemmArgs& g, int sm_count, cudaStream_t stream) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kernel, map_p, map_q, p);
+    e = cudaLaunchKernelEx(&cfg, kernel, map_p, map_q, map_sp, map_sq, p);
     if (e == cudaSuccess) e = cudaGetLastError();
     return e == cudaSuccess ? MXFP8_OK : launch_failed("mxfp4_gemm_wide_kernel launch", e);
 }
@@ -665,8 +672,8 @@ int launch_narrow(const Fp4GemmArgs& g, int sm_count, cudaStream_t stream) {
     cudaError_t e = opt_in(kernel, C::smem, done);
     if (e != cudaSuccess) return launch_failed("cudaFuncSetAttribute", e);
     CUtensorMap map_p, map_q;
-    if (int rc = encode_payload(&map_p, g.b.q, g.b.rows, g.k / 2, g.b.ld, kTileP)) return rc;
-    if (int rc = encode_payload(&map_q, g.a.q, g.a.rows, g.k / 2, g.a.ld, BN)) return rc;
+    if (int rc = encode_payload(&map_p, g.b, g.k, kTileP)) return rc;
+    if (int rc = encode_payload(&map_q, g.a, g.k, BN)) return rc;
     GemmParams p = params_of(g, g.b, g.a, kTileP, BN);
     // double the CTAs of a tile while they fit the SMs and each keeps two stages
     while (p.split < 8 && (int64_t)p.n_tiles * p.split * 2 <= sm_count && p.n_stages >= 4 * p.split) p.split *= 2;

@@ -158,20 +158,35 @@ __device__ __forceinline__ float4 cluster_load_f32x4(uint32_t addr) {
     return v;
 }
 // Arrive on a barrier of another CTA of the cluster (a cluster_map address).
+// For handing tensor memory over (after tcgen05_fence_before), not memory: a
+// release at cluster scope took 1100 cycles.
 __device__ __forceinline__ void cluster_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// mbar_try_wait that also sees what CTAs of the cluster wrote before arriving.
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
+
+// One lane of a converged warp, always the same.  The warp walks its loop as
+// one and only issues under this: a loop that a single lane walks keeps its
+// addresses and descriptors out of the uniform registers that TMA and tcgen05
+// instructions read, which took 925 cycles a stage to issue.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "elect.sync _|p, 0xFFFFFFFF;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
+        : "=r"(one));
+    return one != 0;
+}
+
+// 2-D TMA tile load of a CTA pair: into this CTA's shared memory, completion
+// signalled on `bar` of either CTA (a shared::cluster address).
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y,
+                                                 uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2"
+        " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
         : "memory");
-    return ok != 0;
 }
 
 }  // namespace mxfp8
