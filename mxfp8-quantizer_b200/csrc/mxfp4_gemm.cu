@@ -664,6 +664,14 @@ int launch_wide(const Fp4GemmArgs& g, int sm_count, cudaStream_t stream) {
     return e == cudaSuccess ? MXFP8_OK : launch_failed("mxfp4_gemm_wide_kernel launch", e);
 }
 
+// CTAs of a narrow tile's cluster: doubled while they fit the SMs and each
+// keeps two stages.
+int narrow_split(int64_t tiles, int n_stages, int sm_count) {
+    int split = 1;
+    while (split < 8 && tiles * split * 2 <= sm_count && n_stages >= 4 * split) split *= 2;
+    return split;
+}
+
 template <int BN, int OUT>
 int launch_narrow(const Fp4GemmArgs& g, int sm_count, cudaStream_t stream) {
     using C = Narrow<BN>;
@@ -675,8 +683,7 @@ int launch_narrow(const Fp4GemmArgs& g, int sm_count, cudaStream_t stream) {
     if (int rc = encode_payload(&map_p, g.b, g.k, kTileP)) return rc;
     if (int rc = encode_payload(&map_q, g.a, g.k, BN)) return rc;
     GemmParams p = params_of(g, g.b, g.a, kTileP, BN);
-    // double the CTAs of a tile while they fit the SMs and each keeps two stages
-    while (p.split < 8 && (int64_t)p.n_tiles * p.split * 2 <= sm_count && p.n_stages >= 4 * p.split) p.split *= 2;
+    p.split = narrow_split(p.n_tiles, p.n_stages, sm_count);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(p.split > 1 ? p.n_tiles * p.split : p.n_tiles < sm_count ? p.n_tiles : sm_count));
     cfg.blockDim = dim3(C::threads);
@@ -701,10 +708,21 @@ int launch_out(const Fp4GemmArgs& g, int sm_count, cudaStream_t stream) {
     if (g.a.rows <= 16) return launch_narrow<16, OUT>(g, sm_count, stream);
     if (g.a.rows <= 32) return launch_narrow<32, OUT>(g, sm_count, stream);
     if (g.a.rows <= 64) return launch_narrow<64, OUT>(g, sm_count, stream);
+    // More than 64 rows: both forms take a time that grows with the stages a CTA
+    // walks one after another, about 5.1 + 0.32 us a stage (wide) and 7.2 + 0.36
+    // (narrow).  Measured, us wide / narrow: 512x2048x2048 7.7 / 8.3,
+    // 384x4096x4096 10.4 / 12.7, 256x8192x8192 16.7 / 18.8; with K long and
+    // split the narrow one wins: 256x4096x4096 10.2 / 9.7, 512x1024x8192 15.3 / 10.0.
+    // The wide form's stores want rows of C on 32 bytes.
     const int es = OUT == MXFP8_F32 ? 4 : 2;
     const bool vec = ((reinterpret_cast<uintptr_t>(g.out) | (uint64_t)(g.ld_out * es)) & 31) == 0;
+    const int64_t stages = (g.k + kStageK - 1) / kStageK;
+    const int64_t narrow_tiles = ((g.a.rows + 127) / 128) * ((g.b.rows + 127) / 128);
     const int64_t wide_tiles = ((g.a.rows + 255) / 256) * ((g.b.rows + 255) / 256);
-    if (vec && wide_tiles >= sm_count / 4) return launch_wide<OUT>(g, sm_count, stream);
+    const int split = narrow_split(narrow_tiles, (int)stages, sm_count);
+    const int64_t narrow_row = (stages + split - 1) / split * ((narrow_tiles * split + sm_count - 1) / sm_count);
+    const int64_t wide_row = stages * ((wide_tiles + sm_count / 2 - 1) / (sm_count / 2));
+    if (vec && wide_row <= narrow_row + 6) return launch_wide<OUT>(g, sm_count, stream);
     return launch_narrow<128, OUT>(g, sm_count, stream);
 }
 
