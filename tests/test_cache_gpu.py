@@ -547,7 +547,7 @@ def test_checked_build():
     pkg.cache_write(cache, x, x, slots)
     want = pkg.cache_attention(q, cache, table, lens)
     rows = pkg.cache_read(cache, table, starts, 550)
-    d = pkg.kv_cache._describe(copy)
+    d = capi.Cache(*(t.data_ptr() for t in copy), pages, heads, page, dim)
     out, k_out, v_out = torch.zeros_like(want), torch.zeros_like(rows[0]), torch.zeros_like(rows[1])
     size = capi.cache_attention_workspace(d, 3, 8)
     ws = torch.empty(size, dtype=torch.uint8, device="cuda")

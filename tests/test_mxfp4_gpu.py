@@ -19,6 +19,7 @@ pytestmark = pytest.mark.gpu
 pkg = MXFP8_quantizer.load_package()
 capi = pkg._capi
 TORCH = {"bf16": torch.bfloat16, "fp16": torch.float16, "f32": torch.float32}
+CODES = {"bf16": capi.BF16, "fp16": capi.FP16, "f32": capi.F32}
 
 
 def on_gpu(bits, dtype, ld=None, offset=0):
@@ -124,7 +125,7 @@ def test_dequantize_unaligned_output_rows(out):
     buf = torch.full((37 * 101 + 8,), -7.0, dtype=TORCH[out], device="cuda")
     view = buf[3:3 + 37 * 101].view(37, 101)
     capi.fp4_dequantize(q.data_ptr(), 37, 96, 48, s.data_ptr(), s.numel(), view.data_ptr(),
-                        pkg._launch.OUT_DTYPES[TORCH[out]], 101, torch.cuda.current_stream().cuda_stream)
+                        CODES[out], 101, torch.cuda.current_stream().cuda_stream)
     assert torch.equal(view[:, :96].cpu(), round_once(v, out))
     assert (view[:, 96:] == -7).all() and (buf[:3] == -7).all() and (buf[3 + 37 * 101:] == -7).all()
 
