@@ -31,7 +31,7 @@ struct CacheWriteArgs {
     const uint16_t* k;
     const uint16_t* v;
     int64_t k_token, k_head, v_token, v_head;  // strides in elements
-    bool k_vec, v_vec;                         // every row starts on a 16-byte boundary
+    bool k_vec, v_vec;                         // every row starts on a 32-byte boundary
     int64_t tokens;
     const int64_t* slots;
     uint8_t *k_out, *v_out, *k_scales, *v_scales;
@@ -46,6 +46,7 @@ struct CacheReadArgs {
     int64_t table_stride, max_pages, batch;
     const int32_t* starts;
     int64_t total;
+    uint32_t cta_rows;  // set by the launch
     uint8_t *k_out, *v_out;
     StoreWindow kw, vw;
     unsigned int* status;

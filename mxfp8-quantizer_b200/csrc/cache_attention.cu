@@ -1002,7 +1002,7 @@ int launch_typed(const CacheAttentionArgs& a, int sm_count, cudaStream_t stream)
     }
     if (e == cudaSuccess) {
         // Many heads are in few pieces each and want few CTAs, few heads in many: one warp or four a head.  64 ragged
-        // sequences, 2048 heads: 54.2 us in all with one, 56.7 with four; 8 long ones, 128 heads: 75 and 72.
+        // sequences, 2048 heads: 54.2 us in all with one, 56.7 with four; 8 long ones, 128 heads: 80.3 and 72.3.
         const int64_t units = a.batch * a.q_heads;
         const bool single = units >= 8 * (int64_t)sm_count;
         cfg.gridDim = dim3((unsigned)(single ? (units + kJoinWarps - 1) / kJoinWarps : units));

@@ -38,16 +38,12 @@ MXFP8_HD int64_t table_page(const int32_t* table, int64_t stride, int64_t max_pa
 
 // The sequence that covers output row `row`: the last b with starts[b] <=
 // row; batch if the row lies past the last sequence, -1 before the first.
-MXFP8_HD int64_t sequence_of(const int32_t* starts, int64_t batch, int64_t row) {
-    if (row < starts[0]) return -1;
-    if (row >= starts[batch]) return batch;
-    int64_t lo = 0, hi = batch;  // starts[lo] <= row < starts[hi]
-    while (hi - lo > 1) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (starts[mid] <= row) lo = mid;
-        else hi = mid;
-    }
-    return lo;
+// `from` is a number of that kind for a row at or before this one: the count of
+// starts that are <= that row, less one.
+MXFP8_HD int64_t sequence_from(const int32_t* starts, int64_t batch, int64_t from, int64_t row) {
+    int64_t b = from;
+    while (b < batch && starts[b + 1] <= row) ++b;
+    return b;
 }
 
 // `total` units over n parts, the first total % n parts one unit longer: part i

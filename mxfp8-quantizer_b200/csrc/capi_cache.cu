@@ -45,8 +45,8 @@ int check_table(const int32_t* table, int64_t stride, int64_t max_pages) {
 
 inline int64_t positions(const CacheShape& c) { return (c.num_pages * c.heads) << c.page_shift; }
 
-// Whether rows of these strides from p all start on 16 bytes.
-inline bool rows_aligned(const void* p, int64_t a, int64_t b) { return aligned(p, 16) && a % 8 == 0 && b % 8 == 0; }
+// Whether rows of these strides from p all start on 32 bytes.
+inline bool rows_aligned(const void* p, int64_t a, int64_t b) { return aligned(p, 32) && a % 16 == 0 && b % 16 == 0; }
 
 int attention_shape(const CacheShape& c, int64_t batch, int64_t q_heads) {
     if (batch < 0 || q_heads < 1 || q_heads > 65536 || q_heads % c.heads != 0 || batch > kInt32Max / q_heads ||

@@ -26,7 +26,7 @@ def probe(tmp_path_factory):
     lib = ctypes.CDLL(str(out))
     i64, i32, vp = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p
     for name, args in (("probe_row", [i64, i32, i32, i64, i32, i32]), ("probe_table", [vp, i64, i64, i64, i64, i32]),
-                       ("probe_sequence", [vp, i64, i64]), ("probe_begin", [i64] * 3), ("probe_part", [i64] * 3),
+                       ("probe_sequence", [vp, i64, i64, i64]), ("probe_begin", [i64] * 3), ("probe_part", [i64] * 3),
                        ("probe_visible", [i64, i64, i32])):
         getattr(lib, name).argtypes, getattr(lib, name).restype = args, i64
     return lib
@@ -60,8 +60,8 @@ def test_positions_past_the_table_have_no_page(probe):
 def test_sequence_of_every_row(probe, starts):
     a = np.array(starts, np.int32)
     batch = len(starts) - 1
-    for row in range(-1, starts[-1] + 3):
-        got = probe.probe_sequence(a.ctypes.data, batch, row)
+    for first, row in ((f, r) for r in range(-1, starts[-1] + 3) for f in range(max(-1, r - 4), r + 1)):
+        got = probe.probe_sequence(a.ctypes.data, batch, first, row)
         if row < starts[0]:
             assert got == -1
         elif row >= starts[-1]:
@@ -71,12 +71,12 @@ def test_sequence_of_every_row(probe, starts):
 
 
 def test_sequence_of_falling_starts_stays_in_range(probe):
-    """starts that fall break the contract; the answer still names a sequence."""
+    """starts that fall break the contract; the answer still names a sequence, or none."""
     rng = np.random.default_rng(0)
     for _ in range(200):
         a = rng.integers(-5, 20, rng.integers(2, 9)).astype(np.int32)
         for row in range(-3, 22):
-            assert -1 <= probe.probe_sequence(a.ctypes.data, len(a) - 1, row) <= len(a) - 1
+            assert -1 <= probe.probe_sequence(a.ctypes.data, len(a) - 1, row - 2, row) <= len(a) - 1
 
 
 @pytest.mark.parametrize("n,total", [(1, 1), (1, 9), (3, 3), (3, 10), (7, 8), (444, 445), (444, 100000),
