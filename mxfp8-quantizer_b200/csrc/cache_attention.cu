@@ -48,6 +48,7 @@ constexpr int kThreads = 32 * kWarps;
 constexpr int kJoinWarps = 4;
 constexpr int kJoinThreads = 32 * kJoinWarps;
 constexpr int kSegmentCost = 2;
+constexpr int kMinRef = 20;  // a weight times 2^(142 - R), and a tile's sum of them, stay below 2^127
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr uint32_t kNoRow32 = 0xFFFFFFFFu;
@@ -107,6 +108,7 @@ struct Cursor {
     int64_t base, end, b;
     const int32_t* pages;
     int g, t, t0, t1, nt, len;
+    uint32_t head;  // KV head of g
     bool done;
 };
 
@@ -117,6 +119,11 @@ __device__ __forceinline__ bool enter(Cursor& c, int64_t begin) {
     c.t1 = c.end - first < c.nt ? (int)(c.end - first) : c.nt;
     c.t = c.t0;
     return c.t0 < c.t1;
+}
+
+__device__ __forceinline__ void set_group(const Params& p, Cursor& c, int g) {
+    c.g = g;
+    c.head = (uint32_t)(p.row_groups == 1 ? g : g / p.row_groups);
 }
 
 template <int POS>
@@ -135,8 +142,10 @@ __device__ __forceinline__ void next_segment(const Params& p, Cursor& c, int gro
             c.done = true;
             return;
         }
-        if (++c.g == groups) {
-            c.g = 0;
+        if (c.g + 1 < groups) {
+            set_group(p, c, c.g + 1);
+        } else {
+            set_group(p, c, 0);
             do {  // total cost is not exhausted: there is another sequence with tiles
                 ++c.b;
                 enter_sequence<POS>(p, c, length_of(p.a, c.b));
@@ -192,6 +201,15 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// The same with nothing in d before.
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     const __half2 t = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&t);
@@ -239,9 +257,47 @@ template <int POS>
 __device__ __forceinline__ uint32_t row_of_lane(const Params& p, const Cursor& c, int page, int lane) {
     const int at = c.t * POS + lane;
     if (lane >= POS || at >= c.len) return kNoRow32;
-    const int64_t row = cache_row(p.a.c, page, c.g / p.row_groups, at & ((1 << p.a.c.page_shift) - 1));
-    if (row == kNoRow && p.a.status) atomicOr(p.a.status, kErrCacheIndex);
-    return row == kNoRow ? kNoRow32 : (uint32_t)row;
+    if ((uint32_t)page >= (uint32_t)p.a.c.num_pages) {
+        if (p.a.status) atomicOr(p.a.status, kErrCacheIndex);
+        return kNoRow32;
+    }
+    // cache_row in 32 bits: a cache has fewer rows
+    return ((((uint32_t)page * (uint32_t)p.a.c.heads + c.head) << p.a.c.page_shift) |
+            ((uint32_t)at & ((1u << p.a.c.page_shift) - 1u)));
+}
+
+// Fetch the rows of a whole tile whose pages hold 16 positions or more: each 16
+// of them are one run of memory.
+template <int D, int POS>
+__device__ __forceinline__ void fetch_runs(const Params& p, uint32_t stage, uint32_t my_row, int lane) {
+    constexpr int kChunks = D / 16, kRows = 32 / kChunks, kKv = POS * D;
+    const int j0 = lane / kChunks, ch = lane % kChunks;
+    const uint32_t k_at = stage + group_at<D>(j0, ch >> 1) + (ch & 1) * 16;
+    const uint32_t v_at = stage + kKv + group_at<D>(v_place(j0), ch >> 1) + (ch & 1) * 16;
+#pragma unroll
+    for (int run = 0; run < POS / 16; ++run) {
+        const uint64_t off = (uint64_t)__shfl_sync(0xFFFFFFFFu, my_row, run * 16) * D + lane * 16;
+        const uint8_t* k = p.a.k + off;
+        const uint8_t* v = p.a.v + off;
+#pragma unroll
+        for (int i = run * 16 / kRows; i < (run + 1) * 16 / kRows; ++i) {
+            const int from = (i - run * 16 / kRows) * 512;
+            cp_async16(i * kRows * D + (k_at ^ (key_of<D>(i * kRows) << 5)), k + from, true);
+            cp_async16(v_place(i * kRows) * D + (v_at ^ (key_of<D>(v_place(i * kRows)) << 5)), v + from, true);
+        }
+    }
+    // a run's scale bytes: 16 * D / 32 of them, 4 a lane
+    constexpr int kWords = D / 8;
+#pragma unroll
+    for (int i = 0; i < (POS / 16 * kWords + 31) / 32; ++i) {
+        const int idx = i * 32 + lane, run = idx / kWords, in = idx - run * kWords;
+        const uint32_t row = __shfl_sync(0xFFFFFFFFu, my_row, (run * 16) & (POS - 1));
+        if (POS / 16 * kWords % 32 == 0 || idx < POS / 16 * kWords) {
+            const uint64_t off = (uint64_t)row * (D / 32) + in * 4;
+            cp_async4(stage + 2 * kKv + idx * 4, p.a.k_scales + off, true);
+            cp_async4(stage + 2 * kKv + POS * D / 32 + idx * 4, p.a.v_scales + off, true);
+        }
+    }
 }
 
 // Fetch those rows into a stage: payloads 16 bytes a lane, scales four bytes a
@@ -302,7 +358,7 @@ __device__ __forceinline__ void fetch(const Params& p, uint32_t stage, uint32_t 
 template <int D, int NT>
 __device__ __forceinline__ void load_query(const Params& p, const Cursor& c, int lane, uint32_t (&qf)[D / 16][2 * NT],
                                            float (&mul)[NT]) {
-    const int sub = c.g % p.row_groups, kv_head = c.g / p.row_groups;
+    const int kv_head = (int)c.head, sub = c.g - kv_head * p.row_groups;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         const int in = sub * Config<D, NT>::rows + n * 8 + (lane >> 2);
@@ -337,8 +393,13 @@ __device__ __forceinline__ void load_query(const Params& p, const Cursor& c, int
         amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 2));
         // exponent of the largest element; subnormal and infinite ones are held at the ends of the range
         const int e = min(max((int)(__float_as_uint(amax) >> 23), 15), 254) - 127;
-        const float down = __uint_as_float((uint32_t)(127 + 14 - e) << 23);  // 2^(14 - e)
-        mul[n] = amax == 0.0f ? 0.0f : p.a.scale * kLog2e * __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+        // 2^(14 - e), with the sign of the scale; a product of 0 is kept as a query of 0, so that mul is above 0
+        float down = copysignf(__uint_as_float((uint32_t)(127 + 14 - e) << 23), p.a.scale);
+        mul[n] = fabsf(p.a.scale) * kLog2e * __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+        if (mul[n] == 0.0f || amax == 0.0f) {
+            mul[n] = 1.0f;
+            down = 0.0f;
+        }
 #pragma unroll
         for (int blk = 0; blk < D / 32; ++blk)
 #pragma unroll
@@ -455,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
         cur.end = split_begin(split, part + 1);
         cur.b = found_b[warp];
         enter_sequence<POS>(p, cur, found_len[warp]);
-        cur.g = (int)((begin - found_base[warp]) / (cur.nt + kSegmentCost));
+        set_group(p, cur, (int)((begin - found_base[warp]) / (cur.nt + kSegmentCost)));
         cur.base = found_base[warp] + (int64_t)cur.g * (cur.nt + kSegmentCost);
         if (!enter(cur, begin)) next_segment<POS>(p, cur, groups);
     }
@@ -474,7 +535,14 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
         if (!next.done) {
             const uint32_t my_row = row_of_lane<POS>(p, next, my_page, lane);
             const uint32_t mask = __ballot_sync(0xFFFFFFFFu, my_row != kNoRow32);
-            if (mask != 0) fetch<D, POS>(p, ring_u + stage * C::stage_bytes, my_row, lane);
+            if constexpr (D != 192) {
+                if (mask == kFull && p.a.c.page_shift >= 4)
+                    fetch_runs<D, POS>(p, ring_u + stage * C::stage_bytes, my_row, lane);
+                else if (mask != 0)
+                    fetch<D, POS>(p, ring_u + stage * C::stage_bytes, my_row, lane);
+            } else {
+                if (mask != 0) fetch<D, POS>(p, ring_u + stage * C::stage_bytes, my_row, lane);
+            }
             if (lane == stage) present = mask;
             advance<POS>(p, next, groups);
             my_page = page_of_lane<POS>(p, next, lane);
@@ -487,14 +555,14 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
     uint32_t qf[D / 16][2 * NT];
     float mul[NT], m[NT], l[NT];
     float acc[NT][D / 16][4];
-    int ref = 15;  // R: the largest V scale byte so far, and at least 15
+    int ref = kMinRef;  // R: the largest V scale byte so far, and at least this
     bool fresh = true;
 
     int stage = 0;
     while (!cur.done) {
         if (fresh) {
             load_query<D, NT>(p, cur, lane, qf, mul);
-            ref = 15;
+            ref = kMinRef;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 m[n] = -INFINITY;
@@ -518,8 +586,6 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
             float s[kCols][2 * NT];
 #pragma unroll
             for (int nt = 0; nt < kCols; ++nt) {
-#pragma unroll
-                for (int j = 0; j < 2 * NT; ++j) s[nt][j] = 0.0f;
                 uint32_t w[kWords], f[kBlocks];  // f: bf16 factors, blocks in pairs, both positions
                 load_scale_pair<kBlocks>(ks + nt * 8 * kBlocks, w);
 #pragma unroll
@@ -530,12 +596,12 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
                     uint32_t b0, b1, b2, b3;
                     e4m3x4_to_half2(b.x, b0, b1);
                     e4m3x4_to_half2(b.y, b2, b3);
-                    float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    float d[4];
                     if constexpr (NT == 1) {
-                        mma_f16(d, qf[2 * blk][0], 0u, qf[2 * blk][1], 0u, b0, b1);
+                        mma_f16_first(d, qf[2 * blk][0], 0u, qf[2 * blk][1], 0u, b0, b1);
                         mma_f16(d, qf[2 * blk + 1][0], 0u, qf[2 * blk + 1][1], 0u, b2, b3);
                     } else {
-                        mma_f16(d, qf[2 * blk][0], qf[2 * blk][2], qf[2 * blk][1], qf[2 * blk][3], b0, b1);
+                        mma_f16_first(d, qf[2 * blk][0], qf[2 * blk][2], qf[2 * blk][1], qf[2 * blk][3], b0, b1);
                         mma_f16(d, qf[2 * blk + 1][0], qf[2 * blk + 1][2], qf[2 * blk + 1][1], qf[2 * blk + 1][3], b2,
                                 b3);
                     }
@@ -544,18 +610,11 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
                     const float fy = __uint_as_float(blk & 1 ? f1 & 0xFFFF0000u : f1 << 16);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        s[nt][2 * n] = fmaf(d[2 * n], fx, s[nt][2 * n]);
-                        s[nt][2 * n + 1] = fmaf(d[2 * n + 1], fy, s[nt][2 * n + 1]);
+                        s[nt][2 * n] = blk == 0 ? d[2 * n] * fx : fmaf(d[2 * n], fx, s[nt][2 * n]);
+                        s[nt][2 * n + 1] = blk == 0 ? d[2 * n + 1] * fy : fmaf(d[2 * n + 1], fy, s[nt][2 * n + 1]);
                     }
                 }
             }
-#pragma unroll
-            for (int nt = 0; nt < kCols; ++nt)
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    s[nt][2 * n] *= mul[n];
-                    s[nt][2 * n + 1] *= mul[n];
-                }
             if (mask != kFull) {
 #pragma unroll
                 for (int nt = 0; nt < kCols; ++nt)
@@ -563,33 +622,9 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
                     for (int j = 0; j < 2 * NT; ++j)
                         if (!((mask >> (nt * 8 + 2 * quad + (j & 1))) & 1)) s[nt][j] = -INFINITY;
             }
-            // ---- softmax, in log2 ----
-            float corr[NT];
-            bool moved = false;
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                float top = -INFINITY;
-#pragma unroll
-                for (int nt = 0; nt < kCols; ++nt) top = fmaxf(top, fmaxf(s[nt][2 * n], s[nt][2 * n + 1]));
-                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-                const float m_new = fmaxf(m[n], top);
-                corr[n] = m_new > m[n] ? exp2_fast(m[n] - m_new) : 1.0f;
-                moved |= m_new > m[n];
-                m[n] = m_new;
-                l[n] *= corr[n];
-#pragma unroll
-                for (int nt = 0; nt < kCols; ++nt)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        float& v = s[nt][2 * n + j];
-                        v = exp2_fast(v - m_new);
-                        l[n] += v;
-                    }
-            }
             // ---- V's scale bytes and the largest of them ----
             uint32_t vw[kCols][kWords];
-            uint32_t most = 0;
+            uint32_t odd = 0, even = 0;  // in the upper byte of each half
 #pragma unroll
             for (int nt = 0; nt < kCols; ++nt) {
                 load_scale_pair<kBlocks>(vs + nt * 8 * kBlocks, vw[nt]);
@@ -604,26 +639,56 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
                     for (int i = 0; i < kWords; ++i) vw[nt][i] = h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
                 }
 #pragma unroll
-                for (int i = 0; i < kWords; ++i) most = __vmaxu4(most, vw[nt][i]);
+                for (int i = 0; i < kWords; ++i) {
+                    odd = __vmaxu2(odd, vw[nt][i]);
+                    even = __vmaxu2(even, vw[nt][i] << 8);
+                }
             }
-            if (__any_sync(0xFFFFFFFFu, __vcmpeq4(most, 0xFFFFFFFFu) != 0)) {
-                // NaN scales reach the result as they are; R is the largest of the others
+            odd = __vmaxu2(odd, even);
+            int most = (int)max(odd >> 24, (odd >> 8) & 0xFFu);
+            most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
+            most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
+            if (most == 255) {  // NaN scales reach the result as they are; R is the largest of the others
                 most = 0;
 #pragma unroll
                 for (int nt = 0; nt < kCols; ++nt)
 #pragma unroll
-                    for (int i = 0; i < kWords; ++i)
-                        most = __vmaxu4(most, vw[nt][i] & ~__vcmpeq4(vw[nt][i], 0xFFFFFFFFu));
+                    for (int i = 0; i < 4 * kWords; ++i) {
+                        const int byte = (int)((vw[nt][i / 4] >> (8 * (i & 3))) & 0xFFu);
+                        most = max(most, byte == 255 ? 0 : byte);
+                    }
+                most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
+                most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
             }
-            most = __vmaxu4(most, most >> 16);
-            most = max(most & 0xFFu, (most >> 8) & 0xFFu);
-            most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
-            most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
-            float down = 1.0f;
-            if ((int)most > ref) {  // acc is in units of 2^(ref - 142)
-                down = exp2_fast((float)(ref - (int)most));
-                ref = (int)most;
-                moved = true;
+            const bool grown = most > ref;  // acc is in units of 2^(ref - 142)
+            const float down = grown ? exp2_fast((float)(ref - most)) : 1.0f;
+            ref = max(ref, most);
+            // ---- softmax, in log2; the weights come out times 2^(142 - ref) ----
+            const float down_l = __uint_as_float((uint32_t)(ref - 142 + 127) << 23);
+            float corr[NT];
+            bool moved = grown;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int nt = 0; nt < kCols; ++nt) top = fmaxf(top, fmaxf(s[nt][2 * n], s[nt][2 * n + 1]));
+                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+                const float m_new = fmaxf(m[n], top * mul[n]);
+                corr[n] = m_new > m[n] ? exp2_fast(m[n] - m_new) : 1.0f;
+                moved |= m_new > m[n];
+                m[n] = m_new;
+                const float shift = (float)(142 - ref) - m_new;
+                float sum = 0.0f;
+#pragma unroll
+                for (int nt = 0; nt < kCols; ++nt)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        float& v = s[nt][2 * n + j];
+                        v = exp2_fast(fmaf(v, mul[n], shift));
+                        sum += v;
+                    }
+                l[n] = fmaf(l[n], corr[n], sum * down_l);
             }
             if (__any_sync(0xFFFFFFFFu, moved)) {
 #pragma unroll
@@ -640,11 +705,6 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
                 }
             }
             // ---- second product: rows are elements of V, columns heads ----
-            const float up = __uint_as_float((uint32_t)(142 - ref + 127) << 23);  // 2^(142 - ref)
-#pragma unroll
-            for (int nt = 0; nt < kCols; ++nt)
-#pragma unroll
-                for (int j = 0; j < 2 * NT; ++j) s[nt][j] *= up;
             const uint8_t* vsm = st + C::kv_bytes;
 #pragma unroll
             for (int half = 0; half < POS / 16; ++half) {
@@ -691,8 +751,8 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
         if (cur.t + 1 == cur.t1) {  // the warp's last tile of this segment
             const bool begins = cur.t0 == 0, ends = cur.t1 == cur.nt;
             const int64_t seg = cur.b * groups + cur.g;
-            const int sub = cur.g % p.row_groups;
-            const int64_t head0 = cur.b * p.a.q_heads + (int64_t)(cur.g / p.row_groups) * p.group + sub * C::rows;
+            const int sub = cur.g - (int)cur.head * p.row_groups;
+            const int64_t head0 = cur.b * p.a.q_heads + (int64_t)cur.head * p.group + sub * C::rows;
             const int rows = min(C::rows, p.group - sub * C::rows);
             if (begins && lane == 0) {
                 const int64_t last = split_part(split, cur.base + kSegmentCost + cur.nt - 1);
@@ -743,7 +803,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
     // ---- warps of this CTA that end inside the same segment: one piece of theirs ----
     cp_async_wait<0>();
     const bool open = !cur.done;
-    const int sub = cur.g % p.row_groups, rows = min(C::rows, p.group - sub * C::rows);
+    const int sub = cur.g - (int)cur.head * p.row_groups, rows = min(C::rows, p.group - sub * C::rows);
     const int64_t open_seg = cur.b * groups + cur.g, open_slot = 2 * part + (cur.t0 == 0 ? 1 : 0);
     if (lane == 0) ends_in[warp] = open ? open_seg : -1;
     __syncthreads();
