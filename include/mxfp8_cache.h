@@ -72,7 +72,7 @@ MXFP8_API int64_t mxfp8_cache_attention_workspace(const mxfp8_cache* cache, int6
  * elements, last dimension contiguous; out contiguous of the same type and
  * lse (batch, q_heads) f32 or NULL: log of the sum of exp(scale * q . k_j).
  * dim is 64, 128, 192 or 256, page_size at least 2, q_heads a multiple of
- * heads.  A length of 0 (or below) gives zeros and lse -inf; a position whose page is
+ * heads, max_pages * page_size < 2^31 - 1024, and batch times that at most 2^34.  A length of 0 (or below) gives zeros and lse -inf; a position whose page is
  * outside the cache takes no part, as if it were not there, and is reported; a
  * length past the table is cut to it and reported.  Scores, sums and outputs
  * are held in f32 and rounded once.  workspace is 16-byte aligned scratch of

@@ -353,11 +353,9 @@ __device__ __forceinline__ void fetch(const Params& p, uint32_t stage, uint32_t 
     }
 }
 
-// Query rows of a head group as MMA operands, and what a score is multiplied
-// by: scale * log2(e) * the power of two taken out of the row.
+// This lane's elements of the cursor's query rows, as they are in memory.
 template <int D, int NT>
-__device__ __forceinline__ void load_query(const Params& p, const Cursor& c, int lane, uint32_t (&qf)[D / 16][2 * NT],
-                                           float (&mul)[NT]) {
+__device__ __forceinline__ void load_query(const Params& p, const Cursor& c, int lane, uint32_t (&raw)[NT][D / 8]) {
     const int kv_head = (int)c.head, sub = c.g - kv_head * p.row_groups;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -365,19 +363,31 @@ __device__ __forceinline__ void load_query(const Params& p, const Cursor& c, int
         const bool on = in < p.group;
         const uint16_t* src = p.a.q + c.b * p.a.q_batch + (int64_t)(kv_head * p.group + (on ? in : 0)) * p.a.q_head;
         const bool vec = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
-        uint32_t w[D / 32][4];
 #pragma unroll
         for (int blk = 0; blk < D / 32; ++blk) {
             const uint4 t = load8(src + blk * 32 + (lane & 3) * 8, vec);
-            w[blk][0] = t.x; w[blk][1] = t.y; w[blk][2] = t.z; w[blk][3] = t.w;
+            raw[n][4 * blk] = on ? t.x : 0u;
+            raw[n][4 * blk + 1] = on ? t.y : 0u;
+            raw[n][4 * blk + 2] = on ? t.z : 0u;
+            raw[n][4 * blk + 3] = on ? t.w : 0u;
         }
+    }
+}
+
+// The rows as MMA operands, and what a score is multiplied by: |scale| *
+// log2(e) * the power of two taken out of the row.
+template <int D, int NT>
+__device__ __forceinline__ void settle_query(const Params& p, const uint32_t (&raw)[NT][D / 8],
+                                             uint32_t (&qf)[D / 16][2 * NT], float (&mul)[NT]) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
         float v[D / 32][8];
         float amax = 0.0f;
 #pragma unroll
         for (int blk = 0; blk < D / 32; ++blk) {
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
-                const uint32_t pair = on ? w[blk][e / 2] : 0u;
+                const uint32_t pair = raw[n][4 * blk + e / 2];
                 if (p.a.q_bf16) {
                     v[blk][e] = __uint_as_float(pair << 16);
                     v[blk][e + 1] = __uint_as_float(pair & 0xFFFF0000u);
@@ -451,73 +461,59 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
     constexpr int kBlocks = D / 32, kWords = kBlocks / 2;
     constexpr uint32_t kFull = POS == 32 ? 0xFFFFFFFFu : (1u << POS) - 1u;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int64_t scan_s[kWarps];
-    __shared__ int64_t found_b[kWarps], found_base[kWarps];
-    __shared__ int found_len[kWarps];
     __shared__ int64_t ends_in[kWarps], lead_slot[kWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = lane >> 2, quad = lane & 3;
     const int groups = p.a.c.heads * p.row_groups;
 
     grid_launch_dependents();  // the second launch may take its place: it waits for this one's end
     grid_wait_prerequisites();
-    // ---- the warps' shares of all costs, and the sequences where they begin ----
-    const int64_t per = (p.a.batch + kThreads - 1) / kThreads;
-    const int64_t b0 = min(p.a.batch, per * threadIdx.x), b1 = min(p.a.batch, b0 + per);
-    int64_t mine = 0;
+    // ---- the warps' shares of all costs, and where this one's begins: every warp for itself ----
+    // a lane has the costs of neighbouring sequences; their sum fits 32 bits (the entry checks it)
+    const int64_t per = (p.a.batch + 31) / 32;
+    const int64_t b0 = min(p.a.batch, per * lane), b1 = min(p.a.batch, b0 + per);
+    uint32_t mine = 0;
+    int len = 0;  // of the last of them: all there is to know while a lane has one
     for (int64_t b = b0; b < b1; ++b) {
-        mine += cost_of<POS>(length_of(p.a, b));
-        if (blockIdx.x == 0 && p.a.status && (int64_t)p.a.lengths[b] > (p.a.max_pages << p.a.c.page_shift))
+        len = length_of(p.a, b);
+        mine += cost_of<POS>(len);
+        if (blockIdx.x == 0 && warp == 0 && p.a.status &&
+            (int64_t)p.a.lengths[b] > (p.a.max_pages << p.a.c.page_shift))
             atomicOr(p.a.status, kErrCacheIndex);
     }
-    int64_t upto = mine;
+    uint32_t upto = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const int64_t o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+        const uint32_t o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
         if (lane >= d) upto += o;
     }
-    if (lane == 31) scan_s[warp] = upto;
-    __syncthreads();
-    int64_t before = 0, cost = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) before += scan_s[w];
-        cost += scan_s[w];
-    }
-    const int64_t total = cost * groups;
+    const int64_t total = (int64_t)__shfl_sync(0xFFFFFFFFu, upto, 31) * groups;
     const int64_t parts = min(p.parts, total);
     const int64_t first_part = (int64_t)blockIdx.x * kWarps;
     if (first_part >= parts) return;
     const Split split = make_split(parts, total);
-    const int64_t from = (before + upto - mine) * groups;  // place of this thread's first sequence
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        const int64_t x = split_begin(split, first_part + w);
-        if (first_part + w < parts && from <= x && x < from + mine * groups) {
-            int64_t at = from;
-            int64_t b = b0;
-            int len;
-            for (;; ++b) {
-                len = length_of(p.a, b);
-                const int64_t n = (int64_t)cost_of<POS>(len) * groups;
-                if (x < at + n) break;
-                at += n;
-            }
-            found_b[w] = b;
-            found_base[w] = at;
-            found_len[w] = len;
-        }
-    }
-    __syncthreads();
     const int64_t part = first_part + warp;
     Cursor cur{};  // the tile that is computed
     cur.done = part >= parts;  // a warp without a share is there for the barriers
     if (!cur.done) {
         const int64_t begin = split_begin(split, part);
         cur.end = split_begin(split, part + 1);
-        cur.b = found_b[warp];
-        enter_sequence<POS>(p, cur, found_len[warp]);
-        set_group(p, cur, (int)((begin - found_base[warp]) / (cur.nt + kSegmentCost)));
-        cur.base = found_base[warp] + (int64_t)cur.g * (cur.nt + kSegmentCost);
+        // the lane whose sequences hold the first unit, and the one of them
+        const int at_lane = __ffs(__ballot_sync(0xFFFFFFFFu, begin < (int64_t)upto * groups)) - 1;
+        cur.b = __shfl_sync(0xFFFFFFFFu, b0, at_lane);
+        cur.base = (int64_t)(__shfl_sync(0xFFFFFFFFu, upto - mine, at_lane)) * groups;
+        cur.len = __shfl_sync(0xFFFFFFFFu, len, at_lane);
+        if (per > 1) {
+            for (;; ++cur.b) {
+                cur.len = length_of(p.a, cur.b);
+                const int64_t n = (int64_t)cost_of<POS>(cur.len) * groups;
+                if (begin < cur.base + n) break;
+                cur.base += n;
+            }
+        }
+        enter_sequence<POS>(p, cur, cur.len);
+        const int g = groups == 1 ? 0 : (int)((begin - cur.base) / (cur.nt + kSegmentCost));
+        set_group(p, cur, g);
+        cur.base += (int64_t)g * (cur.nt + kSegmentCost);
         if (!enter(cur, begin)) next_segment<POS>(p, cur, groups);
     }
 
@@ -530,6 +526,8 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
     // ---- fetch ahead: `next` is the tile whose pages are being looked up ----
     Cursor next = cur;
     int my_page = page_of_lane<POS>(p, next, lane);
+    uint32_t first_query[NT][D / 8] = {};
+    if (!cur.done) load_query<D, NT>(p, cur, lane, first_query);  // on its way while the pages are
     uint32_t present = 0;  // lane s: which positions of stage s are there
     auto issue = [&](int stage) {
         if (!next.done) {
@@ -556,24 +554,23 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
     float mul[NT], m[NT], l[NT];
     float acc[NT][D / 16][4];
     int ref = kMinRef;  // R: the largest V scale byte so far, and at least this
-    bool fresh = true;
+    auto start_segment = [&](const uint32_t (&raw)[NT][D / 8]) {
+        settle_query<D, NT>(p, raw, qf, mul);
+        ref = kMinRef;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            m[n] = -INFINITY;
+            l[n] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[n][i][j] = 0.0f;
+        }
+    };
+    start_segment(first_query);
 
     int stage = 0;
     while (!cur.done) {
-        if (fresh) {
-            load_query<D, NT>(p, cur, lane, qf, mul);
-            ref = kMinRef;
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                m[n] = -INFINITY;
-                l[n] = 0.0f;
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[n][i][j] = 0.0f;
-            }
-            fresh = false;
-        }
         cp_async_wait<C::stages - 2>();
         __syncwarp();  // also: the stage before this one is read, it can be filled again
         const uint32_t mask = __shfl_sync(0xFFFFFFFFu, present, stage);
@@ -795,9 +792,15 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
             } else {  // the rest of a segment that began before: slot 0
                 put_piece<D, NT>(p, 2 * part, rows, lane, m, l, acc);
             }
-            fresh = true;
+            advance<POS>(p, cur, groups);
+            if (!cur.done) {
+                uint32_t raw[NT][D / 8];
+                load_query<D, NT>(p, cur, lane, raw);
+                start_segment(raw);
+            }
+        } else {
+            ++cur.t;
         }
-        advance<POS>(p, cur, groups);
     }
 
     // ---- warps of this CTA that end inside the same segment: one piece of theirs ----
@@ -878,7 +881,8 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attention_join_kernel(cons
     constexpr int kUnits = kJoinWarps / W;
     __shared__ float tops[kJoinWarps], totals[kJoinWarps];
     __shared__ float weights_of[kUnits][kPass];
-    __shared__ uint32_t present_of[kUnits][kPass / 32];  // pieces with something in them
+    __shared__ uint32_t present_of[kUnits][kPass / 32];  // which pieces have something in them
+    __shared__ uint16_t list_of[kUnits][kPass];
     __shared__ float2 sums[W > 1 ? W : 1][W > 1 ? D / 2 : 1];
     grid_launch_dependents();
     grid_wait_prerequisites();
@@ -888,6 +892,7 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attention_join_kernel(cons
     if (unit >= p.a.batch * p.a.q_heads) return;
     float* const weights = weights_of[W == 1 ? warp : 0];
     uint32_t* const present = present_of[W == 1 ? warp : 0];
+    uint16_t* const list = list_of[W == 1 ? warp : 0];
     auto sync = [] {
         if (W == 1) __syncwarp();
         else __syncthreads();
@@ -931,43 +936,43 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attention_join_kernel(cons
             if (lane == 0) present[j * W + mine] = there;
         }
         sync();
-        int turn = 0, n = 0;
-        int pick[4];
-        auto take = [&] {  // the picked pieces, all loads before the first use
-            float2 v[4][kVecs];
+        // pieces with something in them, in order
+        int count = 0;
+        for (int word = 0; word < kPass / 32; ++word) count += __popc(present[word]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (j < n) {
-                    const float* src = p.part_o + slot_of(i0 + pick[j]) * D + 2 * lane;
-#pragma unroll
-                    for (int k = 0; k < kVecs; ++k) v[j][k] = *reinterpret_cast<const float2*>(src + 64 * k);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (j < n) {
-                    const float f = weights[pick[j]];
-#pragma unroll
-                    for (int k = 0; k < kVecs; ++k) {
-                        o[k].x += v[j][k].x * f;
-                        o[k].y += v[j][k].y * f;
-                    }
-                }
-            }
-            n = 0;
-        };
-        for (int word = 0; word < kPass / 32 && i0 + 32 * word < pieces; ++word) {
-            for (uint32_t left = present[word]; left != 0; left &= left - 1) {
-                if ((turn++ & (W - 1)) != mine) continue;
-                const int i = word * 32 + __ffs(left) - 1;
-                if (n == 0) pick[0] = i;
-                else if (n == 1) pick[1] = i;
-                else if (n == 2) pick[2] = i;
-                else pick[3] = i;
-                if (++n == 4) take();
-            }
+        for (int j = 0; j < kEach; ++j) {
+            const int own = j * W + mine;
+            const uint32_t there = present[own];
+            if (!((there >> lane) & 1)) continue;
+            int rank = __popc(there & ((1u << lane) - 1));
+            for (int word = 0; word < own; ++word) rank += __popc(present[word]);
+            list[rank] = (uint16_t)(own * 32 + lane);
         }
-        take();
+        sync();
+        for (int n0 = mine; n0 < count; n0 += 4 * W) {  // four pieces' loads before the first use
+            float2 v[4][kVecs];
+            float f[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bool on = n0 + j * W < count;
+                const int i = list[on ? n0 + j * W : n0];
+                f[j] = on ? weights[i] : 0.0f;
+                const float* src = p.part_o + slot_of(i0 + i) * D + 2 * lane;
+#pragma unroll
+                for (int k = 0; k < kVecs; ++k) v[j][k] = *reinterpret_cast<const float2*>(src + 64 * k);
+                if (!on) {
+#pragma unroll
+                    for (int k = 0; k < kVecs; ++k) v[j][k] = make_float2(0.0f, 0.0f);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int k = 0; k < kVecs; ++k) {
+                    o[k].x += v[j][k].x * f[j];
+                    o[k].y += v[j][k].y * f[j];
+                }
+        }
         sync();
     }
     sum = warp_sum(sum);

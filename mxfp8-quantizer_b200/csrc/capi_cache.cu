@@ -146,7 +146,8 @@ extern "C" MXFP8_API int mxfp8_cache_attention(const mxfp8_cache* cache, const v
     if (int rc = attention_shape(a.c, batch, q_heads)) return rc;
     if (int rc = check_table(table, table_stride, max_pages)) return rc;
     if ((max_pages << a.c.page_shift) > kInt32Max - 1024 || q_batch_stride < 0 || q_batch_stride > kMaxStride ||
-        q_head_stride < 0 || q_head_stride > kMaxStride)
+        q_head_stride < 0 || q_head_stride > kMaxStride ||
+        batch > (int64_t(1) << 34) / ((max_pages << a.c.page_shift) + 1024))
         return MXFP8_ERR_SHAPE;
     if (batch == 0) return MXFP8_OK;
     if (!q || !lengths || !out || !workspace) return MXFP8_ERR_NULL_POINTER;
