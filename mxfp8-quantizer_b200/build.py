@@ -84,7 +84,7 @@ def _native_command(out: pathlib.Path) -> list[str]:
     cmd += ["-I", str(ROOT / "include"), "-o", str(out), str(BINDING)]
     for path in library_paths():
         cmd += ["-L", path]
-    return cmd + ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+    return cmd + ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python"]
 
 
 def build(force: bool = False, verbose_ptxas: bool = False) -> pathlib.Path:

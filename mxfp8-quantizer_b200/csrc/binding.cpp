@@ -11,6 +11,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/utils/pybind.h>
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 
 #include <cmath>
 #include <optional>
@@ -76,6 +77,12 @@ void* enter(c10::cuda::OptionalCUDAGuard& guard, const Tensor& first, const T&..
     return c10::cuda::getCurrentCUDAStream(first.device().index()).stream();
 }
 
+// A new contiguous tensor beside t, from torch's allocator without the way
+// through its dispatcher.
+Tensor new_empty(at::IntArrayRef sizes, at::ScalarType type, const Tensor& t) {
+    return at::detail::empty_cuda(sizes, type, t.device(), std::nullopt);
+}
+
 int in_dtype(const char* name, const Tensor& t) {
     if (t.scalar_type() == at::kBFloat16) return MXFP8_BF16;
     if (t.scalar_type() == at::kHalf) return MXFP8_FP16;
@@ -126,13 +133,12 @@ std::tuple<Tensor, Tensor> quantize_mxfp4(const Tensor& x_in, const OptTensor& q
     c10::cuda::OptionalCUDAGuard guard;
     void* stream = enter(guard, x, q_in, s_in);
     if ((x.stride(1) != 1 && k > 1) || (m > 1 && x.stride(0) < k)) x = x.contiguous();
-    const auto bytes = x.options().dtype(at::kByte);
-    Tensor q = q_in ? *q_in : at::empty({m, q_cols / 2}, bytes);
+    Tensor q = q_in ? *q_in : new_empty({m, q_cols / 2}, at::kByte, x);
     if (q_in) {
         const Payload p = payload("q", q);
         TORCH_CHECK_VALUE(p.rows == m && p.cols == q_cols, "q must be (", m, ", ", q_cols / 2, ") bytes, got ", q.sizes());
     }
-    Tensor s = s_in ? *s_in : at::empty({(m + 127) / 128 * 128 * ((q_cols + 127) / 128 * 4)}, bytes);
+    Tensor s = s_in ? *s_in : new_empty({(m + 127) / 128 * 128 * ((q_cols + 127) / 128 * 4)}, at::kByte, x);
     if (s_in) check_scales("s", s);
     const int64_t ld_x = row_stride(x), ld_q = row_stride(q), s_bytes = s.numel();
     call("MXFP4 quantizer launch", [&] {
@@ -147,7 +153,7 @@ Tensor dequantize_mxfp4(const Tensor& q, const Tensor& s, at::ScalarType type) {
     const int code = out_dtype(type);
     c10::cuda::OptionalCUDAGuard guard;
     void* stream = enter(guard, q, s);
-    Tensor out = at::empty({p.rows, p.cols}, q.options().dtype(type));
+    Tensor out = new_empty({p.rows, p.cols}, type, q);
     call("MXFP4 dequantizer launch", [&] {
         return api.fp4_dequantize(q.data_ptr(), p.rows, p.cols, p.ld, s.data_ptr(), s.numel(), out.data_ptr(), code,
                                   p.cols, stream);
@@ -170,7 +176,7 @@ Tensor gemm_mxfp4(const Tensor& a_q, const Tensor& b_q, const Tensor& a_s, const
     const int code = out_dtype(type);
     c10::cuda::OptionalCUDAGuard guard;
     void* stream = enter(guard, a_q, b_q, a_s, b_s, out_in);
-    Tensor out = out_in ? *out_in : at::empty({a.rows, b.rows}, a_q.options().dtype(type));
+    Tensor out = out_in ? *out_in : new_empty({a.rows, b.rows}, type, a_q);
     const int64_t ld_out = row_stride(out);
     call("MXFP4 product launch", [&] {
         return api.fp4_gemm(a_q.data_ptr(), a.rows, a.ld, a_s.data_ptr(), a_s.numel(), b_q.data_ptr(), b.rows, b.ld,
@@ -263,9 +269,8 @@ std::tuple<Tensor, Tensor> cache_read(const Tensor& ck, const Tensor& cv, const 
     const int code = out_dtype(type);
     c10::cuda::OptionalCUDAGuard guard;
     void* stream = enter(guard, table, starts, ck, cv, cks, cvs, k_given, v_given);
-    const auto options = table.options().dtype(type);
-    Tensor k = k_given ? *k_given : at::empty({total, c.heads, c.dim}, options);
-    Tensor v = v_given ? *v_given : at::empty({total, c.heads, c.dim}, options);
+    Tensor k = k_given ? *k_given : new_empty({total, c.heads, c.dim}, type, table);
+    Tensor v = v_given ? *v_given : new_empty({total, c.heads, c.dim}, type, table);
     call("cache read launch", [&] {
         return api.cache_read(&c, int32s(table), table_stride(table), table.size(1), batch, int32s(starts), total,
                               k.data_ptr(), v.data_ptr(), code, stream);
@@ -292,16 +297,16 @@ std::tuple<Tensor, OptTensor> cache_attention(const Tensor& q_in, const Tensor& 
     c10::cuda::OptionalCUDAGuard guard;
     void* stream = enter(guard, q_in, table, lengths, ck, cv, cks, cvs);
     const Tensor q = rows(q_in);
-    Tensor out = at::empty({batch, q_heads, (int64_t)c.dim}, q.options());
+    Tensor out = new_empty({batch, q_heads, c.dim}, q.scalar_type(), q);
     OptTensor lse;
-    if (return_lse) lse = at::empty({batch, q_heads}, q.options().dtype(at::kFloat));
+    if (return_lse) lse = new_empty({batch, q_heads}, at::kFloat, q);
     int64_t size = 0;
     call("cache attention workspace", [&] {
         size = api.attention_workspace(&c, batch, q_heads);
         return size < 0 ? (int)size : MXFP8_OK;
     });
     // scratch of this call: its memory may serve others once the stream has passed it
-    Tensor workspace = at::empty({size}, q.options().dtype(at::kByte));
+    Tensor workspace = new_empty({size}, at::kByte, q);
     const float factor = (float)(scale ? *scale : 1.0 / std::sqrt((double)c.dim));
     call("cache attention launch", [&] {
         return api.attention(&c, q.data_ptr(), q.stride(0), q.stride(1), code, batch, q_heads, int32s(table),
