@@ -75,7 +75,8 @@ MXFP8_API int64_t mxfp8_cache_attention_workspace(const mxfp8_cache* cache, int6
  * heads, max_pages * page_size < 2^31 - 1024, and batch times that at most 2^34.  A length of 0 (or below) gives zeros and lse -inf; a position whose page is
  * outside the cache takes no part, as if it were not there, and is reported; a
  * length past the table is cut to it and reported.  Scores, sums and outputs
- * are held in f32 and rounded once.  workspace is 16-byte aligned scratch of
+ * are held in f32 and rounded once; a score overflows where a K block's scale
+ * is 2^96 or more (the query is held with its largest element near 2^14).  workspace is 16-byte aligned scratch of
  * one call at a time; its contents do not matter before or after. */
 MXFP8_API int mxfp8_cache_attention(const mxfp8_cache* cache, const void* q, int64_t q_batch_stride,
                                     int64_t q_head_stride, int dtype, int64_t batch, int64_t q_heads,

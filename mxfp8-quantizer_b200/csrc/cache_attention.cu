@@ -1046,7 +1046,7 @@ int launch_typed(const CacheAttentionArgs& a, int sm_count, cudaStream_t stream)
     // no more warps than the longest lengths that the table allows would use
     const int64_t most = segments * (((a.max_pages << a.c.page_shift) + C::pos - 1) / C::pos + kSegmentCost);
     const int64_t ctas = ctas_of<D, NT>(sm_count), slots = 2 * kWarps * ctas * C::rows;
-    const int64_t grid = a.max_pages == 0 ? 0 : most < ctas * kWarps ? (most + kWarps - 1) / kWarps : ctas;
+    const int64_t grid = most < ctas * kWarps ? (most + kWarps - 1) / kWarps : ctas;
     p.parts = grid * kWarps;
     p.part_o = static_cast<float*>(a.workspace);
     p.part_ml = reinterpret_cast<float2*>(p.part_o + slots * D);
@@ -1059,12 +1059,10 @@ int launch_typed(const CacheAttentionArgs& a, int sm_count, cudaStream_t stream)
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (grid > 0) {
-        cfg.gridDim = dim3((unsigned)grid);
-        cfg.blockDim = dim3(kThreads);
-        cfg.dynamicSmemBytes = C::smem;
-        e = cudaLaunchKernelEx(&cfg, kernel, p);
-    }
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = C::smem;
+    e = cudaLaunchKernelEx(&cfg, kernel, p);
     if (e == cudaSuccess) {
         // Many heads are in few pieces each and want few CTAs, few heads in many: one warp or four a head.  64 ragged
         // sequences, 2048 heads: 54.2 us in all with one, 56.7 with four; 8 long ones, 128 heads: 80.3 and 72.3.

@@ -296,7 +296,8 @@ def test_attention(heads, group, dim, page, dtype):
 
 @pytest.mark.parametrize("lengths,heads,group,dim", [([20000], 2, 4, 128), ([5000, 1, 0, 9001], 1, 8, 256),
                                                      ([64] * 300, 2, 2, 64), ([0] * 5, 2, 4, 128),
-                                                     ([1] * 700, 1, 4, 64), ([3000] * 40, 4, 8, 128)])
+                                                     ([1] * 700, 1, 4, 64), ([3000] * 40, 4, 8, 128),
+                                                     ([30000] + [3] * 300, 1, 4, 64), ([40000], 1, 1, 64)])
 def test_attention_splits(lengths, heads, group, dim):
     """Few long sequences, many short ones, nothing at all."""
     q, cache, table = attention_case(lengths, 16, heads, group, dim, "bf16", seed=len(lengths))
@@ -412,6 +413,21 @@ def test_attention_bad_pages_take_no_part():
     assert torch.equal(out, want) and (out[1] == 0).all()
 
 
+def test_attention_without_pages():
+    """An empty table and an empty cache: nothing to attend to, and a positive length is reported."""
+    q = torch.randn((3, 4, 64), device="cuda").half()
+    none = torch.empty((3, 0), dtype=torch.int32, device="cuda")
+    zero, some = torch.zeros(3, dtype=torch.int32, device="cuda"), torch.tensor([0, 5, 0], dtype=torch.int32, device="cuda")
+    for cache in (pkg.allocate_cache(0, 16, 2, 64), filled(2, 16, 2, 64)):
+        for lens, expect in ((zero, 0), (some, INDEX_BIT)):
+            out, lse = pkg.cache_attention(q, cache, none, lens, return_lse=True)
+            assert (out == 0).all() and (lse == -math.inf).all()
+            assert capi.device_status(clear=True) == expect
+    table = torch.zeros((3, 1), dtype=torch.int32, device="cuda")
+    out = pkg.cache_attention(q, pkg.allocate_cache(0, 16, 2, 64), table, some)
+    assert (out == 0).all() and capi.device_status(clear=True) == INDEX_BIT
+
+
 def test_attention_lse_joins_two_halves():
     """A context attended to in two parts and joined by their lse equals the whole."""
     q, cache, table = attention_case([160], 16, 2, 4, 128, "bf16")
@@ -436,6 +452,8 @@ def test_streams_graphs_and_repeats():
     side.wait_stream(torch.cuda.current_stream())
     there = [pkg.cache_attention(*s, lens, return_lse=True, stream=side) for s in sets for _ in range(3)]
     rows = [pkg.cache_read(s[1], s[2], starts, 980, stream=side.cuda_stream) for s in sets]
+    default = pkg.cache_attention(*sets[0], lens, stream=torch.cuda.default_stream())
+    assert torch.equal(default, want[0][0])
     here = [pkg.cache_attention(*s, lens, return_lse=True) for s in sets for _ in range(3)]
     torch.cuda.current_stream().wait_stream(side)
     for i in range(6):
