@@ -65,7 +65,11 @@ struct Config {
     static constexpr int sc_bytes = pos * D / 32;
     static constexpr int stage_bytes = 2 * kv_bytes + 2 * sc_bytes;
     static constexpr int stages = D <= 64 ? 3 : 2;
-    static constexpr int warp_bytes = stages * stage_bytes;
+    // Long queries are kept in shared memory: in registers they took what the compiler needs to overlap a tile's
+    // steps (8 sequences of 65536, D = 256: 61.1 us, 69.2 in registers).  16 rows of D = 128 are better off there
+    // (16 sequences of 8192: 20.6 us, 21.4 in shared memory).
+    static constexpr int query_bytes = D > 128 ? D * 16 * NT : 0;
+    static constexpr int warp_bytes = stages * stage_bytes + query_bytes;
     static constexpr int smem = kWarps * warp_bytes;
     static constexpr int ctas_per_sm = 2;
 };
@@ -378,7 +382,7 @@ __device__ __forceinline__ void load_query(const Params& p, const Cursor& c, int
 // log2(e) * the power of two taken out of the row.
 template <int D, int NT>
 __device__ __forceinline__ void settle_query(const Params& p, const uint32_t (&raw)[NT][D / 8],
-                                             uint32_t (&qf)[D / 16][2 * NT], float (&mul)[NT]) {
+                                             uint32_t (&qf)[D / 32][4 * NT], float (&mul)[NT]) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         float v[D / 32][8];
@@ -416,7 +420,7 @@ __device__ __forceinline__ void settle_query(const Params& p, const uint32_t (&r
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int r = 0; r < 2; ++r)
-                    qf[blk * 2 + h][n * 2 + r] =
+                    qf[blk][h * 2 * NT + n * 2 + r] =
                         pack_half2(v[blk][4 * h + 2 * r] * down, v[blk][4 * h + 2 * r + 1] * down);
     }
 }
@@ -550,12 +554,22 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
 #pragma unroll
     for (int s = 0; s < C::stages - 1; ++s) issue(s);
 
-    uint32_t qf[D / 16][2 * NT];
+    uint4* const queries = reinterpret_cast<uint4*>(ring + C::stages * C::stage_bytes);  // where they are kept there
+    uint32_t qf[C::query_bytes > 0 ? 1 : kBlocks][4 * NT];
     float mul[NT], m[NT], l[NT];
     float acc[NT][D / 16][4];
     int ref = kMinRef;  // R: the largest V scale byte so far, and at least this
     auto start_segment = [&](const uint32_t (&raw)[NT][D / 8]) {
-        settle_query<D, NT>(p, raw, qf, mul);
+        if constexpr (C::query_bytes > 0) {
+            uint32_t own[kBlocks][4 * NT];
+            settle_query<D, NT>(p, raw, own, mul);
+#pragma unroll
+            for (int i = 0; i < kBlocks * NT; ++i)  // read back by the lane that wrote them
+                queries[i * 32 + lane] = make_uint4(own[i / NT][4 * (i % NT)], own[i / NT][4 * (i % NT) + 1],
+                                                    own[i / NT][4 * (i % NT) + 2], own[i / NT][4 * (i % NT) + 3]);
+        } else {
+            settle_query<D, NT>(p, raw, qf, mul);
+        }
         ref = kMinRef;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -581,35 +595,56 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
             const uint8_t* vs = ks + C::sc_bytes;
             // ---- scores: rows are heads, columns positions 8 nt + 2 quad + {0, 1} ----
             float s[kCols][2 * NT];
-#pragma unroll
-            for (int nt = 0; nt < kCols; ++nt) {
-                uint32_t w[kWords], f[kBlocks];  // f: bf16 factors, blocks in pairs, both positions
+            auto factors = [&](int nt, uint32_t (&f)[kBlocks]) {  // bf16, blocks in pairs, both positions
+                uint32_t w[kWords];
                 load_scale_pair<kBlocks>(ks + nt * 8 * kBlocks, w);
 #pragma unroll
                 for (int i = 0; i < kWords; ++i) ue8m0x4_to_bf162(w[i], f[2 * i], f[2 * i + 1]);
+            };
+            auto add_block = [&](int nt, int blk, const uint32_t (&q)[4 * NT], const uint32_t (&f)[kBlocks]) {
+                const uint2 b = *reinterpret_cast<const uint2*>(st + in_block<D>(k_at, blk) + nt * 8 * D);
+                uint32_t b0, b1, b2, b3;
+                e4m3x4_to_half2(b.x, b0, b1);
+                e4m3x4_to_half2(b.y, b2, b3);
+                float d[4];
+                if constexpr (NT == 1) {
+                    mma_f16_first(d, q[0], 0u, q[1], 0u, b0, b1);
+                    mma_f16(d, q[2], 0u, q[3], 0u, b2, b3);
+                } else {
+                    mma_f16_first(d, q[0], q[2], q[1], q[3], b0, b1);
+                    mma_f16(d, q[4], q[6], q[5], q[7], b2, b3);
+                }
+                const uint32_t f0 = f[blk / 2], f1 = f[kWords + blk / 2];
+                const float fx = __uint_as_float(blk & 1 ? f0 & 0xFFFF0000u : f0 << 16);
+                const float fy = __uint_as_float(blk & 1 ? f1 & 0xFFFF0000u : f1 << 16);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    s[nt][2 * n] = blk == 0 ? d[2 * n] * fx : fmaf(d[2 * n], fx, s[nt][2 * n]);
+                    s[nt][2 * n + 1] = blk == 0 ? d[2 * n + 1] * fy : fmaf(d[2 * n + 1], fy, s[nt][2 * n + 1]);
+                }
+            };
+            if constexpr (C::query_bytes > 0) {
+                uint32_t f[kCols][kBlocks];
+#pragma unroll
+                for (int nt = 0; nt < kCols; ++nt) factors(nt, f[nt]);
 #pragma unroll
                 for (int blk = 0; blk < kBlocks; ++blk) {
-                    const uint2 b = *reinterpret_cast<const uint2*>(st + in_block<D>(k_at, blk) + nt * 8 * D);
-                    uint32_t b0, b1, b2, b3;
-                    e4m3x4_to_half2(b.x, b0, b1);
-                    e4m3x4_to_half2(b.y, b2, b3);
-                    float d[4];
-                    if constexpr (NT == 1) {
-                        mma_f16_first(d, qf[2 * blk][0], 0u, qf[2 * blk][1], 0u, b0, b1);
-                        mma_f16(d, qf[2 * blk + 1][0], 0u, qf[2 * blk + 1][1], 0u, b2, b3);
-                    } else {
-                        mma_f16_first(d, qf[2 * blk][0], qf[2 * blk][2], qf[2 * blk][1], qf[2 * blk][3], b0, b1);
-                        mma_f16(d, qf[2 * blk + 1][0], qf[2 * blk + 1][2], qf[2 * blk + 1][1], qf[2 * blk + 1][3], b2,
-                                b3);
-                    }
-                    const uint32_t f0 = f[blk / 2], f1 = f[kWords + blk / 2];
-                    const float fx = __uint_as_float(blk & 1 ? f0 & 0xFFFF0000u : f0 << 16);
-                    const float fy = __uint_as_float(blk & 1 ? f1 & 0xFFFF0000u : f1 << 16);
+                    uint32_t q[4 * NT];
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        s[nt][2 * n] = blk == 0 ? d[2 * n] * fx : fmaf(d[2 * n], fx, s[nt][2 * n]);
-                        s[nt][2 * n + 1] = blk == 0 ? d[2 * n + 1] * fy : fmaf(d[2 * n + 1], fy, s[nt][2 * n + 1]);
+                    for (int i = 0; i < NT; ++i) {
+                        const uint4 t = queries[(blk * NT + i) * 32 + lane];
+                        q[4 * i] = t.x; q[4 * i + 1] = t.y; q[4 * i + 2] = t.z; q[4 * i + 3] = t.w;
                     }
+#pragma unroll
+                    for (int nt = 0; nt < kCols; ++nt) add_block(nt, blk, q, f[nt]);
+                }
+            } else {
+#pragma unroll
+                for (int nt = 0; nt < kCols; ++nt) {
+                    uint32_t f[kBlocks];
+                    factors(nt, f);
+#pragma unroll
+                    for (int blk = 0; blk < kBlocks; ++blk) add_block(nt, blk, qf[blk], f);
                 }
             }
             if (mask != kFull) {
