@@ -48,6 +48,7 @@ constexpr int kThreads = 32 * kWarps;
 constexpr int kJoinWarps = 4;
 constexpr int kJoinThreads = 32 * kJoinWarps;
 constexpr int kSegmentCost = 2;
+constexpr int64_t kScanBatch = 128;
 constexpr int kMinRef = 20;  // a weight times 2^(142 - R), and a tile's sum of them, stay below 2^127
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -84,17 +85,6 @@ struct Params {
     int2* meta;       // (batch * heads * row_groups): first and last warp of a split segment
 };
 
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, d));
-    return v;
-}
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
-    return v;
-}
-
 __device__ __forceinline__ int length_of(const CacheAttentionArgs& a, int64_t b) {
     return (int)visible_length(a.lengths[b], a.max_pages, a.c.page_shift);
 }
@@ -103,6 +93,36 @@ __device__ __forceinline__ int length_of(const CacheAttentionArgs& a, int64_t b)
 template <int POS>
 __device__ __forceinline__ int cost_of(int len) {
     return len == 0 ? 0 : (len + POS - 1) / POS + kSegmentCost;
+}
+
+// A lane's share of the sequences' costs: neighbouring sequences b0 .. b1 - 1;
+// the sums (over one head group) fit 32 bits, the entry checks it.
+struct Costs {
+    int64_t b0, b1, total;
+    uint32_t mine, upto;  // of these sequences, and of all up to them
+    int len;              // of the last of them
+};
+
+template <int POS>
+__device__ __forceinline__ Costs costs_of(const CacheAttentionArgs& a, int lane) {
+    Costs c;
+    const int64_t per = (a.batch + 31) / 32;
+    c.b0 = min(a.batch, per * lane);
+    c.b1 = min(a.batch, c.b0 + per);
+    c.mine = 0;
+    c.len = 0;
+    for (int64_t b = c.b0; b < c.b1; ++b) {
+        c.len = length_of(a, b);
+        c.mine += cost_of<POS>(c.len);
+    }
+    c.upto = c.mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const uint32_t o = __shfl_up_sync(0xFFFFFFFFu, c.upto, d);
+        if (lane >= d) c.upto += o;
+    }
+    c.total = (int64_t)__shfl_sync(0xFFFFFFFFu, c.upto, 31);
+    return c;
 }
 
 // A warp's place: sequence b, head group g (KV head and row group), tile t of
@@ -469,28 +489,15 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = lane >> 2, quad = lane & 3;
     const int groups = p.a.c.heads * p.row_groups;
 
-    grid_launch_dependents();  // the second launch may take its place: it waits for this one's end
     grid_wait_prerequisites();
+    grid_launch_dependents();  // the second launch may take its place, with what ran before this one complete
     // ---- the warps' shares of all costs, and where this one's begins: every warp for itself ----
-    // a lane has the costs of neighbouring sequences; their sum fits 32 bits (the entry checks it)
-    const int64_t per = (p.a.batch + 31) / 32;
-    const int64_t b0 = min(p.a.batch, per * lane), b1 = min(p.a.batch, b0 + per);
-    uint32_t mine = 0;
-    int len = 0;  // of the last of them: all there is to know while a lane has one
-    for (int64_t b = b0; b < b1; ++b) {
-        len = length_of(p.a, b);
-        mine += cost_of<POS>(len);
-        if (blockIdx.x == 0 && warp == 0 && p.a.status &&
-            (int64_t)p.a.lengths[b] > (p.a.max_pages << p.a.c.page_shift))
-            atomicOr(p.a.status, kErrCacheIndex);
+    const Costs costs = costs_of<POS>(p.a, lane);
+    if (blockIdx.x == 0 && warp == 0 && p.a.status) {
+        for (int64_t b = costs.b0; b < costs.b1; ++b)
+            if ((int64_t)p.a.lengths[b] > (p.a.max_pages << p.a.c.page_shift)) atomicOr(p.a.status, kErrCacheIndex);
     }
-    uint32_t upto = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const uint32_t o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
-        if (lane >= d) upto += o;
-    }
-    const int64_t total = (int64_t)__shfl_sync(0xFFFFFFFFu, upto, 31) * groups;
+    const int64_t total = costs.total * groups;
     const int64_t parts = min(p.parts, total);
     const int64_t first_part = (int64_t)blockIdx.x * kWarps;
     if (first_part >= parts) return;
@@ -502,11 +509,11 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
         const int64_t begin = split_begin(split, part);
         cur.end = split_begin(split, part + 1);
         // the lane whose sequences hold the first unit, and the one of them
-        const int at_lane = __ffs(__ballot_sync(0xFFFFFFFFu, begin < (int64_t)upto * groups)) - 1;
-        cur.b = __shfl_sync(0xFFFFFFFFu, b0, at_lane);
-        cur.base = (int64_t)(__shfl_sync(0xFFFFFFFFu, upto - mine, at_lane)) * groups;
-        cur.len = __shfl_sync(0xFFFFFFFFu, len, at_lane);
-        if (per > 1) {
+        const int at_lane = __ffs(__ballot_sync(0xFFFFFFFFu, begin < (int64_t)costs.upto * groups)) - 1;
+        cur.b = __shfl_sync(0xFFFFFFFFu, costs.b0, at_lane);
+        cur.base = (int64_t)(__shfl_sync(0xFFFFFFFFu, costs.upto - costs.mine, at_lane)) * groups;
+        cur.len = __shfl_sync(0xFFFFFFFFu, costs.len, at_lane);
+        if (p.a.batch > 32) {
             for (;; ++cur.b) {
                 cur.len = length_of(p.a, cur.b);
                 const int64_t n = (int64_t)cost_of<POS>(cur.len) * groups;
@@ -786,9 +793,9 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
             const int sub = cur.g - (int)cur.head * p.row_groups;
             const int64_t head0 = cur.b * p.a.q_heads + (int64_t)cur.head * p.group + sub * C::rows;
             const int rows = min(C::rows, p.group - sub * C::rows);
-            if (begins && lane == 0) {
+            if (begins && lane == 0 && p.a.batch > kScanBatch) {
                 const int64_t last = split_part(split, cur.base + kSegmentCost + cur.nt - 1);
-                gstore_plain(p.meta + seg, ends ? make_int2(0, -1) : make_int2((int)part, (int)last), p.a.ww,
+                gstore_plain(p.meta + seg, ends ? make_int2(1, 0) : make_int2((int)part, (int)last), p.a.ww,
                              p.a.status);
             }
             const float unit = exp2f((float)(ref - 142));
@@ -898,135 +905,120 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
                 gstore_plain(reinterpret_cast<float2*>(p.part_o + at * D + 2 * lane + 64 * k), o[k], p.a.ww, p.a.status);
             if (lane == 0) gstore_plain(p.part_ml + at, make_float2(top, sum), p.a.ww, p.a.status);
         }
-        // the others' slots hold nothing
-        if (warp != first && lane < rows)
-            gstore_plain(p.part_ml + open_slot * C::rows + lane, make_float2(-INFINITY, 0.0f), p.a.ww, p.a.status);
     }
 }
 
 // Second launch: W warps (a CTA, or one of its four) per (sequence, query
 // head).  Empty sequences get their zeros here; segments that one warp held are
-// done; the pieces of the others are joined in order, every W-th by one warp.
-// Latency is all there is to it, so a thread looks at up to four pieces at
-// once, and a warp reads four.
+// done.  The pieces of the others (one for the warps first .. last - 1 of each
+// CTA, one of warp last) are joined in order, every W-th by one warp.  Latency
+// is all there is to it, so where the pieces are follows from (first, last)
+// alone, and a warp has its maxima, sums and elements of kEach pieces on their
+// way at once.
 template <int D, int NT, int W>
 __global__ void __launch_bounds__(kJoinThreads) cache_attention_join_kernel(const Params p) {
     using C = Config<D, NT>;
-    constexpr int kVecs = D / 64, kEach = 4, kThreadsEach = 32 * W, kPass = kEach * kThreadsEach;
-    constexpr int kUnits = kJoinWarps / W;
-    __shared__ float tops[kJoinWarps], totals[kJoinWarps];
-    __shared__ float weights_of[kUnits][kPass];
-    __shared__ uint32_t present_of[kUnits][kPass / 32];  // which pieces have something in them
-    __shared__ uint16_t list_of[kUnits][kPass];
+    constexpr int kVecs = D / 64, kEach = 4;
+    __shared__ float2 ml_of[kJoinWarps];
     __shared__ float2 sums[W > 1 ? W : 1][W > 1 ? D / 2 : 1];
     grid_launch_dependents();
-    grid_wait_prerequisites();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int tid = W == 1 ? lane : threadIdx.x, mine = W == 1 ? 0 : warp;  // thread and warp of the unit
     const int64_t unit = W == 1 ? (int64_t)blockIdx.x * kJoinWarps + warp : blockIdx.x;
-    if (unit >= p.a.batch * p.a.q_heads) return;
-    float* const weights = weights_of[W == 1 ? warp : 0];
-    uint32_t* const present = present_of[W == 1 ? warp : 0];
-    uint16_t* const list = list_of[W == 1 ? warp : 0];
-    auto sync = [] {
-        if (W == 1) __syncwarp();
-        else __syncthreads();
-    };
-    const int64_t b = unit / p.a.q_heads;
+    const bool on_grid = unit < p.a.batch * p.a.q_heads;
+    const int64_t b = on_grid ? unit / p.a.q_heads : 0;
     const int head = (int)(unit - b * p.a.q_heads);
     const int in = head % p.group, sub = in / C::rows, r = in - sub * C::rows;
-    int2 parts = p.meta[(b * p.a.c.heads + head / p.group) * p.row_groups + sub];  // not written for an empty sequence
-    if (length_of(p.a, b) == 0) parts = make_int2(0, -1);
-    else if (parts.y < parts.x) return;
-    const int pieces = parts.y - parts.x + 1;
-    auto slot_of = [&](int i) { return (2 * (int64_t)(parts.x + i) + (i == 0)) * C::rows + r; };
-    auto piece_of = [&](int i) { return i < pieces ? p.part_ml[slot_of(i)] : make_float2(-INFINITY, 0.0f); };
-    float2 ml[kEach];  // of the pass in hand: pieces 32 W j + thread
-    float top = -INFINITY;
-    for (int i0 = (pieces - 1) / kPass * kPass; i0 >= 0; i0 -= kPass) {  // the first pass last: it is kept
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) ml[j] = piece_of(i0 + j * kThreadsEach + tid);
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) top = fmaxf(top, ml[j].x);
+    const int g = head / p.group * p.row_groups + sub, groups = p.a.c.heads * p.row_groups;
+    int2 parts;
+    if (p.a.batch <= kScanBatch) {  // the lengths are there already: what the first launch waited for is complete
+        const Costs costs = costs_of<C::pos>(p.a, lane);
+        const int at_lane = (int)(b / ((p.a.batch + 31) / 32));
+        uint32_t before = __shfl_sync(0xFFFFFFFFu, costs.upto - costs.mine, at_lane);
+        for (int64_t i = __shfl_sync(0xFFFFFFFFu, costs.b0, at_lane); i < b; ++i)
+            before += cost_of<C::pos>(length_of(p.a, i));
+        const int len = length_of(p.a, b), nt = (len + C::pos - 1) / C::pos;
+        const int64_t total = costs.total * groups;
+        parts = make_int2(0, -1);
+        if (len > 0) {
+            const Split split = make_split(min(p.parts, total), total);
+            const int64_t tiles = (int64_t)before * groups + (int64_t)g * (nt + kSegmentCost) + kSegmentCost;
+            parts = make_int2((int)split_part(split, tiles), (int)split_part(split, tiles + nt - 1));
+            if (parts.x == parts.y) parts.x = parts.y + 1;
+        }
     }
-    top = warp_max(top);
-    if constexpr (W > 1) {
-        if (lane == 0) tops[warp] = top;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < W; ++w) top = fmaxf(top, tops[w]);
+    grid_wait_prerequisites();
+    if (!on_grid) return;
+    if (p.a.batch > kScanBatch) {
+        parts = p.meta[b * groups + g];  // not written for an empty sequence
+        if (length_of(p.a, b) == 0) parts = make_int2(0, -1);
     }
-    float sum = 0.0f;
+    if (parts.y >= 0 && parts.y < parts.x) return;  // one warp held it
+    const int first_cta = parts.x / kWarps;
+    const int pieces = parts.y < 0 ? 0 : (parts.y - 1) / kWarps - first_cta + 2;
+    auto slot_of = [&](int i) {
+        const int64_t slot = i == 0 ? 2 * (int64_t)parts.x + 1 : 2 * (int64_t)(i + 1 < pieces ? (first_cta + i) * kWarps : parts.y);
+        return slot * C::rows + r;
+    };
+    float top = -INFINITY, sum = 0.0f;
     float2 o[kVecs];
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) o[k] = make_float2(0.0f, 0.0f);
-    for (int i0 = 0; i0 < pieces; i0 += kPass) {
+    for (int i0 = W == 1 ? 0 : warp; i0 < pieces; i0 += kEach * W) {
+        float2 ml[kEach], v[kEach][kVecs];
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
-            if (i0 > 0) ml[j] = piece_of(i0 + j * kThreadsEach + tid);
+            const bool on = i0 + j * W < pieces;
+            const int64_t at = slot_of(on ? i0 + j * W : i0);
+            ml[j] = on ? p.part_ml[at] : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+            for (int k = 0; k < kVecs; ++k)
+                v[j][k] = on ? *reinterpret_cast<const float2*>(p.part_o + at * D + 2 * lane + 64 * k)
+                             : make_float2(0.0f, 0.0f);
+        }
+        float most = top;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) most = fmaxf(most, ml[j].x);
+        const float keep = sum != 0.0f ? exp2_fast(top - most) : 0.0f;
+        top = most;
+        sum *= keep;
+#pragma unroll
+        for (int k = 0; k < kVecs; ++k) {
+            o[k].x *= keep;
+            o[k].y *= keep;
+        }
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
             const float weight = ml[j].y != 0.0f ? exp2_fast(ml[j].x - top) : 0.0f;
             sum += ml[j].y * weight;
-            weights[j * kThreadsEach + tid] = weight;
-            const uint32_t there = __ballot_sync(0xFFFFFFFFu, ml[j].y != 0.0f);
-            if (lane == 0) present[j * W + mine] = there;
-        }
-        sync();
-        // pieces with something in them, in order
-        int count = 0;
-        for (int word = 0; word < kPass / 32; ++word) count += __popc(present[word]);
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-            const int own = j * W + mine;
-            const uint32_t there = present[own];
-            if (!((there >> lane) & 1)) continue;
-            int rank = __popc(there & ((1u << lane) - 1));
-            for (int word = 0; word < own; ++word) rank += __popc(present[word]);
-            list[rank] = (uint16_t)(own * 32 + lane);
-        }
-        sync();
-        for (int n0 = mine; n0 < count; n0 += 4 * W) {  // four pieces' loads before the first use
-            float2 v[4][kVecs];
-            float f[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const bool on = n0 + j * W < count;
-                const int i = list[on ? n0 + j * W : n0];
-                f[j] = on ? weights[i] : 0.0f;
-                const float* src = p.part_o + slot_of(i0 + i) * D + 2 * lane;
-#pragma unroll
-                for (int k = 0; k < kVecs; ++k) v[j][k] = *reinterpret_cast<const float2*>(src + 64 * k);
-                if (!on) {
-#pragma unroll
-                    for (int k = 0; k < kVecs; ++k) v[j][k] = make_float2(0.0f, 0.0f);
-                }
+            for (int k = 0; k < kVecs; ++k) {
+                o[k].x += v[j][k].x * weight;
+                o[k].y += v[j][k].y * weight;
             }
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int k = 0; k < kVecs; ++k) {
-                    o[k].x += v[j][k].x * f[j];
-                    o[k].y += v[j][k].y * f[j];
-                }
         }
-        sync();
     }
-    sum = warp_sum(sum);
     uint16_t* const out = p.a.out + unit * D;
     if constexpr (W > 1) {
-        if (lane == 0) totals[warp] = sum;
+        if (lane == 0) ml_of[warp] = make_float2(top, sum);
 #pragma unroll
         for (int k = 0; k < kVecs; ++k) sums[warp][lane + 32 * k] = o[k];
         __syncthreads();
+        float weight[W];
+#pragma unroll
+        for (int w = 0; w < W; ++w) top = fmaxf(top, ml_of[w].x);
         sum = 0.0f;
 #pragma unroll
-        for (int w = 0; w < W; ++w) sum += totals[w];
+        for (int w = 0; w < W; ++w) {
+            weight[w] = ml_of[w].y != 0.0f ? exp2_fast(ml_of[w].x - top) : 0.0f;
+            sum += ml_of[w].y * weight[w];
+        }
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         for (int d = threadIdx.x; d < D / 2; d += kJoinThreads) {
-            float2 v = sums[0][d];
+            float2 v = make_float2(0.0f, 0.0f);
 #pragma unroll
-            for (int w = 1; w < W; ++w) {
-                v.x += sums[w][d].x;
-                v.y += sums[w][d].y;
+            for (int w = 0; w < W; ++w) {
+                v.x += sums[w][d].x * weight[w];
+                v.y += sums[w][d].y * weight[w];
             }
             gstore_plain(reinterpret_cast<uint32_t*>(out + 2 * d), pack_out(p.a.q_bf16, v.x * inv, v.y * inv), p.a.ow,
                          p.a.status);
@@ -1038,7 +1030,7 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attention_join_kernel(cons
             gstore_plain(reinterpret_cast<uint32_t*>(out + 2 * lane + 64 * k),
                          pack_out(p.a.q_bf16, o[k].x * inv, o[k].y * inv), p.a.ow, p.a.status);
     }
-    if (p.a.lse && tid == 0)
+    if (p.a.lse && lane == 0 && (W == 1 || warp == 0))
         gstore_plain(p.a.lse + unit, (top + log2f(sum)) * kLn2, p.a.lw, p.a.status);
 }
 

@@ -51,19 +51,19 @@ MXFP8_HD int64_t sequence_from(const int32_t* starts, int64_t batch, int64_t fro
 struct Split {
     int64_t each, longer;
 };
+// a / b, both at least 0: in 32 bits where they allow it, the common case.
+MXFP8_HD int64_t quotient(int64_t a, int64_t b) {
+    return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
 MXFP8_HD Split make_split(int64_t n, int64_t total) {
-    if (total <= 0xFFFFFFFFll) {  // the common case: a 32-bit division
-        const uint32_t each = (uint32_t)total / (uint32_t)n;
-        return Split{each, total - (int64_t)each * n};
-    }
-    const int64_t each = total / n;
+    const int64_t each = quotient(total, n);
     return Split{each, total - each * n};
 }
 MXFP8_HD int64_t split_begin(const Split& s, int64_t i) { return i * s.each + (i < s.longer ? i : s.longer); }
 // The part that holds unit x < total.
 MXFP8_HD int64_t split_part(const Split& s, int64_t x) {
     const int64_t edge = s.longer * (s.each + 1);  // end of the longer parts
-    return x < edge ? x / (s.each + 1) : s.longer + (x - edge) / s.each;
+    return x < edge ? quotient(x, s.each + 1) : s.longer + quotient(x - edge, s.each);
 }
 
 // Positions of a sequence that the attention visits.
