@@ -305,6 +305,15 @@ def test_attention_splits(lengths, heads, group, dim):
     assert capi.device_status() == 0
 
 
+@pytest.mark.parametrize("batch", [31, 32, 33, 127, 128, 129])
+def test_attention_batches(batch):
+    """Around the batches at which a lane gets another sequence, and the join looks up where the pieces are."""
+    lengths = [(37 * i) % 1500 if i % 5 else 0 for i in range(batch)]
+    q, cache, table = attention_case(lengths, 16, 2, 4, 64, "bf16", seed=batch)
+    check_attention(q, cache, table, lengths, 16)
+    assert capi.device_status() == 0
+
+
 @pytest.mark.parametrize("scale", [0.0, 1.0, -0.3])
 def test_attention_scales(scale):
     q, cache, table = attention_case([100, 7], 8, 2, 4, 64, "bf16")
