@@ -72,11 +72,14 @@ MXFP8_API int64_t mxfp8_cache_attention_workspace(const mxfp8_cache* cache, int6
  * elements, last dimension contiguous; out contiguous of the same type and
  * lse (batch, q_heads) f32 or NULL: log of the sum of exp(scale * q . k_j).
  * dim is 64, 128, 192 or 256, page_size at least 2, q_heads a multiple of
- * heads, max_pages * page_size < 2^31 - 1024, and batch times that at most 2^34.  A length of 0 (or below) gives zeros and lse -inf; a position whose page is
- * outside the cache takes no part, as if it were not there, and is reported; a
- * length past the table is cut to it and reported.  Scores, sums and outputs
- * are held in f32 and rounded once; a score overflows where a K block's scale
- * is 2^96 or more (the query is held with its largest element near 2^14).  workspace is 16-byte aligned scratch of
+ * heads, max_pages * page_size < 2^31 - 1024, and batch times that at most
+ * 2^34.  A length of 0 (or below) gives zeros and lse -inf; a position whose
+ * page is outside the cache takes no part, as if it were not there, and is
+ * reported; a length past the table is cut to it and reported.  Scores and sums
+ * are held in f32, weights in f16 (2^-11 relative, scaled so that they neither
+ * overflow nor vanish beside the others), outputs rounded once; a score
+ * overflows where a K block's scale is 2^96 or more (the query is held with its
+ * largest element near 2^14).  workspace is 16-byte aligned scratch of
  * one call at a time; its contents do not matter before or after. */
 MXFP8_API int mxfp8_cache_attention(const mxfp8_cache* cache, const void* q, int64_t q_batch_stride,
                                     int64_t q_head_stride, int dtype, int64_t batch, int64_t q_heads,

@@ -12,13 +12,24 @@
 // wide: P is A, Q is B.  The two CTAs of a cluster pair compute one 256 x 256
 //   tile (cta_group::2): each loads its 128 rows of A and half of the 256 rows
 //   of B, 35 KB a stage for 4 MMAs where a CTA on its own would load 51.  A lane
-//   is a row of C, its columns are contiguous in memory: 32-byte stores.
+//   is a row of C, its columns are contiguous in memory: 32-byte stores.  Where
+//   rows of C do not start on 32 bytes, P is B and Q is A, as in the narrow form.
 // narrow: P is B, Q is A.  A lane is a column of C, so a warp's stores are
 //   contiguous for any alignment, and few rows of A make a narrow tile: the
 //   form for single tokens, where streaming B is the whole cost.  If there are
 //   fewer tiles than SMs, a cluster of CTAs shares a tile: each takes a part of
 //   K, and their sums meet in shared memory over the cluster in rank order, so
 //   the result does not depend on timing.
+//
+// Measured, bf16 out: 8192x8192x8192 187 us = 5.9 PFLOP/s for a burst, 216 us
+// under the power cap; 4096x4096x4096 29.5 us = 4.7.  One pair a tile leaves the
+// tensor cores waiting while its accumulators are read (256 + 48 of 512 columns
+// of tensor memory: no second set fits): 8192x4096x1024 22.8 us = 3.0 PFLOP/s.
+// One token through 16384x8192 14.8 us = 4.8 TB/s, through 4096x4096 5.7 us =
+// 1.6 TB/s: there the launch, the first loads and the join of the split take
+// longer than the stream.  Loops of a whole warp with one elected lane issue a
+// stage's instructions in about a tenth of the cycles that a one-lane branch
+// takes: 8192x8192x8192 was 348 us with those.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
@@ -196,14 +207,13 @@ __device__ __forceinline__ void store_quad(const GemmParams& p, int64_t row, int
         if (col + i < p.rows_p) store1<OUT>(p.out, at + i, f[i], p.ow, p.status);
 }
 
-// NC f32 of one row of C, columns col .. col + NC - 1 (those below n), to out.
+// NC f32 of one row of C, columns col .. col + NC - 1 (those below n), to out, whose rows start on 32 bytes.
 template <int OUT, int NC>
-__device__ __forceinline__ void store_row(const GemmParams& p, int64_t row, int col, int n, const uint32_t* acc,
-                                          bool vec) {
+__device__ __forceinline__ void store_row(const GemmParams& p, int64_t row, int col, int n, const uint32_t* acc) {
     constexpr int kEs = OUT == MXFP8_F32 ? 4 : 2;
     constexpr int kPer = 32 / kEs;  // elements of one 32-byte store
     const int64_t at = row * p.ld_out + col;
-    if (vec && col + NC <= n) {
+    if (col + NC <= n) {
 #pragma unroll
         for (int i = 0; i < NC; i += kPer) {
             if constexpr (OUT == MXFP8_F32) {
@@ -413,8 +423,8 @@ __global__ void __launch_bounds__(Narrow<BN>::threads, 1)
 
 // The wide form: a cluster pair a tile.  Each CTA loads its share, all of it
 // signalled on the even CTA's barriers; that one issues for both, and each
-// reads its half of the rows back.
-template <int OUT>
+// reads its half of the rows back: rows of C, or columns if ACROSS.
+template <int OUT, bool ACROSS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide::threads, 1)
     mxfp4_gemm_wide_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
                            const __grid_constant__ CUtensorMap map_sp, const __grid_constant__ CUtensorMap map_sq,
@@ -528,8 +538,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide::threads, 1)
         const int q4 = warp & 3, col0 = (warp >> 2) * 128;
         const uint32_t d = tmem + col0 + ((uint32_t)(q4 * 32) << 16);
         const uint32_t peer_acc_empty = cluster_map(acc_empty, 0);
-        constexpr int kEs = OUT == MXFP8_F32 ? 4 : 2;
-        const bool vec = ((reinterpret_cast<uintptr_t>(p.out) | (uint64_t)(p.ld_out * kEs)) & 31) == 0;
         int a = 0;
         for (int t = first_tile; t < p.n_tiles; t += tile_step, ++a) {
             if (!wait_phase(acc_full, a & 1, ctl, p.status)) break;
@@ -549,8 +557,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide::threads, 1)
             const int64_t row = (int64_t)(2 * tp + rank) * kTileP + q4 * 32 + lane;
             if (row < p.rows_p) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    store_row<OUT, 32>(p, row, tq * C::bn + col0 + 32 * i, p.rows_q, v[i], vec);
+                for (int i = 0; i < 4; ++i) {
+                    const int col = tq * C::bn + col0 + 32 * i;
+                    if constexpr (ACROSS) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (col + j < p.rows_q)
+                                store1<OUT>(p.out, (int64_t)(col + j) * p.ld_out + row, __uint_as_float(v[i][j]), p.ow,
+                                            p.status);
+                    } else {
+                        store_row<OUT, 32>(p, row, col, p.rows_q, v[i]);
+                    }
+                }
             }
         }
     }
@@ -635,19 +653,21 @@ GemmParams params_of(const Fp4GemmArgs& g, const Fp4Operand& P, const Fp4Operand
     return p;
 }
 
-template <int OUT>
+template <int OUT, bool ACROSS>
 int launch_wide(const Fp4GemmArgs& g, int sm_count, cudaStream_t stream) {
     using C = Wide;
     static std::atomic<uint64_t> done{0};
-    auto kernel = mxfp4_gemm_wide_kernel<OUT>;
+    auto kernel = mxfp4_gemm_wide_kernel<OUT, ACROSS>;
+    const Fp4Operand& P = ACROSS ? g.b : g.a;
+    const Fp4Operand& Q = ACROSS ? g.a : g.b;
     cudaError_t e = opt_in(kernel, C::smem, done);
     if (e != cudaSuccess) return launch_failed("cudaFuncSetAttribute", e);
     CUtensorMap map_p, map_q, map_sp, map_sq;
-    if (int rc = encode_payload(&map_p, g.a, g.k, kTileP)) return rc;
-    if (int rc = encode_payload(&map_q, g.b, g.k, C::bn / 2)) return rc;
-    if (int rc = encode_scales(&map_sp, g.a, g.k, 1)) return rc;
-    if (int rc = encode_scales(&map_sq, g.b, g.k, 2)) return rc;
-    const GemmParams p = params_of(g, g.a, g.b, 2 * kTileP, C::bn);
+    if (int rc = encode_payload(&map_p, P, g.k, kTileP)) return rc;
+    if (int rc = encode_payload(&map_q, Q, g.k, C::bn / 2)) return rc;
+    if (int rc = encode_scales(&map_sp, P, g.k, 1)) return rc;
+    if (int rc = encode_scales(&map_sq, Q, g.k, 2)) return rc;
+    const GemmParams p = params_of(g, P, Q, 2 * kTileP, C::bn);
     cudaLaunchConfig_t cfg = {};
     const int pairs = sm_count / 2;
     cfg.gridDim = dim3(2u * (unsigned)(p.n_tiles < pairs ? p.n_tiles : pairs));
@@ -713,7 +733,10 @@ int launch_out(const Fp4GemmArgs& g, int sm_count, cudaStream_t stream) {
     // (narrow).  Measured, us wide / narrow: 512x2048x2048 7.7 / 8.3,
     // 384x4096x4096 10.4 / 12.7, 256x8192x8192 16.7 / 18.8; with K long and
     // split the narrow one wins: 256x4096x4096 10.2 / 9.7, 512x1024x8192 15.3 / 10.0.
-    // The wide form's stores want rows of C on 32 bytes.
+    // Rows of C that are not all on 32 bytes are stored an element a lane, which
+    // costs the wide form more: 4096x4097x4096 36.4 / 54.5, 2000x2001x7168 19.1 /
+    // 27.2, 1024x4097x512 9.7 / 12.8, but as many stages in both 512x4097x4096
+    // 13.8 / 13.0, 1500x1501x256 8.7 / 7.6.
     const int es = OUT == MXFP8_F32 ? 4 : 2;
     const bool vec = ((reinterpret_cast<uintptr_t>(g.out) | (uint64_t)(g.ld_out * es)) & 31) == 0;
     const int64_t stages = (g.k + kStageK - 1) / kStageK;
@@ -722,7 +745,8 @@ int launch_out(const Fp4GemmArgs& g, int sm_count, cudaStream_t stream) {
     const int split = narrow_split(narrow_tiles, (int)stages, sm_count);
     const int64_t narrow_row = (stages + split - 1) / split * ((narrow_tiles * split + sm_count - 1) / sm_count);
     const int64_t wide_row = stages * ((wide_tiles + sm_count / 2 - 1) / (sm_count / 2));
-    if (vec && wide_row <= narrow_row + 6) return launch_wide<OUT>(g, sm_count, stream);
+    if (vec && wide_row <= narrow_row + 6) return launch_wide<OUT, false>(g, sm_count, stream);
+    if (!vec && wide_row < narrow_row) return launch_wide<OUT, true>(g, sm_count, stream);
     return launch_narrow<128, OUT>(g, sm_count, stream);
 }
 

@@ -226,6 +226,13 @@ def test_gemm_many_tiles(m, n, k, out):
     check_gemm(m, n, k, out)
 
 
+@pytest.mark.parametrize("m,n,k", [(65, 129, 32), (300, 515, 512), (513, 1001, 96), (256, 257, 4096), (1025, 2047, 288),
+                                   (3001, 2999, 160)])
+@pytest.mark.parametrize("out", ["bf16", "fp16", "f32"])
+def test_gemm_rows_off_32_bytes(m, n, k, out):
+    check_gemm(m, n, k, out, seed=1)
+
+
 @pytest.mark.parametrize("m", [1, 16, 40, 130, 4096])
 def test_gemm_small_integers_are_exact(m):
     """All scales 1 and k <= 1024: every partial sum is a multiple of 1/4 below 2^16, so f32 holds it."""
