@@ -7,8 +7,9 @@
  * power of two, at most 4096):
  *   k, v               (num_pages, heads, page_size, dim) E4M3 bytes
  *   k_scales, v_scales (num_pages, heads, page_size, dim / 32) UE8M0 bytes
- * all contiguous, dim % 32 == 0 and dim <= 1024, k and v 16-byte aligned, the
- * scales 4-byte aligned, num_pages * heads * page_size < 2^32.  A position
+ * all contiguous, dim % 32 == 0 and dim <= 1024, heads <= 65536, k and v
+ * 16-byte aligned, the scales 4-byte aligned, num_pages * heads * page_size <
+ * 2^32.  A position
  * (slot) is page * page_size + offset.  Rows are quantized by the recipe of
  * mxfp8_quantize along dim, so a row's bytes equal those of quantizing it
  * alone.

@@ -13,6 +13,7 @@ namespace {
 
 constexpr int64_t kInt32Max = 2147483647;
 constexpr int64_t kMaxStride = int64_t(1) << 38;
+constexpr int kMaxHeads = 65536;  // a token's rows are counted in 32 bits
 
 inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
@@ -20,8 +21,9 @@ inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintp
 int check_cache(const mxfp8_cache* cache, CacheShape* c) {
     if (!cache) return MXFP8_ERR_NULL_POINTER;
     const int s = cache->page_size;
-    if (cache->num_pages < 0 || cache->heads < 1 || s < 1 || s > 4096 || (s & (s - 1)) != 0 || cache->dim < 32 ||
-        cache->dim > 1024 || cache->dim % 32 != 0 || cache->num_pages > ((int64_t(1) << 32) - 1) / cache->heads / s)
+    if (cache->num_pages < 0 || cache->heads < 1 || cache->heads > kMaxHeads || s < 1 || s > 4096 ||
+        (s & (s - 1)) != 0 || cache->dim < 32 || cache->dim > 1024 || cache->dim % 32 != 0 ||
+        cache->num_pages > ((int64_t(1) << 32) - 1) / cache->heads / s)
         return MXFP8_ERR_SHAPE;
     if (cache->num_pages > 0) {
         if (!cache->k || !cache->v || !cache->k_scales || !cache->v_scales) return MXFP8_ERR_NULL_POINTER;
@@ -49,7 +51,7 @@ inline int64_t positions(const CacheShape& c) { return (c.num_pages * c.heads) <
 inline bool rows_aligned(const void* p, int64_t a, int64_t b) { return aligned(p, 32) && a % 16 == 0 && b % 16 == 0; }
 
 int attention_shape(const CacheShape& c, int64_t batch, int64_t q_heads) {
-    if (batch < 0 || q_heads < 1 || q_heads > 65536 || q_heads % c.heads != 0 || batch > kInt32Max / q_heads ||
+    if (batch < 0 || q_heads < 1 || q_heads > kMaxHeads || q_heads % c.heads != 0 || batch > kInt32Max / q_heads ||
         c.page_shift < 1 || (c.dim != 64 && c.dim != 128 && c.dim != 192 && c.dim != 256))
         return MXFP8_ERR_SHAPE;
     return MXFP8_OK;

@@ -142,6 +142,15 @@ def test_bad_caches_are_refused(call, change, match):
         call(a_cache(**change))
 
 
+@pytest.mark.parametrize("heads", [65537, 2 ** 25, 2 ** 28, 2 ** 31 - 1])
+@pytest.mark.parametrize("call", [write, read, attend])
+def test_more_heads_than_32_bits_count_are_refused(call, heads):
+    """Rows of a token: heads * dim / 16 of them a thread each; 2^28 heads of 128 elements are 2^32 eighths."""
+    for pages in (0, 1):
+        with pytest.raises(ValueError, match="sizes"):
+            call(a_cache(num_pages=pages, page_size=2, heads=heads))
+
+
 @pytest.mark.parametrize("call,change,match", [
     (write, dict(dtype=2), "dtype"), (write, dict(tokens=-1), "sizes"), (write, dict(kt=-1), "sizes"),
     (write, dict(k=0), "NULL"), (write, dict(slots=0), "NULL"), (write, dict(v=0x6001), "alignment"),
