@@ -46,6 +46,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "../../include/mxfp8_cache.h"
@@ -97,6 +98,7 @@ struct Params {
     int group;        // query heads of a KV head
     int row_groups;   // ceil(group / rows)
     int64_t parts;    // warps
+    int join_segments;  // that a CTA of the join looks at
     float* part_o;    // (2 * parts, rows, D): unscaled sums of the pieces
     float2* part_ml;  // (2 * parts, rows): running maximum (log2) and sum
     int2* meta;       // (batch * heads * row_groups): first and last warp of a split segment, if batch > kScanBatch
@@ -929,28 +931,39 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
     }
 }
 
-// Second launch: W warps (a CTA, or one of its four) per (sequence, query
-// head).  Empty sequences get their zeros here; segments that one warp held are
-// done.  The pieces of the others (one for the warps first .. last - 1 of each
-// CTA, one of warp last) are joined in order, every W-th by one warp.  Latency
-// is all there is to it, so where the pieces are follows from (first, last)
-// alone, and a warp has its maxima, sums and elements of kEach pieces on their
-// way at once.
+// Second launch: zeros for the segments of empty sequences, and the pieces of
+// those that more than one warp held (one for the warps first .. last - 1 of
+// each CTA, one of warp last) joined in order.  W = 4: a CTA a (sequence, query
+// head), every fourth piece by one warp.  W = 1: a CTA looks at p.join_segments
+// segments, a lane each, and its warps (with those of the other blockIdx.y)
+// take the query heads of those with work in turn.  Latency is all there is to it, so where the pieces are follows from
+// (first, last) alone, and a warp has its maxima, sums and elements of kEach
+// pieces on their way at once.
 template <int D, int NT, int W>
 __global__ void __launch_bounds__(kJoinThreads) cache_attention_join_kernel(const Params p) {
     using C = Config<D, NT>;
     constexpr int kVecs = D / 64, kEach = 4;
-    __shared__ float2 ml_of[kJoinWarps];
-    __shared__ float2 sums[W > 1 ? W : 1][W > 1 ? D / 2 : 1];
+    __shared__ float2 ml_of[W];
+    __shared__ float2 sums[W][W > 1 ? D / 2 : 1];
     grid_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t unit = W == 1 ? (int64_t)blockIdx.x * kJoinWarps + warp : blockIdx.x;
-    const bool on_grid = unit < p.a.batch * p.a.q_heads;
-    const int64_t b = on_grid ? unit / p.a.q_heads : 0;
-    const int head = (int)(unit - b * p.a.q_heads);
-    const int in = head % p.group, sub = in / C::rows, r = in - sub * C::rows;
-    const int g = head / p.group * p.row_groups + sub, groups = p.a.c.heads * p.row_groups;
-    int2 parts;
+    const int groups = p.a.c.heads * p.row_groups;
+    const int64_t segments = p.a.batch * groups;
+    int64_t seg, seg0 = 0;
+    int only_row = 0;  // W = 4: the one row of the segment
+    if constexpr (W > 1) {
+        const uint32_t b = blockIdx.x / (uint32_t)p.a.q_heads, head = blockIdx.x - b * (uint32_t)p.a.q_heads;
+        const uint32_t kv_head = head / (uint32_t)p.group, in = head - kv_head * (uint32_t)p.group;
+        const uint32_t sub = in / C::rows;
+        seg = (int64_t)b * groups + kv_head * (uint32_t)p.row_groups + sub;
+        only_row = (int)(in - sub * C::rows);
+    } else {
+        seg0 = (int64_t)blockIdx.x * p.join_segments;
+        seg = seg0 + lane;
+    }
+    const bool own = W > 1 || (lane < p.join_segments && seg < segments);
+    const int64_t b = own ? (uint32_t)seg / (uint32_t)groups : 0u;  // there are fewer than 2^31 of them
+    int2 parts = make_int2(1, 0);  // first and last warp: (0, -1) of an empty sequence, first > last >= 0 nothing to do
     if (p.a.batch <= kScanBatch) {
         // The lengths are complete in L2: this launch began after every CTA of the first one had passed its own wait
         // for what ran before.
@@ -958,100 +971,119 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attention_join_kernel(cons
         const uint32_t before = __shfl_sync(0xFFFFFFFFu, costs.upto - costs.mine, (int)b);
         const int len = __shfl_sync(0xFFFFFFFFu, costs.len, (int)b), nt = (len + C::pos - 1) / C::pos;
         const int64_t total = costs.total * groups;
-        parts = make_int2(0, -1);
-        if (len > 0) {
+        if (own && len == 0) parts = make_int2(0, -1);
+        if (own && len > 0) {
             const Split split = make_split(min(p.parts, total), total);
-            const int64_t tiles = (int64_t)before * groups + (int64_t)g * (nt + kSegmentCost) + kSegmentCost;
-            parts = make_int2((int)split_part(split, tiles), (int)split_part(split, tiles + nt - 1));
-            if (parts.x == parts.y) parts.x = parts.y + 1;
+            const int64_t tiles = (int64_t)before * groups + (seg - b * groups) * (nt + kSegmentCost) + kSegmentCost;
+            const int2 held = make_int2((int)split_part(split, tiles), (int)split_part(split, tiles + nt - 1));
+            if (held.x < held.y) parts = held;
         }
     }
     grid_wait_prerequisites();
-    if (!on_grid) return;
-    if (p.a.batch > kScanBatch) {
-        parts = p.meta[b * groups + g];  // not written for an empty sequence
-        if (length_of(p.a, b) == 0) parts = make_int2(0, -1);
-    }
-    if (parts.y >= 0 && parts.y < parts.x) return;  // one warp held it
-    const int first_cta = parts.x / kWarps;
-    const int pieces = parts.y < 0 ? 0 : (parts.y - 1) / kWarps - first_cta + 2;
-    auto slot_of = [&](int i) {
-        const int64_t slot = i == 0 ? 2 * (int64_t)parts.x + 1 : 2 * (int64_t)(i + 1 < pieces ? (first_cta + i) * kWarps : parts.y);
-        return slot * C::rows + r;
-    };
-    float top = -INFINITY, sum = 0.0f;
-    float2 o[kVecs];
+    if (p.a.batch > kScanBatch && own) parts = length_of(p.a, b) == 0 ? make_int2(0, -1) : p.meta[seg];
+
+    // one query head, row r of its segment
+    auto join = [&](const int2 held, int64_t unit, int r) {
+        const int first_cta = held.x / kWarps;
+        const int pieces = held.y < 0 ? 0 : (held.y - 1) / kWarps - first_cta + 2;
+        auto slot_of = [&](int i) {
+            const int64_t slot =
+                i == 0 ? 2 * (int64_t)held.x + 1 : 2 * (int64_t)(i + 1 < pieces ? (first_cta + i) * kWarps : held.y);
+            return slot * C::rows + r;
+        };
+        float top = -INFINITY, sum = 0.0f;
+        float2 o[kVecs];
 #pragma unroll
-    for (int k = 0; k < kVecs; ++k) o[k] = make_float2(0.0f, 0.0f);
-    for (int i0 = W == 1 ? 0 : warp; i0 < pieces; i0 += kEach * W) {
-        float2 ml[kEach], v[kEach][kVecs];
+        for (int k = 0; k < kVecs; ++k) o[k] = make_float2(0.0f, 0.0f);
+        for (int i0 = W == 1 ? 0 : warp; i0 < pieces; i0 += kEach * W) {
+            float2 ml[kEach], v[kEach][kVecs];
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-            const bool on = i0 + j * W < pieces;
-            const int64_t at = slot_of(on ? i0 + j * W : i0);
-            ml[j] = on ? p.part_ml[at] : make_float2(-INFINITY, 0.0f);
+            for (int j = 0; j < kEach; ++j) {
+                const bool on = i0 + j * W < pieces;
+                const int64_t at = slot_of(on ? i0 + j * W : i0);
+                ml[j] = on ? p.part_ml[at] : make_float2(-INFINITY, 0.0f);
 #pragma unroll
-            for (int k = 0; k < kVecs; ++k)
-                v[j][k] = on ? *reinterpret_cast<const float2*>(p.part_o + at * D + 2 * lane + 64 * k)
-                             : make_float2(0.0f, 0.0f);
-        }
-        float most = top;
+                for (int k = 0; k < kVecs; ++k)
+                    v[j][k] = on ? *reinterpret_cast<const float2*>(p.part_o + at * D + 2 * lane + 64 * k)
+                                 : make_float2(0.0f, 0.0f);
+            }
+            float most = top;
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) most = fmaxf(most, ml[j].x);
-        const float keep = sum != 0.0f ? exp2_fast(top - most) : 0.0f;
-        top = most;
-        sum *= keep;
-#pragma unroll
-        for (int k = 0; k < kVecs; ++k) {
-            o[k].x *= keep;
-            o[k].y *= keep;
-        }
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-            const float weight = ml[j].y != 0.0f ? exp2_fast(ml[j].x - top) : 0.0f;
-            sum += ml[j].y * weight;
+            for (int j = 0; j < kEach; ++j) most = fmaxf(most, ml[j].x);
+            const float keep = sum != 0.0f ? exp2_fast(top - most) : 0.0f;
+            top = most;
+            sum *= keep;
 #pragma unroll
             for (int k = 0; k < kVecs; ++k) {
-                o[k].x += v[j][k].x * weight;
-                o[k].y += v[j][k].y * weight;
+                o[k].x *= keep;
+                o[k].y *= keep;
+            }
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) {
+                const float weight = ml[j].y != 0.0f ? exp2_fast(ml[j].x - top) : 0.0f;
+                sum += ml[j].y * weight;
+#pragma unroll
+                for (int k = 0; k < kVecs; ++k) {
+                    o[k].x += v[j][k].x * weight;
+                    o[k].y += v[j][k].y * weight;
+                }
             }
         }
-    }
-    uint16_t* const out = p.a.out + unit * D;
-    if constexpr (W > 1) {
-        if (lane == 0) ml_of[warp] = make_float2(top, sum);
+        uint16_t* const out = p.a.out + unit * D;
+        if constexpr (W > 1) {
+            if (lane == 0) ml_of[warp] = make_float2(top, sum);
 #pragma unroll
-        for (int k = 0; k < kVecs; ++k) sums[warp][lane + 32 * k] = o[k];
-        __syncthreads();
-        float weight[W];
+            for (int k = 0; k < kVecs; ++k) sums[warp][lane + 32 * k] = o[k];
+            __syncthreads();
+            float weight[W];
 #pragma unroll
-        for (int w = 0; w < W; ++w) top = fmaxf(top, ml_of[w].x);
-        sum = 0.0f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            weight[w] = ml_of[w].y != 0.0f ? exp2_fast(ml_of[w].x - top) : 0.0f;
-            sum += ml_of[w].y * weight[w];
-        }
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        for (int d = threadIdx.x; d < D / 2; d += kJoinThreads) {
-            float2 v = make_float2(0.0f, 0.0f);
+            for (int w = 0; w < W; ++w) top = fmaxf(top, ml_of[w].x);
+            sum = 0.0f;
 #pragma unroll
             for (int w = 0; w < W; ++w) {
-                v.x += sums[w][d].x * weight[w];
-                v.y += sums[w][d].y * weight[w];
+                weight[w] = ml_of[w].y != 0.0f ? exp2_fast(ml_of[w].x - top) : 0.0f;
+                sum += ml_of[w].y * weight[w];
             }
-            gstore_plain(reinterpret_cast<uint32_t*>(out + 2 * d), pack_out(p.a.q_bf16, v.x * inv, v.y * inv), p.a.ow,
-                         p.a.status);
-        }
-    } else {
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            for (int d = threadIdx.x; d < D / 2; d += kJoinThreads) {
+                float2 v = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int k = 0; k < kVecs; ++k)
-            gstore_plain(reinterpret_cast<uint32_t*>(out + 2 * lane + 64 * k),
-                         pack_out(p.a.q_bf16, o[k].x * inv, o[k].y * inv), p.a.ow, p.a.status);
+                for (int w = 0; w < W; ++w) {
+                    v.x += sums[w][d].x * weight[w];
+                    v.y += sums[w][d].y * weight[w];
+                }
+                gstore_plain(reinterpret_cast<uint32_t*>(out + 2 * d), pack_out(p.a.q_bf16, v.x * inv, v.y * inv),
+                             p.a.ow, p.a.status);
+            }
+        } else {
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+            for (int k = 0; k < kVecs; ++k)
+                gstore_plain(reinterpret_cast<uint32_t*>(out + 2 * lane + 64 * k),
+                             pack_out(p.a.q_bf16, o[k].x * inv, o[k].y * inv), p.a.ow, p.a.status);
+        }
+        if (p.a.lse && lane == 0 && (W == 1 || warp == 0))
+            gstore_plain(p.a.lse + unit, (top + log2f(sum)) * kLn2, p.a.lw, p.a.status);
+    };
+
+    const bool work = parts.y < 0 || parts.x <= parts.y;
+    if constexpr (W > 1) {
+        if (work) join(parts, blockIdx.x, only_row);
+    } else {
+        int turn = 0;  // of the warps
+        for (uint32_t left = __ballot_sync(0xFFFFFFFFu, work); left != 0; left &= left - 1) {
+            const int from = __ffs(left) - 1;
+            const int2 held = make_int2(__shfl_sync(0xFFFFFFFFu, parts.x, from), __shfl_sync(0xFFFFFFFFu, parts.y, from));
+            const int64_t at = __shfl_sync(0xFFFFFFFFu, b, from);
+            const int g = (int)(seg0 + from - at * groups);
+            const int kv_head = p.row_groups == 1 ? g : g / p.row_groups, sub = g - kv_head * p.row_groups;
+            const int rows = min(C::rows, p.group - sub * C::rows);
+            const int64_t unit = at * p.a.q_heads + (int64_t)kv_head * p.group + sub * C::rows;
+            for (int r = ((warp - turn) & (kJoinWarps - 1)) + kJoinWarps * blockIdx.y; r < rows; r += kJoinWarps * gridDim.y)
+                join(held, unit + r, r);
+            turn = (turn + rows) & (kJoinWarps - 1);
+        }
     }
-    if (p.a.lse && lane == 0 && (W == 1 || warp == 0))
-        gstore_plain(p.a.lse + unit, (top + log2f(sum)) * kLn2, p.a.lw, p.a.status);
 }
 
 template <int D, int NT>
@@ -1089,6 +1121,7 @@ int launch_typed(const CacheAttentionArgs& a, int sm_count, cudaStream_t stream)
     p.a = a;
     p.group = a.q_heads / a.c.heads;
     p.row_groups = (p.group + C::rows - 1) / C::rows;
+    p.join_segments = 1;
     const int64_t segments = a.batch * a.c.heads * p.row_groups;
     // no more warps than the longest lengths that the table allows would use
     const int64_t most = segments * (((a.max_pages << a.c.page_shift) + C::pos - 1) / C::pos + kSegmentCost);
@@ -1111,11 +1144,16 @@ int launch_typed(const CacheAttentionArgs& a, int sm_count, cudaStream_t stream)
     cfg.dynamicSmemBytes = C::smem;
     e = cudaLaunchKernelEx(&cfg, kernel, p);
     if (e == cudaSuccess) {
-        // Many heads are in few pieces each and want few CTAs, few heads in many: one warp or four a head.  64 ragged
-        // sequences, 2048 heads: 54.2 us in all with one, 56.7 with four; 8 long ones, 128 heads: 80.3 and 72.3.
+        // Few heads are in many pieces each and get a CTA, many in few pieces a warp.  64 ragged sequences, 2048 heads:
+        // 48.7 us in all with a warp, 8 long ones, 128 heads: 60 with a CTA (80 and 72 us the other way round with an
+        // earlier join).  At most one segment a warp of the first launch is split: where there are more segments than
+        // those, a CTA looks at several.
         const int64_t units = a.batch * a.q_heads;
         const bool single = units >= 8 * (int64_t)sm_count;
-        cfg.gridDim = dim3((unsigned)(single ? (units + kJoinWarps - 1) / kJoinWarps : units));
+        const int64_t each = std::max(segments / p.parts, (int64_t)(kJoinWarps - 1) / p.group + 1);
+        p.join_segments = (int)std::min(each, (int64_t)32);
+        cfg.gridDim = dim3((unsigned)(single ? (segments + p.join_segments - 1) / p.join_segments : units));
+        if (single && each == 1) cfg.gridDim.y = (unsigned)((std::min(p.group, (int)C::rows) + kJoinWarps - 1) / kJoinWarps);
         cfg.blockDim = dim3(kJoinThreads);
         cfg.dynamicSmemBytes = 0;
         e = single ? cudaLaunchKernelEx(&cfg, cache_attention_join_kernel<D, NT, 1>, p)
