@@ -30,8 +30,8 @@
 // order, so the result does not depend on timing.
 //
 // Measured, both launches: 64 ragged sequences of up to 4096, 32 heads over 8,
-// D = 128: 48.8 us = 4.9 TB/s of cache; 8 of up to 65536, 16 heads over 2,
-// D = 256: 60 us = 5.0 TB/s; 1 of 1000: 7.7 us.  In the first, 43 us are left
+// D = 128: 49.1 us = 4.9 TB/s of cache; 8 of up to 65536, 16 heads over 2,
+// D = 256: 60 us = 5.0 TB/s; 1 of 1000: 7.9 us.  In the first, 43 us are left
 // without the arithmetic, 46 without the fetches, 45.5 without the join: a
 // warp's tile takes about 1.7 us either way, and eight warps an SM are what the
 // registers allow (12 or 16 with fewer registers, tiles of 16 positions for
@@ -40,8 +40,10 @@
 // into E4M3 pieces of 4 bits, saves the conversions of K and half of the products
 // but was no faster with two pieces (49.7 us), which do not hold every query, and
 // slower with the four that do (57.7 us; 8 of 65536: 75 us).
-// Many short sequences are bound by the change from one to the next (query,
-// lengths, output): 4096 of up to 128 positions 230 us, floor 95.
+// Many short sequences pay for the change from one to the next and for tiles
+// that end inside: 4096 of up to 128 positions 198 us, floor 95; 182 if the
+// queries cost nothing (a prefetch of them to L2 or L1 with a segment's first
+// tile gained nothing), 192 without the stores.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
