@@ -4,7 +4,7 @@ _native.so, the binding of the 4-bit and cache operators, with the host compiler
     python mxfp8-quantizer_b200/build.py [--force] [--ptxas-verbose]
 
 The library links the CUDA runtime statically and exports only the C ABI
-of include/mxfp8.h.  The checked build compiles the same sources with
+of include/mxfp8.h, mxfp4.h and mxfp8_cache.h.  The checked build compiles the same sources with
 MXFP8_CHECKED (every global store tested against its output's bytes; see
 include/mxfp8_checked.h).  nvcc cross-compiles, so this runs without a GPU.
 The binding compiles against the installed torch and calls the library by the
