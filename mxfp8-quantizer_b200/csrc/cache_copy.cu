@@ -184,8 +184,8 @@ __global__ void __launch_bounds__(kCopyThreads) cache_read_kernel(const CacheRea
             kq = __ldcs(reinterpret_cast<const uint4*>(a.k + row * a.c.dim + 16 * piece));
             vq = __ldcs(reinterpret_cast<const uint4*>(a.v + row * a.c.dim + 16 * piece));
             const int64_t s = row * (a.c.dim / 32) + (piece >> 1);
-            kb = __ldg(a.k_scales + s);
-            vb = __ldg(a.v_scales + s);
+            kb = a.k_scales[s];
+            vb = a.v_scales[s];
         }
         const int64_t at = ((row0 + r) * per_row + in) * (16 * kEs);
         widen16<OUT>(kq, kb, a.k_out + at, vec, a.kw, a.status);

@@ -227,8 +227,8 @@ __device__ __forceinline__ void store8(void* out, int64_t o, const float (&v)[8]
 
 template <int OUT>
 __global__ void __launch_bounds__(kConvertThreads) mxfp4_dequantize_kernel(
-    const uint8_t* __restrict__ q, int64_t rows, int64_t cols, int64_t ld_q, const uint8_t* __restrict__ s,
-    int64_t col_chunks, uint32_t segs, void* out, int64_t ld_out, StoreWindow ow, unsigned int* status) {
+    const uint8_t* q, int64_t rows, int64_t cols, int64_t ld_q, const uint8_t* s, int64_t col_chunks, uint32_t segs,
+    void* out, int64_t ld_out, StoreWindow ow, unsigned int* status) {
     grid_launch_dependents();
     grid_wait_prerequisites();
     const WarpUnit u = warp_unit(segs, kDequantCols);
@@ -241,8 +241,9 @@ __global__ void __launch_bounds__(kConvertThreads) mxfp4_dequantize_kernel(
         const int64_t row = u.row0 + 32 * i;
         codes[i] = row < rows ? __ldcs(reinterpret_cast<const uint32_t*>(q + row * ld_q + col / 2)) : 0u;
     }
-    const uint4 sv = __ldg(reinterpret_cast<const uint4*>(s + ((u.row0 >> 7) * col_chunks + col / 128) * 512 +
-                                                          (u.row0 & 31) * 16));
+    // not through the read-only path: the launch may begin while what writes the scales still runs
+    const uint4 sv = *reinterpret_cast<const uint4*>(s + ((u.row0 >> 7) * col_chunks + col / 128) * 512 +
+                                                     (u.row0 & 31) * 16);
     const uint32_t sw[4] = {sv.x, sv.y, sv.z, sv.w};
     constexpr int kOutBytes = OUT == MXFP8_F32 ? 4 : 2;
 #pragma unroll
