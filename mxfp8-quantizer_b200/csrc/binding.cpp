@@ -257,9 +257,9 @@ std::tuple<Tensor, Tensor> cache_read(const Tensor& ck, const Tensor& cv, const 
     TORCH_CHECK_VALUE(starts.size(0) == batch + 1, "starts must have batch + 1 = ", batch + 1, " values, got ",
                       starts.size(0));
     TORCH_CHECK_VALUE(total >= 0, "total must be >= 0, got ", total);
-    if (k_given) {
+    if (k_given || v_given) {  // both are written: one alone is refused
         for (const OptTensor* t : {&k_given, &v_given})
-            TORCH_CHECK_VALUE(*t && (*t)->dim() == 3 && (*t)->size(0) == total && (*t)->size(1) == c.heads &&
+            TORCH_CHECK_VALUE(k_given && *t && (*t)->dim() == 3 && (*t)->size(0) == total && (*t)->size(1) == c.heads &&
                                   (*t)->size(2) == c.dim && (*t)->is_contiguous() &&
                                   (*t)->scalar_type() == k_given->scalar_type(),
                               "out must be a pair of contiguous (", total, ", ", c.heads, ", ", c.dim,

@@ -1,0 +1,25 @@
+"""Calls of the 4-bit and cache operators that are refused before a device is
+touched, beside those of test_mxfp4_cpu.py and test_cache_cpu.py."""
+
+import pytest
+import torch
+
+import MXFP8_quantizer
+
+pkg = MXFP8_quantizer.load_package()
+
+
+@pytest.mark.parametrize("which", ["first missing", "second missing", "second too small", "second narrower",
+                                   "second strided", "first missing and second too small"])
+def test_read_refuses_an_output_that_is_not_a_whole_pair(which):
+    """Both outputs are written whole, so each is checked, also where the other is missing."""
+    cache = pkg.allocate_cache(4, 16, 2, 64, device="cpu")
+    table, starts = torch.zeros((3, 4), dtype=torch.int32), torch.zeros(4, dtype=torch.int32)
+    good = torch.zeros((8, 2, 64))
+    pair = {"first missing": (None, good), "second missing": (good, None), "second too small": (good, good[:7]),
+            "second narrower": (good, good.half()), "second strided": (good, torch.zeros((8, 2, 128))[:, :, ::2]),
+            "first missing and second too small": (None, good[:1].half())}[which]
+    with pytest.raises(ValueError, match="out must"):
+        pkg.cache_read(cache, table, starts, 8, out=pair)
+    with pytest.raises(ValueError, match="CUDA"):                # a whole pair gets as far as the device
+        pkg.cache_read(cache, table, starts, 8, out=(good, good.clone()))
