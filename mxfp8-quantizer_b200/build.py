@@ -32,7 +32,7 @@ SOURCES = ["capi.cu", "quantize_tma.cu", "quantize_generic.cu", "dequantize.cu",
            "capi_mxfp4.cu", "mxfp4_convert.cu", "mxfp4_gemm.cu", "capi_cache.cu", "cache_copy.cu",
            "cache_attention.cu"]
 HEADERS = ["ptx.cuh", "recipe.cuh", "launch.h", "guard.cuh", "tile.cuh", "row_path.cuh", "stores.cuh", "mxfp4.cuh",
-           "tcgen05.cuh", "cache.cuh", "cache_index.h"]
+           "tcgen05.cuh", "cache.cuh", "cache_index.h", "gemm_barriers.h"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -40,6 +40,7 @@
 #include <cstring>
 
 #include "../../include/mxfp4.h"
+#include "gemm_barriers.h"
 #include "launch.h"
 #include "ptx.cuh"
 #include "tcgen05.cuh"
@@ -70,9 +71,9 @@ struct Narrow {
     static constexpr int sf_cols = 16;
     static constexpr int cols_used = acc * BN + 2 * sf_cols;
     static constexpr int tmem_cols = cols_used <= 64 ? 64 : cols_used <= 128 ? 128 : cols_used <= 256 ? 256 : 512;
+    using Bars = GemmBarriers<stages, acc>;
     static constexpr int bar_off = stages * stage_bytes;
-    static constexpr int n_bars = 2 * stages + 2 * acc;
-    static constexpr int ctl_off = bar_off + 8 * n_bars;
+    static constexpr int ctl_off = bar_off + Bars::bytes;
     static constexpr int smem = ctl_off + 16 + 1024;            // and room to align the base to 1024
     static_assert(BN <= 128 && cols_used <= 512 && stage_bytes % 1024 == 0);
     static_assert(BN * 512 <= stages * stage_bytes, "the join of a split K holds a BN x 128 f32 tile in the stages");
@@ -89,9 +90,9 @@ struct Wide {
     static constexpr int threads = 32 * (epi_warps + 2);
     static constexpr int sf_cols = 8 + 16;
     static constexpr int tmem_cols = 512;                       // 256 + 2 * 24 of them used
+    using Bars = GemmBarriers<stages, 1>;
     static constexpr int bar_off = stages * stage_bytes;
-    static constexpr int n_bars = 2 * stages + 2;
-    static constexpr int ctl_off = bar_off + 8 * n_bars;
+    static constexpr int ctl_off = bar_off + Bars::bytes;
     static constexpr int smem = ctl_off + 16 + 1024;
     static_assert(stage_bytes % 1024 == 0 && smem <= 227 * 1024);
 };
@@ -241,8 +242,9 @@ __global__ void __launch_bounds__(Narrow<BN>::threads, 1)
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t base = smem_u32(smem);
-    const uint32_t full0 = base + C::bar_off, empty0 = full0 + 8 * C::stages;
-    const uint32_t acc_full0 = empty0 + 8 * C::stages, acc_empty0 = acc_full0 + 8 * C::acc;
+    using B = typename C::Bars;
+    const uint32_t bars = base + C::bar_off, full0 = bars + B::full(0), empty0 = bars + B::empty(0);
+    const uint32_t acc_full0 = bars + B::acc_full(0), acc_empty0 = bars + B::acc_empty(0), drained = bars + B::drained();
     volatile int* ctl = reinterpret_cast<volatile int*>(smem + C::ctl_off);  // abort, -, TMEM address
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int kLoadWarp = C::epi_warps, kMmaWarp = C::epi_warps + 1;
@@ -256,6 +258,7 @@ __global__ void __launch_bounds__(Narrow<BN>::threads, 1)
             mbar_init(acc_full0 + 8 * i, 1);
             mbar_init(acc_empty0 + 8 * i, C::epi_warps);
         }
+        mbar_init(drained, 1);
         ctl[0] = 0;
         fence_mbar_init();
     }
@@ -335,12 +338,11 @@ __global__ void __launch_bounds__(Narrow<BN>::threads, 1)
                 __syncwarp();
             }
         }
-        // an abort leaves MMAs in flight: let them end before the tensor memory goes
-        if (ctl[0]) {
-            if (elect_one()) tcgen05_commit<1>(acc_full0);
-            __syncwarp();
-            mbar_wait_bounded(acc_full0, 0, kWaitNs);
-        }
+        // the readers have waited for every tile's MMAs, unless one of them gave up: then some are still in flight,
+        // and they end before the tensor memory goes
+        if (elect_one()) tcgen05_commit<1>(drained);
+        __syncwarp();
+        mbar_wait_bounded(drained, 0, kWaitNs);
     } else {
         const int q4 = warp & 3;
         const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
@@ -433,8 +435,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide::threads, 1)
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t base = smem_u32(smem);
-    const uint32_t full0 = base + C::bar_off, empty0 = full0 + 8 * C::stages;
-    const uint32_t acc_full = empty0 + 8 * C::stages, acc_empty = acc_full + 8;
+    using B = C::Bars;
+    const uint32_t bars = base + C::bar_off, full0 = bars + B::full(0), empty0 = bars + B::empty(0);
+    const uint32_t acc_full = bars + B::acc_full(0), acc_empty = bars + B::acc_empty(0), drained = bars + B::drained();
     volatile int* ctl = reinterpret_cast<volatile int*>(smem + C::ctl_off);  // abort, -, TMEM address
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int kLoadWarp = C::epi_warps, kMmaWarp = C::epi_warps + 1;
@@ -447,6 +450,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide::threads, 1)
         }
         mbar_init(acc_full, 1);
         mbar_init(acc_empty, 2 * C::epi_warps);           // used in the even CTA: both CTAs' readers
+        mbar_init(drained, 1);                            // waited for in the even CTA, which issues for both
         ctl[0] = 0;
         fence_mbar_init();
     }
@@ -527,11 +531,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide::threads, 1)
                 __syncwarp();
             }
         }
-        // an abort leaves MMAs in flight: let them end before the tensor memory goes
-        if (rank == 0 && ctl[0]) {
-            if (elect_one()) tcgen05_commit<2>(acc_full);
+        // as in the narrow form; the other CTA frees its tensor memory after the cluster barrier that follows
+        if (rank == 0) {
+            if (elect_one()) tcgen05_commit<2>(drained);
             __syncwarp();
-            mbar_wait_bounded(acc_full, 0, kWaitNs);
+            mbar_wait_bounded(drained, 0, kWaitNs);
         }
     } else {
         // two warps for each quarter of the lanes, 128 columns each
