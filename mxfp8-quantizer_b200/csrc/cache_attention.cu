@@ -11,9 +11,13 @@
 //     (largest element in [2^14, 2^15)): a bf16 or fp16 value is exact there
 //     down to 2^-38 of the head's largest.
 //   sum_j p_j v_j: p_j 2^(sv - 127) is the operand, as p_j 2^(sv - R + 15) in
-//     f16 with R the largest V scale byte met so far: 2^-11 of relative error at
-//     most for every term within 29 binades of the largest possible one, terms
-//     below lose bits gradually; the accumulator is rescaled when R grows.
+//     f16, for the V scale bytes sv in the window R - 11 .. R: 2^-11 of relative
+//     error at most, or 2^-29 of the largest weight where f16 has no more bits.
+//     A tile whose scales span more takes several windows from its largest byte
+//     down (zero rows among small ones do: their byte is 127), each a pass over
+//     V in shared memory; the accumulator is kept in units of the latest R, and
+//     the last window, 2^64 below the largest V scale met, takes all the rest.
+//     In one R for all, 2^29 apart, the smaller columns and rows were lost.
 // The m16n8k16 shapes are used because a decode step has at most 16 rows of
 // queries: a 128-row tcgen05 tile would be empty to 7/8 and would want K and V
 // converted into shared memory first.
@@ -69,7 +73,10 @@ constexpr int kSegmentCost = 2;
 // the first launch leaves a note (meta).  1 sequence of 1000: 7.6 us, 8.0 with notes; 32 of 4096, D = 64: 24.6 and
 // 27.3; 128 of 512: 28.5 with four lengths a lane, 23.7 with notes.
 constexpr int64_t kScanBatch = 32;
-constexpr int kMinRef = 20;  // a weight times 2^(142 - R), and a tile's sum of them, stay below 2^127
+// V's scale bytes that one window takes, and how far below the largest so far a window goes: 448 2^15 of it, times as
+// many positions as there are, stays below 2^127 in units that are 2^64 smaller.  64 ragged sequences of up to 4096
+// whose scales fit a window: 50.4 us, with the windows as one loop that all tiles go through 66.
+constexpr int kWindow = 12, kReach = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr uint32_t kNoRow32 = 0xFFFFFFFFu;
@@ -590,7 +597,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
     uint32_t qf[C::query_bytes > 0 ? 1 : kBlocks][4 * NT];
     float mul[NT], m[NT], l[NT];
     float acc[NT][D / 16][4];
-    int ref = kMinRef;  // R: the largest V scale byte so far, and at least this
+    int ref = 0, peak = 0;  // R of the latest window of V's scales, and the largest so far
     auto start_segment = [&](const uint32_t (&raw)[NT][D / 8]) {
         if constexpr (C::query_bytes > 0) {
             uint32_t own[kBlocks][4 * NT];
@@ -602,7 +609,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
         } else {
             settle_query<D, NT>(p, raw, qf, mul);
         }
-        ref = kMinRef;
+        ref = peak = 0;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             m[n] = -INFINITY;
@@ -686,51 +693,9 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
                     for (int j = 0; j < 2 * NT; ++j)
                         if (!((mask >> (nt * 8 + 2 * quad + (j & 1))) & 1)) s[nt][j] = -INFINITY;
             }
-            // ---- V's scale bytes and the largest of them ----
-            uint32_t vw[kCols][kWords];
-            uint32_t odd = 0, even = 0;  // in the upper byte of each half
-#pragma unroll
-            for (int nt = 0; nt < kCols; ++nt) {
-                load_scale_pair<kBlocks>(vs + nt * 8 * kBlocks, vw[nt]);
-                if (mask != kFull) {  // an absent position may share its four bytes with one that is there
-                    uint16_t h[kBlocks];
-#pragma unroll
-                    for (int i = 0; i < kBlocks; ++i) {
-                        h[i] = (uint16_t)(vw[nt][i / 2] >> (16 * (i & 1)));
-                        if (!((mask >> (nt * 8 + 2 * quad + (i >= kWords))) & 1)) h[i] = 0;
-                    }
-#pragma unroll
-                    for (int i = 0; i < kWords; ++i) vw[nt][i] = h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
-                }
-#pragma unroll
-                for (int i = 0; i < kWords; ++i) {
-                    odd = __vmaxu2(odd, vw[nt][i]);
-                    even = __vmaxu2(even, vw[nt][i] << 8);
-                }
-            }
-            odd = __vmaxu2(odd, even);
-            int most = (int)max(odd >> 24, (odd >> 8) & 0xFFu);
-            most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
-            most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
-            if (most == 255) {  // NaN scales reach the result as they are; R is the largest of the others
-                most = 0;
-#pragma unroll
-                for (int nt = 0; nt < kCols; ++nt)
-#pragma unroll
-                    for (int i = 0; i < 4 * kWords; ++i) {
-                        const int byte = (int)((vw[nt][i / 4] >> (8 * (i & 3))) & 0xFFu);
-                        most = max(most, byte == 255 ? 0 : byte);
-                    }
-                most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
-                most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
-            }
-            const bool grown = most > ref;  // acc is in units of 2^(ref - 142)
-            const float down = grown ? exp2_fast((float)(ref - most)) : 1.0f;
-            ref = max(ref, most);
-            // ---- softmax, in log2; the weights come out times 2^(142 - ref) ----
-            const float down_l = __uint_as_float((uint32_t)(ref - 142 + 127) << 23);
+            // ---- softmax, in log2 ----
             float corr[NT];
-            bool moved = grown;
+            bool moved = false;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float top = -INFINITY;
@@ -742,19 +707,60 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
                 corr[n] = m_new > m[n] ? exp2_fast(m[n] - m_new) : 1.0f;
                 moved |= m_new > m[n];
                 m[n] = m_new;
-                const float shift = (float)(142 - ref) - m_new;
                 float sum = 0.0f;
 #pragma unroll
                 for (int nt = 0; nt < kCols; ++nt)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         float& v = s[nt][2 * n + j];
-                        v = exp2_fast(fmaf(v, mul[n], shift));
+                        v = exp2_fast(fmaf(v, mul[n], -m_new));
                         sum += v;
                     }
-                l[n] = fmaf(l[n], corr[n], sum * down_l);
+                l[n] = fmaf(l[n], corr[n], sum);
             }
-            if (__any_sync(0xFFFFFFFFu, moved)) {
+            // ---- V's scale bytes, the largest and the smallest of them ----
+            uint32_t vw[kCols][kWords];
+            uint32_t high = 0, low = 0xFFFFFFFFu;  // in the upper byte of each half
+#pragma unroll
+            for (int nt = 0; nt < kCols; ++nt) {
+                load_scale_pair<kBlocks>(vs + nt * 8 * kBlocks, vw[nt]);
+                if (mask != kFull) {  // an absent position (its weights are 0) counts with the bytes of one that is there
+                    const uint8_t* there = st + 2 * C::kv_bytes + C::sc_bytes + (__ffs(mask) - 1) * kBlocks;
+                    uint32_t h[kBlocks];
+#pragma unroll
+                    for (int i = 0; i < kBlocks; ++i) {
+                        h[i] = (vw[nt][i / 2] >> (16 * (i & 1))) & 0xFFFFu;
+                        if (!((mask >> (nt * 8 + 2 * quad + (i >= kWords))) & 1))
+                            h[i] = *reinterpret_cast<const uint16_t*>(there + 2 * (i % kWords));
+                    }
+#pragma unroll
+                    for (int i = 0; i < kWords; ++i) vw[nt][i] = h[2 * i] | (h[2 * i + 1] << 16);
+                }
+#pragma unroll
+                for (int i = 0; i < kWords; ++i) {
+                    high = __vmaxu2(__vmaxu2(high, vw[nt][i]), vw[nt][i] << 8);
+                    low = __vminu2(__vminu2(low, vw[nt][i]), vw[nt][i] << 8);
+                }
+            }
+            uint32_t ends = max((high >> 8) & 0xFFu, high >> 24) << 16 | (255u - min((low >> 8) & 0xFFu, low >> 24));
+            ends = __vmaxu2(ends, __shfl_xor_sync(0xFFFFFFFFu, ends, 1));
+            ends = __vmaxu2(ends, __shfl_xor_sync(0xFFFFFFFFu, ends, 2));
+            const int most = (int)(ends >> 16), least = 255 - (int)(ends & 0xFFFFu);
+            // the largest byte up to `bound`, 0 if there is none
+            auto largest = [&](int bound) {
+                int found = 0;
+#pragma unroll
+                for (int nt = 0; nt < kCols; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 4 * kWords; ++i) {
+                        const int byte = (int)((vw[nt][i / 4] >> (8 * (i & 3))) & 0xFFu);
+                        found = max(found, byte <= bound ? byte : 0);
+                    }
+                found = max(found, __shfl_xor_sync(0xFFFFFFFFu, found, 1));
+                return max(found, __shfl_xor_sync(0xFFFFFFFFu, found, 2));
+            };
+            // ---- second product, a window of V's scales at a time; nearly always one takes all of them ----
+            auto rescale = [&](float down) {  // from units of 2^(ref - 142) to others
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     const float c0 = __shfl_sync(0xFFFFFFFFu, corr[n], 8 * quad) * down;
@@ -767,46 +773,77 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
                         acc[n][i][3] *= c1;
                     }
                 }
-            }
-            // ---- second product: rows are elements of V, columns heads ----
-            const uint8_t* vsm = st + C::kv_bytes;
+            };
+            auto product = [&](auto factors_of) {
+                // rows are elements of V, columns heads
+                const uint8_t* vsm = st + C::kv_bytes;
 #pragma unroll
-            for (int half = 0; half < POS / 16; ++half) {
-                uint32_t f[2][kBlocks];
+                for (int half = 0; half < POS / 16; ++half) {
+                    uint32_t f[2][kBlocks];
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
+                    for (int t = 0; t < 2; ++t)
 #pragma unroll
-                    for (int i = 0; i < kWords; ++i)
-                        ue8m0x4_to_bf162(vw[2 * half + t][i], f[t][2 * i], f[t][2 * i + 1]);
+                        for (int i = 0; i < kBlocks; ++i) {  // two bytes of a word to the exponents of two bf16
+                            const uint32_t two = __byte_perm(vw[2 * half + t][i / 2], 0u, i & 1 ? 0x4342 : 0x4140);
+                            f[t][i] = factors_of(two);
+                        }
 #pragma unroll
-                for (int blk = 0; blk < kBlocks; ++blk) {
-                    uint32_t pb[NT][2];
+                    for (int blk = 0; blk < kBlocks; ++blk) {
+                        uint32_t pb[NT][2];
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        const uint32_t f0 = f[t][blk / 2], f1 = f[t][kWords + blk / 2];
-                        const float fx = __uint_as_float(blk & 1 ? f0 & 0xFFFF0000u : f0 << 16);
-                        const float fy = __uint_as_float(blk & 1 ? f1 & 0xFFFF0000u : f1 << 16);
+                        for (int t = 0; t < 2; ++t) {
+                            const uint32_t f0 = f[t][blk / 2], f1 = f[t][kWords + blk / 2];
+                            const float fx = __uint_as_float(blk & 1 ? f0 & 0xFFFF0000u : f0 << 16);
+                            const float fy = __uint_as_float(blk & 1 ? f1 & 0xFFFF0000u : f1 << 16);
 #pragma unroll
-                        for (int n = 0; n < NT; ++n)
-                            pb[n][t] = pack_half2(s[2 * half + t][2 * n] * fx, s[2 * half + t][2 * n + 1] * fy);
+                            for (int n = 0; n < NT; ++n)
+                                pb[n][t] = pack_half2(s[2 * half + t][2 * n] * fx, s[2 * half + t][2 * n + 1] * fy);
+                        }
+                        // positions 2 quad, 2 quad + 1, 8 + 2 quad, 9 + 2 quad; elements 4 row .. 4 row + 3 of the block
+                        uint32_t w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            w[i] = *reinterpret_cast<const uint32_t*>(
+                                vsm + in_block<D>(v_at, blk) + (16 * half + 4 * (i >> 1) + 8 * (i & 1)) * D);
+                        uint32_t h[2][4];  // [positions low or high][element]: pairs of neighbouring positions
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            e4m3x4_to_half2(__byte_perm(w[2 * i], w[2 * i + 1], 0x5140), h[i][0], h[i][1]);
+                            e4m3x4_to_half2(__byte_perm(w[2 * i], w[2 * i + 1], 0x7362), h[i][2], h[i][3]);
+                        }
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            mma_f16(acc[n][2 * blk], h[0][0], h[0][1], h[1][0], h[1][1], pb[n][0], pb[n][1]);
+                            mma_f16(acc[n][2 * blk + 1], h[0][2], h[0][3], h[1][2], h[1][3], pb[n][0], pb[n][1]);
+                        }
                     }
-                    // positions 2 quad, 2 quad + 1, 8 + 2 quad, 9 + 2 quad; elements 4 row .. 4 row + 3 of the block
-                    uint32_t w[4];
+                }
+            };
+            const int upper = max(ref, most);  // R, if all scales are in its window
+            if (most < 255 && least > upper - kWindow) {
+                if (__any_sync(0xFFFFFFFFu, moved || upper != ref)) rescale(exp2_fast((float)(ref - upper)));
+                ref = upper;
+                peak = max(peak, ref);
+                const uint32_t shift = (uint32_t)(142 - ref) * 0x00800080u;
+                product([&](uint32_t two) { return two * 128u + shift; });
+            } else {
+                int bound = 254;  // the largest byte that is left; NaN goes with the first window
+                for (bool first = true;; first = false) {
+                    int r = max(largest(bound), peak - kReach);
+                    peak = max(peak, r);
+                    rescale(exp2_fast((float)(ref - r)));
+                    ref = r;
+                    const bool last = least > ref - kWindow || ref <= peak - kReach;
+                    auto factor = [&](uint32_t byte) {
+                        const int e = (int)byte + 142 - ref;
+                        const bool in = (int)byte <= bound && ((int)byte > ref - kWindow || ref <= peak - kReach);
+                        return byte == 255u ? (first ? 0x7FC0u : 0u) : in && e > 0 ? (uint32_t)e << 7 : 0u;
+                    };
+                    product([&](uint32_t two) { return factor(two & 0xFFu) | factor(two >> 16) << 16; });
+                    if (last) break;
+                    bound = ref - kWindow;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        w[i] = *reinterpret_cast<const uint32_t*>(
-                            vsm + in_block<D>(v_at, blk) + (16 * half + 4 * (i >> 1) + 8 * (i & 1)) * D);
-                    uint32_t h[2][4];  // [positions low or high][element]: pairs of neighbouring positions
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        e4m3x4_to_half2(__byte_perm(w[2 * i], w[2 * i + 1], 0x5140), h[i][0], h[i][1]);
-                        e4m3x4_to_half2(__byte_perm(w[2 * i], w[2 * i + 1], 0x7362), h[i][2], h[i][3]);
-                    }
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        mma_f16(acc[n][2 * blk], h[0][0], h[0][1], h[1][0], h[1][1], pb[n][0], pb[n][1]);
-                        mma_f16(acc[n][2 * blk + 1], h[0][2], h[0][3], h[1][2], h[1][3], pb[n][0], pb[n][1]);
-                    }
+                    for (int n = 0; n < NT; ++n) corr[n] = 1.0f;
                 }
             }
         }
