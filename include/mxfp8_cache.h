@@ -77,10 +77,9 @@ MXFP8_API int64_t mxfp8_cache_attention_workspace(const mxfp8_cache* cache, int6
  * 2^34.  A length of 0 (or below) gives zeros and lse -inf; a position whose
  * page is outside the cache takes no part, as if it were not there, and is
  * reported; a length past the table is cut to it and reported.  Scores and sums
- * are held in f32; a weight is held to 2^-11 of itself or 2^-29 of the largest
- * one, whichever is more, whatever the scales of V's other blocks are (a block
- * whose scale is more than 2^64 below the largest one of its sequence and head
- * counts with at least 2^-104 of that scale); outputs are rounded once.  A score
+ * are held in f32; a weight is held to 2^-22 of itself or 2^-28 of the largest
+ * one, whichever is more, whatever the scales of V's blocks are (V more than
+ * 2^70 below its head's sums so far counts as zero); outputs are rounded once.  A score
  * overflows where a K block's scale is 2^96 or more (the query is held with its
  * largest element near 2^14).  workspace is 16-byte aligned scratch of
  * one call at a time; its contents do not matter before or after. */

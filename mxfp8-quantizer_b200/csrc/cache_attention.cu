@@ -10,14 +10,15 @@
 //     block scaled in f32.  q is brought to f16 with one power of two a head
 //     (largest element in [2^14, 2^15)): a bf16 or fp16 value is exact there
 //     down to 2^-38 of the head's largest.
-//   sum_j p_j v_j: p_j 2^(sv - 127) is the operand, as p_j 2^(sv - R + 15) in
-//     f16, for the V scale bytes sv in the window R - 11 .. R: 2^-11 of relative
-//     error at most, or 2^-29 of the largest weight where f16 has no more bits.
+//   sum_j p_j v_j: the operand is p_j 2^(sv - R + 15), for the V scale bytes sv
+//     in the window R - 11 .. R.  It is two f16, p_j 2^15 and what that leaves,
+//     each times the power of two: 2^-22 of relative error at most, or 2^-28 of
+//     the largest weight where f16 has no more bits.  (One f16, 2^-11, was 3 %
+//     faster and showed in fp16 outputs and in one bf16 output of thirty.)
 //     A tile whose scales span more takes several windows from its largest byte
-//     down (zero rows among small ones do: their byte is 127), each a pass over
-//     V in shared memory; the accumulator is kept in units of the latest R, and
-//     the last window, 2^64 below the largest V scale met, takes all the rest.
-//     In one R for all, 2^29 apart, the smaller columns and rows were lost.
+//     down, each a pass over V in shared memory (zero rows among small ones do:
+//     their byte is 127); the accumulator is kept in units of the latest R.
+//     With one R for all, columns and rows 2^29 below the largest were lost.
 // The m16n8k16 shapes are used because a decode step has at most 16 rows of
 // queries: a 128-row tcgen05 tile would be empty to 7/8 and would want K and V
 // converted into shared memory first.
@@ -34,9 +35,10 @@
 // order, so the result does not depend on timing.
 //
 // Measured, both launches: 64 ragged sequences of up to 4096, 32 heads over 8,
-// D = 128: 49.1 us = 4.9 TB/s of cache; 8 of up to 65536, 16 heads over 2,
-// D = 256: 60 us = 5.0 TB/s; 1 of 1000: 7.9 us.  In the first, 43 us are left
-// without the arithmetic, 46 without the fetches, 45.5 without the join: a
+// D = 128: 50.3 us = 4.8 TB/s of cache; 8 of up to 65536, 16 heads over 2,
+// D = 256: 61.3 us = 4.9 TB/s; 1 of 1000: 7.9 us.  With weights of one f16 the
+// first took 49.1, of which 43 us were left without the arithmetic, 46 without
+// the fetches, 45.5 without the join: a
 // warp's tile takes about 1.7 us either way, and eight warps an SM are what the
 // registers allow (12 or 16 with fewer registers, tiles of 16 positions for
 // D <= 128, a third stage for D = 256: all slower).  Half of the issue slots are
@@ -45,7 +47,8 @@
 // but was no faster with two pieces (49.7 us), which do not hold every query, and
 // slower with the four that do (57.7 us; 8 of 65536: 75 us).
 // Many short sequences pay for the change from one to the next and for tiles
-// that end inside: 4096 of up to 128 positions 198 us, floor 95; 182 if the
+// that end inside: 4096 of up to 128 positions 210 us, floor 95; 12 of them are
+// the second f16 and the scales of absent positions.  Before those, 182 if the
 // queries cost nothing (a prefetch of them to L2 or L1 with a segment's first
 // tile gained nothing), 192 without the stores.
 #include <cuda_bf16.h>
@@ -73,10 +76,10 @@ constexpr int kSegmentCost = 2;
 // the first launch leaves a note (meta).  1 sequence of 1000: 7.6 us, 8.0 with notes; 32 of 4096, D = 64: 24.6 and
 // 27.3; 128 of 512: 28.5 with four lengths a lane, 23.7 with notes.
 constexpr int64_t kScanBatch = 32;
-// V's scale bytes that one window takes, and how far below the largest so far a window goes: 448 2^15 of it, times as
-// many positions as there are, stays below 2^127 in units that are 2^64 smaller.  64 ragged sequences of up to 4096
-// whose scales fit a window: 50.4 us, with the windows as one loop that all tiles go through 66.
-constexpr int kWindow = 12, kReach = 64;
+// V's scale bytes that one window takes: 2^(sv - R) is an f16 with three binades to spare, and p_j 2^15 keeps its bits
+// down to p_j = 2^-18.  A tile's windows are a loop around the second product that is left after one turn; a copy of the
+// product for tiles with several was as fast where it fitted the registers and 2 to 6 % slower where it did not.
+constexpr int kWindow = 12;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr uint32_t kNoRow32 = 0xFFFFFFFFu;
@@ -268,6 +271,10 @@ __device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32
 
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     const __half2 t = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&t);
+}
+__device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
+    const __half2 t = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&t);
 }
 __device__ __forceinline__ uint32_t pack_out(bool bf16, float lo, float hi) {
@@ -485,6 +492,48 @@ __device__ __forceinline__ void load_scale_pair(const uint8_t* src, uint32_t (&w
     for (int i = 0; i < NB / 2; ++i) w[i] = reinterpret_cast<const uint32_t*>(src)[i];
 }
 
+// The next window of a tile's V scales, from the largest byte up to `left` down, but not below `floor`: the tile's scales
+// in shared memory are replaced by the window's own, the others by a byte whose factor is a zero; NaN blocks (in the
+// first window, left = 254) by payloads of NaN.  The scales as they were are kept in the place of K's, which are used
+// up.  Returns R; `left` becomes the largest byte that the next window may take, or -1.  `least` is the tile's smallest.
+template <int D, int POS>
+__device__ __forceinline__ int take_window(uint8_t* st, int lane, int floor, int least, int& left) {
+    constexpr int kKv = POS * D, kWords = D / 64;
+    uint16_t* const kept = reinterpret_cast<uint16_t*>(st + 2 * kKv) + lane * kWords;
+    uint16_t* const used = kept + kKv / 64;
+    const bool first = left == 254;
+    int upper = floor;
+    __syncwarp();  // everyone has read what is replaced here
+    if (lane < POS) {
+        for (int i = 0; i < 2 * kWords; ++i) {
+            if (first && (i & 1) == 0) kept[i / 2] = used[i / 2];
+            const int byte = (kept[i / 2] >> (8 * (i & 1))) & 0xFF;
+            if (byte <= left) upper = max(upper, byte);
+        }
+    }
+    upper = __reduce_max_sync(0xFFFFFFFFu, upper);
+    const bool last = least > upper - kWindow || upper == floor;  // the lowest window has no lower end
+    const int zero = upper < 15 ? upper + 17 : upper - 15;        // (byte + 15 - R) << 10 is an f16 zero, of either sign
+    if (lane < POS) {
+        for (int i = 0; i < kWords; ++i) {
+            int two = 0;
+            for (int h = 0; h < 2; ++h) {
+                const int byte = (kept[i] >> (8 * h)) & 0xFF;
+                const bool in = byte <= left && byte + 15 >= upper && (last || byte > upper - kWindow);
+                two |= (in ? byte : zero) << (8 * h);
+                if (first && byte == 255) {
+                    uint4* const row = reinterpret_cast<uint4*>(st + kKv + group_at<D>(v_place(lane), 2 * i + h));
+                    row[0] = row[1] = make_uint4(0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+                }
+            }
+            used[i] = (uint16_t)two;
+        }
+    }
+    __syncwarp();
+    left = last ? -1 : upper - kWindow;
+    return upper;
+}
+
 // A warp's piece of a segment to a slot of the workspace: rows as in the
 // scores (8 n + row) for m and l, as in acc (8 n + 2 quad + {0, 1}) for the sums.
 template <int D, int NT>
@@ -597,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
     uint32_t qf[C::query_bytes > 0 ? 1 : kBlocks][4 * NT];
     float mul[NT], m[NT], l[NT];
     float acc[NT][D / 16][4];
-    int ref = 0, peak = 0;  // R of the latest window of V's scales, and the largest so far
+    int ref = 0;  // R of the latest window of V's scales
     auto start_segment = [&](const uint32_t (&raw)[NT][D / 8]) {
         if constexpr (C::query_bytes > 0) {
             uint32_t own[kBlocks][4 * NT];
@@ -609,7 +658,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
         } else {
             settle_query<D, NT>(p, raw, qf, mul);
         }
-        ref = peak = 0;
+        ref = 0;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             m[n] = -INFINITY;
@@ -628,8 +677,16 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
         __syncwarp();  // also: the stage before this one is read, it can be filled again
         const uint32_t mask = __shfl_sync(0xFFFFFFFFu, present, stage);
         issue(stage == 0 ? C::stages - 1 : stage - 1);
-        const uint8_t* st = ring + stage * C::stage_bytes;
+        uint8_t* const st = ring + stage * C::stage_bytes;
         if (mask != 0) {
+            if (mask != kFull) {  // an absent position (its weights are 0) gets the V scales of one that is there
+                uint16_t* const scales = reinterpret_cast<uint16_t*>(st + 2 * C::kv_bytes + C::sc_bytes);
+                if (lane < POS && !((mask >> lane) & 1)) {
+#pragma unroll
+                    for (int i = 0; i < kWords; ++i) scales[lane * kWords + i] = scales[(__ffs(mask) - 1) * kWords + i];
+                }
+                __syncwarp();
+            }
             const uint8_t* ks = st + 2 * C::kv_bytes + quad * (2 * kBlocks);
             const uint8_t* vs = ks + C::sc_bytes;
             // ---- scores: rows are heads, columns positions 8 nt + 2 quad + {0, 1} ----
@@ -718,24 +775,23 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
                     }
                 l[n] = fmaf(l[n], corr[n], sum);
             }
+            // ---- the weights times 2^15 as two f16 each, neighbouring positions in a pair: the value, and what it leaves ----
+            uint32_t ph[kCols][NT], pl[kCols][NT];
+#pragma unroll
+            for (int nt = 0; nt < kCols; ++nt)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const float x = s[nt][2 * n] * 32768.0f, y = s[nt][2 * n + 1] * 32768.0f;
+                    ph[nt][n] = pack_half2(x, y);
+                    const float2 held = __half22float2(*reinterpret_cast<const __half2*>(&ph[nt][n]));
+                    pl[nt][n] = pack_half2(x - held.x, y - held.y);
+                }
             // ---- V's scale bytes, the largest and the smallest of them ----
             uint32_t vw[kCols][kWords];
             uint32_t high = 0, low = 0xFFFFFFFFu;  // in the upper byte of each half
 #pragma unroll
             for (int nt = 0; nt < kCols; ++nt) {
                 load_scale_pair<kBlocks>(vs + nt * 8 * kBlocks, vw[nt]);
-                if (mask != kFull) {  // an absent position (its weights are 0) counts with the bytes of one that is there
-                    const uint8_t* there = st + 2 * C::kv_bytes + C::sc_bytes + (__ffs(mask) - 1) * kBlocks;
-                    uint32_t h[kBlocks];
-#pragma unroll
-                    for (int i = 0; i < kBlocks; ++i) {
-                        h[i] = (vw[nt][i / 2] >> (16 * (i & 1))) & 0xFFFFu;
-                        if (!((mask >> (nt * 8 + 2 * quad + (i >= kWords))) & 1))
-                            h[i] = *reinterpret_cast<const uint16_t*>(there + 2 * (i % kWords));
-                    }
-#pragma unroll
-                    for (int i = 0; i < kWords; ++i) vw[nt][i] = h[2 * i] | (h[2 * i + 1] << 16);
-                }
 #pragma unroll
                 for (int i = 0; i < kWords; ++i) {
                     high = __vmaxu2(__vmaxu2(high, vw[nt][i]), vw[nt][i] << 8);
@@ -746,35 +802,42 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
             ends = __vmaxu2(ends, __shfl_xor_sync(0xFFFFFFFFu, ends, 1));
             ends = __vmaxu2(ends, __shfl_xor_sync(0xFFFFFFFFu, ends, 2));
             const int most = (int)(ends >> 16), least = 255 - (int)(ends & 0xFFFFu);
-            // the largest byte up to `bound`, 0 if there is none
-            auto largest = [&](int bound) {
-                int found = 0;
-#pragma unroll
-                for (int nt = 0; nt < kCols; ++nt)
-#pragma unroll
-                    for (int i = 0; i < 4 * kWords; ++i) {
-                        const int byte = (int)((vw[nt][i / 4] >> (8 * (i & 3))) & 0xFFu);
-                        found = max(found, byte <= bound ? byte : 0);
-                    }
-                found = max(found, __shfl_xor_sync(0xFFFFFFFFu, found, 1));
-                return max(found, __shfl_xor_sync(0xFFFFFFFFu, found, 2));
-            };
             // ---- second product, a window of V's scales at a time; nearly always one takes all of them ----
-            auto rescale = [&](float down) {  // from units of 2^(ref - 142) to others
+            int upper = max(ref, most);  // R
+            int left = most < 255 && least > upper - kWindow ? -1 : 254;  // the largest byte that is still to be taken
+            for (;;) {
+                if (left >= 0) {
+                    // acc, where it is not 0 yet, stays below 2^126 in the units of the lowest R
+                    float size = 0.0f;
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const float c0 = __shfl_sync(0xFFFFFFFFu, corr[n], 8 * quad) * down;
-                    const float c1 = __shfl_sync(0xFFFFFFFFu, corr[n], 8 * quad + 4) * down;
+                    for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int i = 0; i < D / 16; ++i) {
-                        acc[n][i][0] *= c0;
-                        acc[n][i][1] *= c1;
-                        acc[n][i][2] *= c0;
-                        acc[n][i][3] *= c1;
+                        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) size = fmaxf(size, fabsf(acc[n][i][j]));
+                    const uint32_t bits = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(size));
+                    const int room = bits == 0 ? ref : min(max(252 - (int)(bits >> 23), 0), 126);
+                    upper = take_window<D, POS>(st, lane, max(ref - room, 0), least, left);
+#pragma unroll
+                    for (int nt = 0; nt < kCols; ++nt) load_scale_pair<kBlocks>(vs + nt * 8 * kBlocks, vw[nt]);
+                }
+                if (__any_sync(0xFFFFFFFFu, moved || upper != ref)) {  // acc is in units of 2^(ref - 142)
+                    const float down = exp2_fast((float)min(ref - upper, 126));
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const float c0 = __shfl_sync(0xFFFFFFFFu, corr[n], 8 * quad) * down;
+                        const float c1 = __shfl_sync(0xFFFFFFFFu, corr[n], 8 * quad + 4) * down;
+#pragma unroll
+                        for (int i = 0; i < D / 16; ++i) {
+                            acc[n][i][0] *= c0;
+                            acc[n][i][1] *= c1;
+                            acc[n][i][2] *= c0;
+                            acc[n][i][3] *= c1;
+                        }
                     }
                 }
-            };
-            auto product = [&](auto factors_of) {
+                ref = upper;
+                const uint32_t shift = (uint32_t)(15 - ref) * 0x04000400u;
                 // rows are elements of V, columns heads
                 const uint8_t* vsm = st + C::kv_bytes;
 #pragma unroll
@@ -783,21 +846,21 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
 #pragma unroll
-                        for (int i = 0; i < kBlocks; ++i) {  // two bytes of a word to the exponents of two bf16
+                        for (int i = 0; i < kBlocks; ++i) {  // two bytes of a word to the exponents of two f16
                             const uint32_t two = __byte_perm(vw[2 * half + t][i / 2], 0u, i & 1 ? 0x4342 : 0x4140);
-                            f[t][i] = factors_of(two);
+                            f[t][i] = two * 1024u + shift;
                         }
 #pragma unroll
                     for (int blk = 0; blk < kBlocks; ++blk) {
-                        uint32_t pb[NT][2];
+                        uint32_t pb[NT][2], rest[NT][2];
 #pragma unroll
                         for (int t = 0; t < 2; ++t) {
-                            const uint32_t f0 = f[t][blk / 2], f1 = f[t][kWords + blk / 2];
-                            const float fx = __uint_as_float(blk & 1 ? f0 & 0xFFFF0000u : f0 << 16);
-                            const float fy = __uint_as_float(blk & 1 ? f1 & 0xFFFF0000u : f1 << 16);
+                            const uint32_t by = __byte_perm(f[t][blk / 2], f[t][kWords + blk / 2], blk & 1 ? 0x7632 : 0x5410);
 #pragma unroll
-                            for (int n = 0; n < NT; ++n)
-                                pb[n][t] = pack_half2(s[2 * half + t][2 * n] * fx, s[2 * half + t][2 * n + 1] * fy);
+                            for (int n = 0; n < NT; ++n) {
+                                pb[n][t] = mul_half2(ph[2 * half + t][n], by);
+                                rest[n][t] = mul_half2(pl[2 * half + t][n], by);
+                            }
                         }
                         // positions 2 quad, 2 quad + 1, 8 + 2 quad, 9 + 2 quad; elements 4 row .. 4 row + 3 of the block
                         uint32_t w[4];
@@ -815,36 +878,15 @@ __global__ void __launch_bounds__(kThreads, Config<D, NT>::ctas_per_sm) cache_at
                         for (int n = 0; n < NT; ++n) {
                             mma_f16(acc[n][2 * blk], h[0][0], h[0][1], h[1][0], h[1][1], pb[n][0], pb[n][1]);
                             mma_f16(acc[n][2 * blk + 1], h[0][2], h[0][3], h[1][2], h[1][3], pb[n][0], pb[n][1]);
+                            mma_f16(acc[n][2 * blk], h[0][0], h[0][1], h[1][0], h[1][1], rest[n][0], rest[n][1]);
+                            mma_f16(acc[n][2 * blk + 1], h[0][2], h[0][3], h[1][2], h[1][3], rest[n][0], rest[n][1]);
                         }
                     }
                 }
-            };
-            const int upper = max(ref, most);  // R, if all scales are in its window
-            if (most < 255 && least > upper - kWindow) {
-                if (__any_sync(0xFFFFFFFFu, moved || upper != ref)) rescale(exp2_fast((float)(ref - upper)));
-                ref = upper;
-                peak = max(peak, ref);
-                const uint32_t shift = (uint32_t)(142 - ref) * 0x00800080u;
-                product([&](uint32_t two) { return two * 128u + shift; });
-            } else {
-                int bound = 254;  // the largest byte that is left; NaN goes with the first window
-                for (bool first = true;; first = false) {
-                    int r = max(largest(bound), peak - kReach);
-                    peak = max(peak, r);
-                    rescale(exp2_fast((float)(ref - r)));
-                    ref = r;
-                    const bool last = least > ref - kWindow || ref <= peak - kReach;
-                    auto factor = [&](uint32_t byte) {
-                        const int e = (int)byte + 142 - ref;
-                        const bool in = (int)byte <= bound && ((int)byte > ref - kWindow || ref <= peak - kReach);
-                        return byte == 255u ? (first ? 0x7FC0u : 0u) : in && e > 0 ? (uint32_t)e << 7 : 0u;
-                    };
-                    product([&](uint32_t two) { return factor(two & 0xFFu) | factor(two >> 16) << 16; });
-                    if (last) break;
-                    bound = ref - kWindow;
+                if (left < 0) break;
+                moved = false;
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) corr[n] = 1.0f;
-                }
+                for (int n = 0; n < NT; ++n) corr[n] = 1.0f;
             }
         }
         stage = stage + 1 == C::stages ? 0 : stage + 1;

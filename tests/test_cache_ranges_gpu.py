@@ -135,3 +135,15 @@ def test_windows_do_not_depend_on_what_is_absent():
         cache.v_scales[table[1, 2].long(), :, 5:] = byte
         for a, b in zip(pkg.cache_attention(q, cache, table, lens, return_lse=True), want):
             assert torch.equal(a, b)
+
+
+def test_a_scale_without_a_payload_takes_nothing():
+    """Zero payloads under the largest scale beside ordinary rows and very small ones, in one tile."""
+    lengths = [32, 100]
+    q, cache, table = attention_case(lengths, 16, 1, 4, 64, "bf16", seed=12)
+    for low in (127, 60, 20, 5):
+        cache.v_scales.fill_(low)
+        at = table[:, 0].long()
+        raw(cache.v)[at, :, 3:9] = 0
+        cache.v_scales[at, :, 3:9] = 254
+        check_elements(q, cache, table, lengths, 16)
