@@ -56,7 +56,6 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <atomic>
 
 #include "../../include/mxfp8_cache.h"
 #include "cache.cuh"
@@ -1182,22 +1181,8 @@ template <int D, int NT>
 int launch_typed(const CacheAttentionArgs& a, int sm_count, cudaStream_t stream) {
     using C = Config<D, NT>;
     auto kernel = cache_attention_kernel<D, NT>;
-    // once per device: later launches, captured ones among them, make no such call
-    static std::atomic<uint64_t> attr_set{0};
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    const uint64_t bit = 1ull << (dev & 63);
-    if (e == cudaSuccess && !(attr_set.load(std::memory_order_acquire) & bit)) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem);
-        if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
-                                     (int)cudaSharedmemCarveoutMaxShared);
-        if (e == cudaSuccess) attr_set.fetch_or(bit, std::memory_order_acq_rel);
-    }
-    if (e != cudaSuccess) {
-        set_last_error("cudaFuncSetAttribute", (int)e);
-        return MXFP8_ERR_CUDA;
-    }
+    static OptIn done;
+    if (int rc = opt_in(reinterpret_cast<const void*>(kernel), C::smem, true, done)) return rc;
     Params p;
     p.a = a;
     p.group = a.q_heads / a.c.heads;
@@ -1223,7 +1208,7 @@ int launch_typed(const CacheAttentionArgs& a, int sm_count, cudaStream_t stream)
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = C::smem;
-    e = cudaLaunchKernelEx(&cfg, kernel, p);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
     if (e == cudaSuccess) {
         // Few heads are in many pieces each and get a CTA, many in few pieces a warp.  64 ragged sequences, 2048 heads:
         // 48.7 us in all with a warp, 8 long ones, 128 heads: 60 with a CTA (80 and 72 us the other way round with an

@@ -18,7 +18,6 @@ namespace mxfp8 {
 
 namespace {
 
-constexpr int kMaxDevices = 64;
 constexpr int64_t kInt32Max = 2147483647;
 
 struct DeviceState {
@@ -206,6 +205,28 @@ int bound_context_key(uint64_t* key) {
         set_last_error("no CUDA context is current", 0);
         return MXFP8_ERR_DEVICE;
     }
+    return MXFP8_OK;
+}
+
+int opt_in(const void* kernel, int smem, bool most_shared, OptIn& done) {
+    int dev = -1;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || dev < 0 || dev >= kMaxDevices) {
+        set_last_error("cudaGetDevice", (int)e);
+        return MXFP8_ERR_DEVICE;
+    }
+    uint64_t ctx = 0;
+    if (int rc = bound_context_key(&ctx)) return rc;
+    if (done.ctx[dev].load(std::memory_order_acquire) == ctx) return MXFP8_OK;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess && most_shared)
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                 (int)cudaSharedmemCarveoutMaxShared);
+    if (e != cudaSuccess) {
+        set_last_error("cudaFuncSetAttribute", (int)e);
+        return MXFP8_ERR_CUDA;
+    }
+    done.ctx[dev].store(ctx, std::memory_order_release);
     return MXFP8_OK;
 }
 

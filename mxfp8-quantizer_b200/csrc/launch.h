@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "guard.cuh"
 
 namespace mxfp8 {
@@ -93,6 +95,15 @@ void set_last_error(const char* what, int code);
 // success).  Per-device caches compare it to notice a new context.
 int context_key(uint64_t* key);
 int bound_context_key(uint64_t* key);
+
+// A kernel's opt-in to `smem` bytes of dynamic shared memory, and with `most_shared` to the largest share of the SM's
+// memory.  It belongs to a context: made by the kernel's first launch in one, so that later launches, captured ones
+// among them, make no such call.  `done` is the kernel's own, static; 0 or a negative mxfp8_status.
+constexpr int kMaxDevices = 64;
+struct OptIn {
+    std::atomic<uint64_t> ctx[kMaxDevices];  // context_key() of the context it was made in last
+};
+int opt_in(const void* kernel, int smem, bool most_shared, OptIn& done);
 
 // Device address of the allocation-free entries' status word (a fixed device
 // array of quantize_tma.cu) on device `dev`, the current device.

@@ -36,7 +36,6 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
-#include <atomic>
 #include <cstring>
 
 #include "../../include/mxfp4.h"
@@ -619,20 +618,6 @@ int encode_scales(CUtensorMap* map, const Fp4Operand& m, int64_t k, int box_bloc
                       2 * (kChunk / 4), (uint32_t)box_blocks, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
-// A kernel's shared memory opt-in, once per device: later launches, captured
-// ones among them, make no such call.
-template <typename K>
-cudaError_t opt_in(K* kernel, int smem, std::atomic<uint64_t>& done) {
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    const uint64_t bit = 1ull << (dev & 63);
-    if (e == cudaSuccess && !(done.load(std::memory_order_acquire) & bit)) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_acq_rel);
-    }
-    return e;
-}
-
 int launch_failed(const char* what, cudaError_t e) {
     set_last_error(what, (int)e);
     return MXFP8_ERR_CUDA;
@@ -660,12 +645,11 @@ GemmParams params_of(const Fp4GemmArgs& g, const Fp4Operand& P, const Fp4Operand
 template <int OUT, bool ACROSS>
 int launch_wide(const Fp4GemmArgs& g, int sm_count, cudaStream_t stream) {
     using C = Wide;
-    static std::atomic<uint64_t> done{0};
+    static OptIn done;
     auto kernel = mxfp4_gemm_wide_kernel<OUT, ACROSS>;
     const Fp4Operand& P = ACROSS ? g.b : g.a;
     const Fp4Operand& Q = ACROSS ? g.a : g.b;
-    cudaError_t e = opt_in(kernel, C::smem, done);
-    if (e != cudaSuccess) return launch_failed("cudaFuncSetAttribute", e);
+    if (int rc = opt_in(reinterpret_cast<const void*>(kernel), C::smem, false, done)) return rc;
     CUtensorMap map_p, map_q, map_sp, map_sq;
     if (int rc = encode_payload(&map_p, P, g.k, kTileP)) return rc;
     if (int rc = encode_payload(&map_q, Q, g.k, C::bn / 2)) return rc;
@@ -683,7 +667,7 @@ int launch_wide(const Fp4GemmArgs& g, int sm_count, cudaStream_t stream) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kernel, map_p, map_q, map_sp, map_sq, p);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, map_p, map_q, map_sp, map_sq, p);
     if (e == cudaSuccess) e = cudaGetLastError();
     return e == cudaSuccess ? MXFP8_OK : launch_failed("mxfp4_gemm_wide_kernel launch", e);
 }
@@ -699,10 +683,9 @@ int narrow_split(int64_t tiles, int n_stages, int sm_count) {
 template <int BN, int OUT>
 int launch_narrow(const Fp4GemmArgs& g, int sm_count, cudaStream_t stream) {
     using C = Narrow<BN>;
-    static std::atomic<uint64_t> done{0};
+    static OptIn done;
     auto kernel = mxfp4_gemm_narrow_kernel<BN, OUT>;
-    cudaError_t e = opt_in(kernel, C::smem, done);
-    if (e != cudaSuccess) return launch_failed("cudaFuncSetAttribute", e);
+    if (int rc = opt_in(reinterpret_cast<const void*>(kernel), C::smem, false, done)) return rc;
     CUtensorMap map_p, map_q;
     if (int rc = encode_payload(&map_p, g.b, g.k, kTileP)) return rc;
     if (int rc = encode_payload(&map_q, g.a, g.k, BN)) return rc;
@@ -722,7 +705,7 @@ int launch_narrow(const Fp4GemmArgs& g, int sm_count, cudaStream_t stream) {
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = p.split > 1 ? 2 : 1;
-    e = cudaLaunchKernelEx(&cfg, kernel, map_p, map_q, p);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, map_p, map_q, p);
     if (e == cudaSuccess) e = cudaGetLastError();
     return e == cudaSuccess ? MXFP8_OK : launch_failed("mxfp4_gemm_narrow_kernel launch", e);
 }

@@ -59,7 +59,6 @@
 #include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 
-#include <atomic>
 #include <cstring>
 #include <mutex>
 
@@ -397,23 +396,8 @@ static int launch_tma_typed(const QuantizeArgs& a, int sm_count, cudaStream_t st
     constexpr int kCtasPerSm = (ROWS || QU) ? kRowCtasPerSm : 1;
     using L = Layout<kSt, ROWS>;
     auto kernel = quantize_tma_kernel<DT, kSt, ROWS, QU, QW>;
-    // The shared-memory opt-in is per device: set it once per device, so that
-    // later launches (including ones under stream capture) make no such call.
-    static std::atomic<uint64_t> attr_set{0};
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    const uint64_t bit = 1ull << (dev & 63);
-    if (e == cudaSuccess && !(attr_set.load(std::memory_order_acquire) & bit)) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::alloc);
-        if (e == cudaSuccess && (ROWS || QU))
-            e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
-                                     (int)cudaSharedmemCarveoutMaxShared);
-        if (e == cudaSuccess) attr_set.fetch_or(bit, std::memory_order_acq_rel);
-    }
-    if (e != cudaSuccess) {
-        set_last_error("cudaFuncSetAttribute", (int)e);
-        return MXFP8_ERR_CUDA;
-    }
+    static OptIn done;
+    if (int rc = opt_in(reinterpret_cast<const void*>(kernel), L::alloc, ROWS || QU, done)) return rc;
     XMaps<ROWS> xm;
     int rc = encode_x_maps<ROWS>(a, xm);
     if (rc) return rc;
@@ -447,6 +431,7 @@ static int launch_tma_typed(const QuantizeArgs& a, int sm_count, cudaStream_t st
         rows_per_launch = max_tiles / a.col_chunks;
         if (rows_per_launch < 1) rows_per_launch = 1;
     }
+    cudaError_t e = cudaSuccess;
     for (int64_t r0 = 0; r0 < n_row_tiles && e == cudaSuccess; r0 += rows_per_launch) {
         const int64_t nr = n_row_tiles - r0 < rows_per_launch ? n_row_tiles - r0 : rows_per_launch;
         p.rt_offset = (int)r0;
