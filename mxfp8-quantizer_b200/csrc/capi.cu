@@ -266,6 +266,8 @@ int read_status_word(unsigned int* word, uint32_t* out, int clear, const char* w
 }
 
 void set_last_error(const char* what, int code) {
+    // the runtime's own note of the error: left there, the check after the next launch would report it again
+    (void)cudaGetLastError();
     g_last_error = what;
     if (code) {
         g_last_error += ": ";

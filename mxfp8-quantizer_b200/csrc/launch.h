@@ -86,7 +86,7 @@ int ready_device(int* sm_count, unsigned int** status);
 // guards fire; the product build ignores the window.
 StoreWindow make_window(void* base, int64_t bytes);
 
-// Records the CUDA error text for mxfp8_last_error() on this host thread.
+// Records the CUDA error text for mxfp8_last_error() on this host thread, and clears the runtime's own note of it.
 void set_last_error(const char* what, int code);
 
 // Key of the CUDA context current on this host thread, unique for the
