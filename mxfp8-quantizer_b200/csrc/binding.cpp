@@ -106,10 +106,8 @@ struct Payload {
     int64_t rows, cols, ld;
 };
 
-// Row stride, also of a matrix whose single row carries none.
-int64_t row_stride(const Tensor& t) {
-    return t.size(0) > 1 ? t.stride(0) : std::max(t.stride(0), t.size(1));
-}
+// Row stride; a single row's own means nothing, and may be any number.
+int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
 Payload payload(const char* name, const Tensor& q) {
     const auto type = q.scalar_type();
