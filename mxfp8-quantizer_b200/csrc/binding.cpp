@@ -188,9 +188,12 @@ Tensor gemm_mxfp4(const Tensor& a_q, const Tensor& b_q, const Tensor& a_s, const
 // ---------------------------------------------------------------------------
 
 mxfp8_cache describe(const Tensor& k, const Tensor& v, const Tensor& k_scales, const Tensor& v_scales) {
-    TORCH_CHECK_VALUE(k.dim() == 4 && k.element_size() == 1 && v.element_size() == 1 && v.sizes() == k.sizes(),
-                      "k and v must be (num_pages, heads, page_size, dim) bytes, got ", k.sizes(), " ", k.scalar_type(),
-                      " and ", v.sizes(), " ", v.scalar_type());
+    auto e4m3 = [](const Tensor& t) {  // or its bytes; another 8-bit format would be misread
+        return t.scalar_type() == at::kFloat8_e4m3fn || t.scalar_type() == at::kByte || t.scalar_type() == at::kChar;
+    };
+    TORCH_CHECK_VALUE(k.dim() == 4 && e4m3(k) && e4m3(v) && v.sizes() == k.sizes(),
+                      "k and v must be (num_pages, heads, page_size, dim) float8_e4m3fn or bytes, got ", k.sizes(), " ",
+                      k.scalar_type(), " and ", v.sizes(), " ", v.scalar_type());
     const int64_t dim = k.size(3);
     for (const Tensor* s : {&k_scales, &v_scales}) {
         TORCH_CHECK_VALUE(dim % 32 == 0 && s->dim() == 4 && s->size(0) == k.size(0) && s->size(1) == k.size(1) &&

@@ -23,3 +23,22 @@ def test_read_refuses_an_output_that_is_not_a_whole_pair(which):
         pkg.cache_read(cache, table, starts, 8, out=pair)
     with pytest.raises(ValueError, match="CUDA"):                # a whole pair gets as far as the device
         pkg.cache_read(cache, table, starts, 8, out=(good, good.clone()))
+
+
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("dtype", [torch.float8_e5m2, torch.float8_e4m3fnuz, torch.float8_e8m0fnu, torch.bool])
+def test_cache_refuses_other_8_bit_formats(which, dtype):
+    """Their bytes would be read as E4M3."""
+    cache = pkg.allocate_cache(4, 16, 2, 64, device="cpu")
+    other = cache._replace(**{which: getattr(cache, which).view(torch.uint8).view(dtype)})
+    rows, slots = torch.zeros((5, 2, 64), dtype=torch.bfloat16), torch.arange(5)
+    table, lengths = torch.zeros((3, 4), dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    for call in (lambda: pkg.cache_write(other, rows, rows, slots),
+                 lambda: pkg.cache_read(other, table, torch.zeros(4, dtype=torch.int32), 8),
+                 lambda: pkg.cache_attention(rows[:3], other, table, lengths)):
+        with pytest.raises(ValueError, match="e4m3"):
+            call()
+    for view in (torch.uint8, torch.int8):                       # bytes are taken as they are
+        same = cache._replace(**{which: getattr(cache, which).view(view)})
+        with pytest.raises(ValueError, match="CUDA"):
+            pkg.cache_write(same, rows, rows, slots)
