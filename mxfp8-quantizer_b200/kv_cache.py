@@ -39,10 +39,14 @@ class MXFP8Cache(NamedTuple):
 
 
 def allocate_cache(num_pages: int, page_size: int, heads: int, dim: int, device=None) -> MXFP8Cache:
-    """An empty cache (zeros).  page_size is a power of two, dim a multiple of 32."""
-    if num_pages < 0 or heads < 1 or page_size < 1 or page_size & (page_size - 1) or dim < 32 or dim % SCALE_BLOCK:
-        raise ValueError(f"a cache needs page_size a power of two, heads >= 1 and dim a multiple of 32, got "
-                         f"num_pages={num_pages}, page_size={page_size}, heads={heads}, dim={dim}")
+    """An empty cache (zeros).  page_size is a power of two up to 4096, dim a
+    multiple of 32 up to 1024, heads at most 65536, and num_pages * heads *
+    page_size below 2^32."""
+    if (num_pages < 0 or not 1 <= heads <= 65536 or not 1 <= page_size <= 4096 or page_size & (page_size - 1)
+            or not 32 <= dim <= 1024 or dim % SCALE_BLOCK or num_pages * heads * page_size >= 2 ** 32):
+        raise ValueError(f"a cache needs page_size a power of two up to 4096, heads from 1 to 65536, dim a multiple of 32 "
+                         f"up to 1024 and num_pages * heads * page_size below 2^32, got num_pages={num_pages}, "
+                         f"page_size={page_size}, heads={heads}, dim={dim}")
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     shape = (num_pages, heads, page_size)
     k, v = (torch.zeros((*shape, dim), dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2))

@@ -42,3 +42,17 @@ def test_cache_refuses_other_8_bit_formats(which, dtype):
         same = cache._replace(**{which: getattr(cache, which).view(view)})
         with pytest.raises(ValueError, match="CUDA"):
             pkg.cache_write(same, rows, rows, slots)
+
+
+@pytest.mark.parametrize("sizes", [(1, 8192, 1, 64), (1, 16, 65537, 32), (1, 16, 1, 1056), (1, 16, 1, 2048),
+                                   (2 ** 28, 16, 1, 32), (2 ** 20, 4096, 2, 32)])
+def test_allocate_cache_refuses_what_every_call_would(sizes):
+    """Before any memory is taken: these sizes were allocated, and each call on them then refused."""
+    with pytest.raises(ValueError, match="a cache needs"):
+        pkg.allocate_cache(*sizes, device="meta")
+
+
+@pytest.mark.parametrize("sizes", [(1, 4096, 1, 32), (1, 1, 65536, 32), (1, 16, 1, 1024), (2 ** 28 - 1, 16, 1, 32), (0, 16, 2, 64)])
+def test_allocate_cache_takes_the_limits(sizes):
+    cache = pkg.allocate_cache(*sizes, device="meta")
+    assert cache.k.shape == (sizes[0], sizes[2], sizes[1], sizes[3])
