@@ -111,3 +111,17 @@ def test_a_decode_step_of_a_layer():
         out = check_elements(q.view(batch, heads * group, dim), cache, table, [step + 1] * batch, page)
         x = out.reshape(batch, -1)[:, :width] + x * 0.5
     assert capi.device_status() == 0
+
+
+def test_attention_of_several_tokens_a_sequence():
+    """Drafted tokens as rows of one batch: a sequence's table row repeated, the lengths rising by one."""
+    page, tokens = 16, 5
+    q, cache, table = attention_case([37, 300], page, 2, 4, 128, "bf16", seed=21)
+    g = torch.Generator(device="cuda").manual_seed(22)
+    q = torch.randn((2 * tokens, 8, 128), device="cuda", generator=g).bfloat16()
+    rows = table.repeat_interleave(tokens, 0)
+    check_elements(q, cache, rows, [33 + t for t in range(tokens)] + [296 + t for t in range(tokens)], page)
+    one = table[:1].expand(tokens, -1)                          # a row given once for all
+    lens = torch.tensor([33 + t for t in range(tokens)], dtype=torch.int32, device="cuda")
+    assert torch.equal(pkg.cache_attention(q[:tokens], cache, one, lens),
+                       pkg.cache_attention(q[:tokens], cache, rows[:tokens].contiguous(), lens))
