@@ -81,7 +81,7 @@ MXFP8_API int64_t mxfp8_cache_attention_workspace(const mxfp8_cache* cache, int6
  * one, whichever is more, whatever the scales of V's blocks are (V more than
  * 2^70 below its head's sums so far counts as zero); outputs are rounded once.  A score
  * overflows where a K block's scale is 2^96 or more (the query is held with its
- * largest element near 2^14).  workspace is 16-byte aligned scratch of
+ * largest element near 2^14; elements 2^28 below it lose bits).  workspace is 16-byte aligned scratch of
  * one call at a time; its contents do not matter before or after. */
 MXFP8_API int mxfp8_cache_attention(const mxfp8_cache* cache, const void* q, int64_t q_batch_stride,
                                     int64_t q_head_stride, int dtype, int64_t batch, int64_t q_heads,

@@ -1,15 +1,17 @@
 // cache_attention.cu -- one query token per sequence against the paged MXFP8
 // cache: o = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q . k_j).
 //
-// Every cached byte is read once and used by the G query heads that share a KV
-// head: 4 G operations for 1 + 1/32 bytes, so HBM bandwidth bounds it as long
-// as the arithmetic keeps up.  Tensor cores do both products (mma m16n8k16,
+// A cached byte is used by the G query heads that share a KV head: 4 G
+// operations for 1 + 1/32 bytes, so HBM bandwidth bounds it as long as the
+// arithmetic keeps up.  It is fetched once by each pass over up to 8 or 16 of
+// those heads (row_tiles).  Tensor cores do both products (mma m16n8k16,
 // f16 operands, f32 sums): an E4M3 value is exact in f16, so the payload needs
 // one conversion and the scales stay outside the products:
 //   q . k_j = sum over blocks of 32 of  2^(sk - 127) (q . payload), a sum per
 //     block scaled in f32.  q is brought to f16 with one power of two a head
-//     (largest element in [2^14, 2^15)): a bf16 or fp16 value is exact there
-//     down to 2^-38 of the head's largest.
+//     (largest element in [2^14, 2^15)): a bf16 value is exact there down to
+//     2^-31 of the head's largest, an fp16 value down to 2^-28, and a smaller
+//     one is off by 2^-39 of the largest at most.
 //   sum_j p_j v_j: the operand is p_j 2^(sv - R + 15), for the V scale bytes sv
 //     in the window R - 11 .. R.  It is two f16, p_j 2^15 and what that leaves,
 //     each times the power of two: 2^-22 of relative error at most, or 2^-28 of
@@ -42,7 +44,7 @@
 // warp's tile takes about 1.7 us either way, and eight warps an SM are what the
 // registers allow (12 or 16 with fewer registers, tiles of 16 positions for
 // D <= 128, a third stage for D = 256: all slower).  Half of the issue slots are
-// used (ncu), no pipe above 44 %.  K as E4M3 operands (m16n8k32), the query split
+// used (ncu), no pipe above 41 %.  K as E4M3 operands (m16n8k32), the query split
 // into E4M3 pieces of 4 bits, saves the conversions of K and half of the products
 // but was no faster with two pieces (49.7 us), which do not hold every query, and
 // slower with the four that do (57.7 us; 8 of 65536: 75 us).
@@ -84,7 +86,11 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr uint32_t kNoRow32 = 0xFFFFFFFFu;
 
 // Heads in groups of 8 * NT rows: 16 where that saves a second pass over K and
-// V and the accumulators fit the registers.
+// V and the accumulators fit the registers.  Each pass is work of its own, so
+// the cache is fetched once a pass, in part from L2.  8 sequences of up to 16384,
+// one KV head: D = 256, 8 heads 20.8 us, 16 (two passes) 25.4; D = 128, 16 heads
+// 17.0 (two passes of 8: 16.5), 24 heads 19.7 (three: 19.2), 64 heads 27.3
+// (eight: 32.4).  16 of up to 65536, 16 heads 41.4 (two of 8: 56.7), 32 heads 69.4 (100).
 inline int row_tiles(int dim, int group) { return group > 8 && dim <= 128 ? 2 : 1; }
 
 template <int D, int NT>

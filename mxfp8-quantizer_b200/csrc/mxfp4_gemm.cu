@@ -22,11 +22,11 @@
 //   the result does not depend on timing.
 //
 // Measured, bf16 out: 8192x8192x8192 187 us = 5.9 PFLOP/s for a burst, 216 us
-// under the power cap; 4096x4096x4096 29.5 us = 4.7.  One pair a tile leaves the
+// under the power cap; 4096x4096x4096 29.1 us = 4.7.  One pair a tile leaves the
 // tensor cores waiting while its accumulators are read (256 + 48 of 512 columns
 // of tensor memory: no second set fits): 8192x4096x1024 22.8 us = 3.0 PFLOP/s.
-// One token through 16384x8192 14.8 us = 4.8 TB/s, through 4096x4096 5.7 us =
-// 1.6 TB/s: there the launch, the first loads and the join of the split take
+// One token through 16384x8192 16.1 us = 4.4 TB/s (matrices in turn, from HBM),
+// through 4096x4096 5.7 us = 1.6 TB/s: there the launch, the first loads and the join of the split take
 // longer than the stream.  Loops of a whole warp with one elected lane issue a
 // stage's instructions in about a tenth of the cycles that a one-lane branch
 // takes: 8192x8192x8192 was 348 us with those.
@@ -673,7 +673,9 @@ int launch_wide(const Fp4GemmArgs& g, int sm_count, cudaStream_t stream) {
 }
 
 // CTAs of a narrow tile's cluster: doubled while they fit the SMs and each
-// keeps two stages.
+// keeps two stages.  With one stage a CTA the join costs more than the stage
+// saves: 77x1000x2080 7.6 us with 4 CTAs, 8.3 with 8; 64x512x2048 5.7 and 7.5,
+// 16x1000x2048 5.2 and 5.9; only 1x1024x1024 gains, 4.5 and 4.3.
 int narrow_split(int64_t tiles, int n_stages, int sm_count) {
     int split = 1;
     while (split < 8 && tiles * split * 2 <= sm_count && n_stages >= 4 * split) split *= 2;
