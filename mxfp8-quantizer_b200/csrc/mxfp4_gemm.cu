@@ -449,7 +449,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide::threads, 1)
         }
         mbar_init(acc_full, 1);
         mbar_init(acc_empty, 2 * C::epi_warps);           // used in the even CTA: both CTAs' readers
-        mbar_init(drained, 1);                            // waited for in the even CTA, which issues for both
+        mbar_init(drained, 1);                            // committed by the even CTA in both
         ctl[0] = 0;
         fence_mbar_init();
     }
@@ -530,12 +530,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide::threads, 1)
                 __syncwarp();
             }
         }
-        // as in the narrow form; the other CTA frees its tensor memory after the cluster barrier that follows
-        if (rank == 0) {
-            if (elect_one()) tcgen05_commit<2>(drained);
-            __syncwarp();
-            mbar_wait_bounded(drained, 0, kWaitNs);
-        }
+        // as in the narrow form; it arrives in both CTAs, and each waits for its own below
+        if (rank == 0 && elect_one()) tcgen05_commit<2>(drained);
+        __syncwarp();
     } else {
         // two warps for each quarter of the lanes, 128 columns each
         const int q4 = warp & 3, col0 = (warp >> 2) * 128;
@@ -575,7 +572,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide::threads, 1)
             }
         }
     }
-    if (warp == kLoadWarp) drain_stages<C::stages>(full0, empty0, issued, ctl, p.status);
+    if (warp == kLoadWarp) {
+        drain_stages<C::stages>(full0, empty0, issued, ctl, p.status);
+        mbar_wait_bounded(drained, 0, kWaitNs);  // the last arrival from the even CTA: none comes after this one has gone
+    }
     __syncwarp();
     tcgen05_fence_before();
     __syncthreads();

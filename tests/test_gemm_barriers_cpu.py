@@ -64,3 +64,12 @@ def test_both_forms_wait_for_it_whatever_happened():
     assert text.count("mbar_init(drained, 1)") == 2 and text.count("mbar_wait_bounded(drained, 0, kWaitNs)") == 2
     assert text.count("tcgen05_commit<1>(drained)") == 1 and text.count("tcgen05_commit<2>(drained)") == 1
     assert "if (ctl[0])" not in text
+
+
+def test_each_cta_of_a_pair_waits_for_its_own_arrival():
+    """The even CTA's commit arrives in both: a CTA that left without waiting could be gone when it does."""
+    text = (ROOT / "mxfp8-quantizer_b200" / "csrc" / "mxfp4_gemm.cu").read_text()
+    wide = text[text.index("mxfp4_gemm_wide_kernel("):]
+    wait = wide[:wide.index("mbar_wait_bounded(drained, 0, kWaitNs)")]
+    last = [line.strip() for line in wait.splitlines() if line.strip()][-2:]
+    assert last[0] == "if (warp == kLoadWarp) {" and last[1].startswith("drain_stages<")
