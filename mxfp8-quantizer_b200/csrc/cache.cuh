@@ -11,12 +11,6 @@ namespace mxfp8 {
 
 constexpr unsigned kErrCacheIndex = 64u;  // device status bit: an index was not followed
 
-// 2^(byte - 127): byte 0 is subnormal, 255 is NaN.
-__device__ __forceinline__ float ue8m0_value(uint32_t byte) {
-    const uint32_t bits = byte == 0u ? 0x00400000u : byte << 23;
-    return __uint_as_float(byte == 255u ? 0x7FC00000u : bits);
-}
-
 // Eight 16-bit values at p; 16-byte load where `vec` says it is aligned.
 __device__ __forceinline__ uint4 load8(const uint16_t* p, bool vec) {
     if (vec) return __ldcs(reinterpret_cast<const uint4*>(p));

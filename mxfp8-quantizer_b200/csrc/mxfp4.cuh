@@ -57,10 +57,4 @@ __device__ __forceinline__ void e2m1x8_to_half2(uint32_t codes, uint32_t (&h)[4]
         : "r"(codes));
 }
 
-// 2^(byte - 127) as f32: byte 0 is subnormal, 255 is NaN.
-__device__ __forceinline__ float fp4_scale_value(uint32_t byte) {
-    const uint32_t bits = byte == 0u ? 0x00400000u : byte << 23;
-    return __uint_as_float(byte == 255u ? 0x7FC00000u : bits);
-}
-
 }  // namespace mxfp8

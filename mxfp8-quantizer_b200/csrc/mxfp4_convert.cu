@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(kConvertThreads) mxfp4_dequantize_kernel(
     for (int i = 0; i < kRowsPerWarp; ++i) {
         const int64_t row = u.row0 + 32 * i;
         if (row >= rows) return;
-        const float scale = fp4_scale_value((sw[i] >> (8 * ((lane >> 2) & 3))) & 0xFFu);
+        const float scale = ue8m0_value((sw[i] >> (8 * ((lane >> 2) & 3))) & 0xFFu);
         uint32_t h[4];
         e2m1x8_to_half2(codes[i], h);
         float v[8];

@@ -55,6 +55,12 @@ __device__ __forceinline__ void scale_from_amax(uint32_t amax_bits, uint32_t& by
     inv = __uint_as_float((254u - e) << 23);
 }
 
+// 2^(byte - 127) as f32: byte 0 is subnormal, 255 is NaN.
+__device__ __forceinline__ float ue8m0_value(uint32_t byte) {
+    const uint32_t bits = byte == 0u ? 0x00400000u : byte << 23;
+    return __uint_as_float(byte == 255u ? 0x7FC00000u : bits);
+}
+
 // Two f32 -> two E4M3 bytes; `lo` lands in the low byte.
 __device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) {
     uint16_t r;
